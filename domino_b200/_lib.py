@@ -24,6 +24,9 @@ DD_F32 = 2
 DD_STATUS_TIMEOUT = 1
 DD_STATUS_BAD_TOKEN = 2
 DD_STATUS_NO_ARGMAX = 4
+DD_STATUS_NO_PAGE = 8
+DD_STATUS_BAD_ROW = 16
+DD_STATUS_SHARED_PAGE = 32
 # dd_set_middle kinds (include/domino_draft.h)
 DD_MIDDLE_SILU, DD_MIDDLE_IDENTITY, DD_MIDDLE_RELU, DD_MIDDLE_GELU = 0, 1, 2, 3
 DD_MIDDLE_GELU_TANH, DD_MIDDLE_TANH, DD_MIDDLE_SIGMOID, DD_MIDDLE_SILU_ROUNDED = 4, 5, 6, 7
@@ -35,6 +38,8 @@ EXPORTS = (
     "dd_get_exchange_buffer", "dd_ipc_export", "dd_ipc_open", "dd_ipc_close", "dd_set_vocab_shard",
     "dd_set_exchange_timeout", "dd_verify_accept", "dd_set_weight_layout", "dd_set_rollout_mode",
     "dd_set_trace", "dd_set_middle",
+    "dd_pages_scratch", "dd_pages_reserve", "dd_pages_crop", "dd_pages_fork", "dd_pages_compact",
+    "dd_cache_write", "dd_cache_attend_workspace", "dd_cache_attend",
 )
 PHASES = {1: "z", 2: "zlm", 3: "gh", 4: "sgh", 5: "fc2", 6: "table", 7: "cell", 8: "gather", 9: "rollout"}
 
@@ -67,6 +72,27 @@ class DDWeights(ctypes.Structure):
 
 class DDTrace(ctypes.Structure):
     _fields_ = [("z", ctypes.c_void_p), ("h", ctypes.c_void_p), ("gh", ctypes.c_void_p), ("s", ctypes.c_void_p)]
+
+
+class DDPagedCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("data", "table", "length", "refs", "scratch", "status")] + [
+        (n, ctypes.c_int32) for n in ("layers", "batch", "kv_heads", "pages", "page_size", "head_dim", "row_pages",
+                                      "dtype", "device")]
+
+
+class DDCacheWriteArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, ctypes.c_void_p) for n in ("start", "lens", "q_norm", "k_norm", "inv_freq")]
+                + [("eps", ctypes.c_float), ("factor", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("layer", "tokens", "heads", "rotary", "interleaved")])
+
+
+class DDCacheAttendArgs(ctypes.Structure):
+    _fields_ = ([("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 3)]
+                + [(n, ctypes.c_void_p) for n in ("start", "lens", "workspace")]
+                + [("workspace_bytes", ctypes.c_uint64), ("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("layer", "tokens", "heads", "causal", "window", "sinks")])
 
 
 class DominoDraftError(RuntimeError):
@@ -119,6 +145,15 @@ def load() -> ctypes.CDLL:
         lib.dd_set_trace.argtypes = [vp, ctypes.POINTER(DDTrace)]
         lib.dd_set_middle.argtypes = [vp, ctypes.c_int]
         lib.dd_read_timing.argtypes = [vp, vp, vp, i32]
+        cache, u64p = ctypes.POINTER(DDPagedCache), ctypes.POINTER(ctypes.c_uint64)
+        lib.dd_pages_scratch.argtypes = [cache, u64p]
+        lib.dd_pages_reserve.argtypes = [cache, vp, vp]
+        lib.dd_pages_crop.argtypes = [cache, vp, vp]
+        lib.dd_pages_fork.argtypes = [cache, vp, vp]
+        lib.dd_pages_compact.argtypes = [cache, vp]
+        lib.dd_cache_write.argtypes = [cache, ctypes.POINTER(DDCacheWriteArgs), vp]
+        lib.dd_cache_attend_workspace.argtypes = [cache, ctypes.POINTER(DDCacheAttendArgs), u64p]
+        lib.dd_cache_attend.argtypes = [cache, ctypes.POINTER(DDCacheAttendArgs), vp]
         for name in EXPORTS:
             if name not in ("dd_last_error", "dd_version"):
                 getattr(lib, name).restype = ctypes.c_int

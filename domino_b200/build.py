@@ -16,11 +16,11 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC_DIR = os.path.join(HERE, "csrc")
-SOURCES = [os.path.join(SRC_DIR, "dd_api.cu")]
+SOURCES = [os.path.join(SRC_DIR, "dd_api.cu"), os.path.join(SRC_DIR, "dd_paged.cu")]
 DEPS = [os.path.join(SRC_DIR, f) for f in os.listdir(SRC_DIR)] + [os.path.join(ROOT, "include", "domino_draft.h")]
 OUT = os.path.join(HERE, "libdomino_draft.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-O2", "-Xptxas", "-v"]
+FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0", "-Xcompiler", "-fPIC,-O2", "-Xptxas", "-v"]
 
 
 def nvcc() -> str:

@@ -30,6 +30,7 @@
 
 #include "../../include/domino_draft.h"
 #include "dd_cell.cuh"
+#include "dd_common.h"
 #include "dd_gemv.cuh"
 #include "dd_gemv_f32.cuh"
 #include "dd_rollout.cuh"
@@ -168,6 +169,19 @@ int fail(dd_handle* h, int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+
+}  // namespace
+
+// The reason of the last failing call without a handle, for the library's other source file.
+int dd::global_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_global_error, sizeof(g_global_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+namespace {
 
 #define DD_CUDA(h, call)                                                                   \
   do {                                                                                     \

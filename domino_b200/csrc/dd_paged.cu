@@ -1,0 +1,350 @@
+// dd_paged.cu -- host side of the paged key / value cache: argument checks,
+// launches, and the C ABI (dd_pages_*, dd_cache_*) of include/domino_draft.h.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+
+#include "../../include/domino_draft.h"
+#include "dd_attend.cuh"
+#include "dd_cache_write.cuh"
+#include "dd_common.h"
+#include "dd_pages.cuh"
+#include "dd_ptx.cuh"
+
+using namespace dd;
+
+namespace {
+
+int ceil_div(long long x, long long m) { return (int)((x + m - 1) / m); }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+#define DD_TRY(call)                                                                                   \
+  do {                                                                                                 \
+    cudaError_t e_ = (call);                                                                           \
+    if (e_ != cudaSuccess) return global_fail(DD_ECUDA, "%s: %s", #call, cudaGetErrorString(e_));      \
+  } while (0)
+
+// Makes the cache's device current for one call and puts the caller's back.
+struct DeviceScope {
+  int prev = -1;
+  bool ok = false, moved = false;
+  explicit DeviceScope(int device) {
+    ok = cudaGetDevice(&prev) == cudaSuccess;
+    if (ok && prev != device) ok = moved = cudaSetDevice(device) == cudaSuccess;
+  }
+  ~DeviceScope() {
+    if (moved) cudaSetDevice(prev);
+  }
+};
+
+struct DeviceInfo {
+  int sms = 0, major = 0;
+};
+// Properties of a device, read once.
+int device_info(int device, DeviceInfo* out) {
+  static DeviceInfo known[64];
+  if (device < 0 || device >= 64) return global_fail(DD_EINVAL, "device %d", device);
+  DeviceInfo d = known[device];
+  if (!d.sms) {
+    DD_TRY(cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, device));
+    DD_TRY(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
+    known[device] = d;
+  }
+  if (d.major != 10) return global_fail(DD_EUNSUPPORTED, "device %d is not sm_100; this library is built for sm_100a", device);
+  *out = d;
+  return DD_OK;
+}
+
+int elem_size(int dtype) { return dtype == DD_F32 ? 4 : 2; }
+
+// Shape checks that need no device.
+int check_shape(const dd_paged_cache* c) {
+  if (!c) return global_fail(DD_EINVAL, "null cache");
+  if (c->layers < 1 || c->batch < 1 || c->kv_heads < 1 || c->pages < 1 || c->row_pages < 1)
+    return global_fail(DD_EINVAL, "paged cache: layers, batch, kv_heads, pages and row_pages must be positive");
+  if (c->batch > kMaxCacheBatch) return global_fail(DD_EINVAL, "paged cache: batch %d above %d", c->batch, kMaxCacheBatch);
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return global_fail(DD_EINVAL, "paged cache: page_size %d is not 16, 32, 64 or 128", c->page_size);
+  if (c->head_dim < 8 || c->head_dim % 8 || c->head_dim > kMaxHeadDim)
+    return global_fail(DD_EINVAL, "paged cache: head_dim %d is not a multiple of 8 up to %d", c->head_dim, kMaxHeadDim);
+  if (c->dtype != DD_BF16 && c->dtype != DD_FP16 && c->dtype != DD_F32)
+    return global_fail(DD_EINVAL, "paged cache: dtype must be DD_BF16, DD_FP16 or DD_F32");
+  if ((long long)c->pages * c->kv_heads > 0x7fffffffll)
+    return global_fail(DD_EINVAL, "paged cache: pages x kv_heads must stay below 2^31");
+  if ((long long)c->batch * c->row_pages > 0x7fffffffll)
+    return global_fail(DD_EINVAL, "paged cache: batch x row_pages must stay below 2^31");
+  return DD_OK;
+}
+
+int check_cache(const dd_paged_cache* c) {
+  int rc = check_shape(c);
+  if (rc) return rc;
+  if (!c->data || !c->table || !c->length || !c->refs || !c->scratch || !c->status)
+    return global_fail(DD_EINVAL, "paged cache: null pointer");
+  if (!aligned16(c->data) || !aligned16(c->scratch))
+    return global_fail(DD_EINVAL, "paged cache: data and scratch must be 16-byte aligned");
+  return DD_OK;
+}
+
+long long plane_bytes(const dd_paged_cache* c) {
+  return (long long)c->pages * c->kv_heads * c->page_size * c->head_dim * elem_size(c->dtype);
+}
+char* plane(const dd_paged_cache* c, int layer, int kv) {
+  return static_cast<char*>(c->data) + (2ll * layer + kv) * plane_bytes(c);
+}
+
+// Launch with programmatic stream serialisation: the kernel may be scheduled
+// while its predecessor drains; every kernel here waits for it first thing.
+template <typename... K, typename... A>
+int launch(const char* what, void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, void* stream, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+  if (e != cudaSuccess) return global_fail(DD_ECUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return DD_OK;
+}
+
+long long* ll(int64_t* p) { return reinterpret_cast<long long*>(p); }
+const long long* ll(const int64_t* p) { return reinterpret_cast<const long long*>(p); }
+
+// The planned moves' pages; with `remap` also the table entries that follow them.
+int copy_pages(const dd_paged_cache* c, const PageScratch& s, const DeviceInfo& dev, bool remap, void* stream) {
+  const long long words = (long long)c->kv_heads * c->page_size * c->head_dim * elem_size(c->dtype) / 16;
+  return launch("page copy", pages_copy_kernel, dim3(dev.sms * 8), dim3(kCopyThreads), 0, stream,
+                static_cast<uint4*>(c->data), s, 2 * c->layers, c->pages, words, remap ? c->table : nullptr,
+                c->batch * c->row_pages);
+}
+
+struct PageCall {
+  DeviceInfo dev;
+  PageScratch s;
+};
+int page_call(const dd_paged_cache* c, const void* arg, const char* what, const DeviceScope& scope, PageCall* p) {
+  if (!arg) return global_fail(DD_EINVAL, "%s: null argument", what);
+  if (!scope.ok) return global_fail(DD_ECUDA, "%s: cannot select device %d", what, c->device);
+  p->s = page_scratch(c->scratch, c->pages, c->batch);
+  return device_info(c->device, &p->dev);
+}
+
+template <typename T, int kGroup, bool kVec>
+int launch_write(const WriteParams& p, int batch, int tokens_per_cta, bool interleaved, void* stream) {
+  const int half = p.rotary / 2;
+  const int pairs = interleaved ? 2 : half % 8 == 0 ? 0 : 1;
+  size_t smem = sizeof(float) * 2 * tokens_per_cta * half;
+  if (pairs == 1) smem += sizeof(float) * (kWriteThreads / kGroup) * p.dim;
+  const dim3 grid(ceil_div(p.tokens, tokens_per_cta), batch);
+  auto kernel = pairs == 0   ? cache_write_kernel<T, kGroup, 0, kVec>
+                : pairs == 1 ? cache_write_kernel<T, kGroup, 1, kVec>
+                             : cache_write_kernel<T, kGroup, 2, kVec>;
+  return launch("cache write", kernel, grid, dim3(kWriteThreads), smem, stream, p, tokens_per_cta);
+}
+
+template <typename T, bool kVec>
+int launch_write(const WriteParams& p, int batch, int tokens_per_cta, bool interleaved, void* stream) {
+  const int lanes = p.dim / 8;
+  if (lanes <= 4) return launch_write<T, 4, kVec>(p, batch, tokens_per_cta, interleaved, stream);
+  if (lanes <= 8) return launch_write<T, 8, kVec>(p, batch, tokens_per_cta, interleaved, stream);
+  if (lanes <= 16) return launch_write<T, 16, kVec>(p, batch, tokens_per_cta, interleaved, stream);
+  return launch_write<T, 32, kVec>(p, batch, tokens_per_cta, interleaved, stream);
+}
+
+template <typename T>
+int launch_write(const WriteParams& p, int batch, int tokens_per_cta, bool interleaved, bool vec, void* stream) {
+  return vec ? launch_write<T, true>(p, batch, tokens_per_cta, interleaved, stream)
+             : launch_write<T, false>(p, batch, tokens_per_cta, interleaved, stream);
+}
+
+int check_attend(const dd_paged_cache* c, const dd_cache_attend_args* a) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  if (!a) return global_fail(DD_EINVAL, "cache attend: null argument");
+  if (a->layer < 0 || a->layer >= c->layers) return global_fail(DD_EINVAL, "cache attend: layer %d of %d", a->layer, c->layers);
+  if (a->tokens < 1) return global_fail(DD_EINVAL, "cache attend: %d tokens", a->tokens);
+  if (a->heads < 1 || a->heads % c->kv_heads)
+    return global_fail(DD_EINVAL, "cache attend: %d query heads for %d key heads", a->heads, c->kv_heads);
+  if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return global_fail(DD_EINVAL, "cache attend: scale must be positive");
+  if (a->window < 0 || a->sinks < 0 || (a->window == 0 && a->sinks > 0) || (a->window > 0 && !a->causal))
+    return global_fail(DD_EINVAL, "cache attend: a window needs causal attention, sinks need a window");
+  if ((long long)a->tokens * (a->heads / c->kv_heads) > 0x3fffffffll || (long long)a->heads * c->head_dim > 0x7fffffffll)
+    return global_fail(DD_EINVAL, "cache attend: chunk too large");
+  return DD_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dd_pages_scratch(const dd_paged_cache* c, uint64_t* bytes) {
+  int rc = check_shape(c);
+  if (rc) return rc;
+  if (!bytes) return global_fail(DD_EINVAL, "null argument");
+  *bytes = page_scratch_bytes(c->pages, c->batch, c->row_pages);
+  return DD_OK;
+}
+
+int dd_pages_reserve(const dd_paged_cache* c, const int64_t* upto, void* stream) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  DeviceScope scope(c->device);
+  PageCall p;
+  if ((rc = page_call(c, upto, "dd_pages_reserve", scope, &p))) return rc;
+  rc = launch("reserve", pages_reserve_kernel, dim3(1), dim3(kPlanThreads), 0, stream, c->table, ll(c->length), c->refs,
+              p.s, c->status, ll(upto), c->batch, c->pages, c->page_size, c->row_pages);
+  return rc ? rc : copy_pages(c, p.s, p.dev, false, stream);
+}
+
+int dd_pages_crop(const dd_paged_cache* c, const int64_t* to, void* stream) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  DeviceScope scope(c->device);
+  PageCall p;
+  if ((rc = page_call(c, to, "dd_pages_crop", scope, &p))) return rc;
+  return launch("crop", pages_crop_kernel, dim3(c->batch), dim3(256), 0, stream, c->table, ll(c->length), c->refs,
+                ll(to), c->pages, c->page_size, c->row_pages);
+}
+
+int dd_pages_fork(const dd_paged_cache* c, const int64_t* src, void* stream) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  DeviceScope scope(c->device);
+  PageCall p;
+  if ((rc = page_call(c, src, "dd_pages_fork", scope, &p))) return rc;
+  const int blocks = std::min(ceil_div((long long)c->batch * c->row_pages, 1024), p.dev.sms * 2);
+  rc = launch("fork snapshot", pages_snapshot_kernel, dim3(blocks), dim3(256), 0, stream, c->table, ll(c->length), p.s,
+              c->batch, c->row_pages);
+  if (rc) return rc;
+  return launch("fork", pages_fork_kernel, dim3(c->batch), dim3(256), 0, stream, c->table, ll(c->length), c->refs, p.s,
+                c->status, ll(src), c->batch, c->pages, c->page_size, c->row_pages);
+}
+
+int dd_pages_compact(const dd_paged_cache* c, void* stream) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  DeviceScope scope(c->device);
+  PageCall p;
+  if ((rc = page_call(c, c, "dd_pages_compact", scope, &p))) return rc;
+  rc = launch("compact", pages_compact_kernel, dim3(1), dim3(kPlanThreads), 0, stream, c->refs, p.s, c->pages);
+  return rc ? rc : copy_pages(c, p.s, p.dev, true, stream);
+}
+
+int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* stream) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  if (!a || !a->k || !a->v || !a->start) return global_fail(DD_EINVAL, "dd_cache_write: null argument");
+  if (a->layer < 0 || a->layer >= c->layers) return global_fail(DD_EINVAL, "dd_cache_write: layer %d of %d", a->layer, c->layers);
+  if (a->tokens < 1) return global_fail(DD_EINVAL, "dd_cache_write: %d tokens", a->tokens);
+  if (a->q && (!a->q_out || a->heads < 1)) return global_fail(DD_EINVAL, "dd_cache_write: q needs q_out and heads");
+  if (a->q && !aligned16(a->q_out)) return global_fail(DD_EINVAL, "dd_cache_write: q_out must be 16-byte aligned");
+  if (a->rotary < 0 || a->rotary % 2 || a->rotary > c->head_dim)
+    return global_fail(DD_EINVAL, "dd_cache_write: rotary %d is not an even number up to head_dim %d", a->rotary, c->head_dim);
+  if (a->rotary && !a->inv_freq) return global_fail(DD_EINVAL, "dd_cache_write: rotary needs inv_freq");
+  if ((long long)(a->heads + 2ll * c->kv_heads) * a->tokens > 0x7fffffffll)
+    return global_fail(DD_EINVAL, "dd_cache_write: chunk too large");
+  DeviceScope scope(c->device);
+  if (!scope.ok) return global_fail(DD_ECUDA, "dd_cache_write: cannot select device %d", c->device);
+  DeviceInfo dev;
+  if ((rc = device_info(c->device, &dev))) return rc;
+  WriteParams p{};
+  const void* x[3] = {a->q, a->k, a->v};
+  const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
+  const int per16 = 16 / elem_size(c->dtype);
+  bool vec = true;
+  for (int i = 0; i < 3; ++i) {
+    p.x[i] = x[i];
+    if (!x[i]) continue;
+    vec = vec && aligned16(x[i]);
+    for (int k = 0; k < 3; ++k) {
+      p.stride[i][k] = st[i][k];
+      vec = vec && st[i][k] % per16 == 0;
+    }
+  }
+  const void* norm[2] = {a->q_norm, a->k_norm};
+  for (int i = 0; i < 2; ++i) {
+    p.norm[i] = norm[i];
+    vec = vec && (!norm[i] || aligned16(norm[i]));
+    p.pool[i] = plane(c, a->layer, i);
+  }
+  p.q_out = a->q_out;
+  p.table = c->table;
+  p.refs = c->refs;
+  p.status = c->status;
+  p.start = ll(a->start);
+  p.lens = ll(a->lens);
+  p.inv_freq = a->inv_freq;
+  p.eps = a->eps;
+  p.factor = a->factor;
+  p.tokens = a->tokens;
+  p.heads = a->heads;
+  p.kv_heads = c->kv_heads;
+  p.dim = c->head_dim;
+  p.rotary = a->rotary;
+  p.pages = c->pages;
+  p.page_size = c->page_size;
+  p.row_pages = c->row_pages;
+  // One token a CTA until that fills the GPU several times over; then four, so
+  // that all threads have an angle to compute.
+  const int per_cta = (long long)c->batch * a->tokens > 16ll * dev.sms ? 4 : 1;
+  const bool il = a->interleaved != 0;
+  if (c->dtype == DD_F32) return launch_write<float>(p, c->batch, per_cta, il, vec, stream);
+  if (c->dtype == DD_FP16) return launch_write<__half>(p, c->batch, per_cta, il, vec, stream);
+  return launch_write<__nv_bfloat16>(p, c->batch, per_cta, il, vec, stream);
+}
+
+int dd_cache_attend_workspace(const dd_paged_cache* c, const dd_cache_attend_args* a, uint64_t* bytes) {
+  int rc = check_attend(c, a);
+  if (rc) return rc;
+  if (!bytes) return global_fail(DD_EINVAL, "null argument");
+  *bytes = 0;
+  return DD_OK;
+}
+
+int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void* stream) {
+  int rc = check_attend(c, a);
+  if (rc) return rc;
+  if (!a->q || !a->out || !a->start) return global_fail(DD_EINVAL, "dd_cache_attend: null argument");
+  if (!aligned16(a->out)) return global_fail(DD_EINVAL, "dd_cache_attend: out must be 16-byte aligned");
+  DeviceScope scope(c->device);
+  if (!scope.ok) return global_fail(DD_ECUDA, "dd_cache_attend: cannot select device %d", c->device);
+  DeviceInfo dev;
+  if ((rc = device_info(c->device, &dev))) return rc;
+  AttendParams p{};
+  p.q = a->q;
+  p.out = a->out;
+  for (int i = 0; i < 3; ++i) p.q_stride[i] = a->q_stride[i];
+  for (int i = 0; i < 2; ++i) p.pool[i] = plane(c, a->layer, i);
+  p.table = c->table;
+  p.start = ll(a->start);
+  p.lens = ll(a->lens);
+  p.scale = a->scale;
+  p.batch = c->batch;
+  p.tokens = a->tokens;
+  p.heads = a->heads;
+  p.kv_heads = c->kv_heads;
+  p.dim = c->head_dim;
+  p.pages = c->pages;
+  p.page_size = c->page_size;
+  p.row_pages = c->row_pages;
+  p.causal = a->causal != 0;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  const long long units = (long long)c->batch * a->tokens * a->heads;
+  const long long blocks = (units + kSimpleWarps - 1) / kSimpleWarps;
+  if (blocks > 0x7fffffffll) return global_fail(DD_EINVAL, "dd_cache_attend: chunk too large");
+  const dim3 grid((unsigned)blocks), block(32 * kSimpleWarps);
+  if (c->dtype == DD_F32) return launch("attend", attend_simple_kernel<float>, grid, block, 0, stream, p);
+  if (c->dtype == DD_FP16) return launch("attend", attend_simple_kernel<__half>, grid, block, 0, stream, p);
+  return launch("attend", attend_simple_kernel<__nv_bfloat16>, grid, block, 0, stream, p);
+}
+
+}  // extern "C"

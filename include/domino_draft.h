@@ -51,6 +51,10 @@ extern "C" {
 #define DD_STATUS_TIMEOUT 1u       /* a bounded wait inside a kernel gave up */
 #define DD_STATUS_BAD_TOKEN 2u     /* a token id was outside [0, vocab) and was clamped */
 #define DD_STATUS_NO_ARGMAX 4u     /* an argmax saw no candidate at all */
+/* Status bits of a paged cache (dd_paged_cache::status). */
+#define DD_STATUS_NO_PAGE 8u       /* no free page, or a position behind the row's table: the write was dropped */
+#define DD_STATUS_BAD_ROW 16u      /* dd_pages_fork: a source row outside [-1, batch); that row was left as it was */
+#define DD_STATUS_SHARED_PAGE 32u  /* dd_cache_write: a page that another row holds too; the write was dropped */
 
 /* Argmax semantics, in every kernel here: the lowest index wins a tie, and a
  * NaN of either sign ranks above every number (the first NaN wins), as
@@ -276,6 +280,105 @@ typedef struct dd_trace {
  * (one kernel per phase; the persistent rollout is not used).  NULL stops
  * tracing.  Unsharded handles only.  Slower: for tests and debugging. */
 int dd_set_trace(dd_handle* h, const dd_trace* t);
+
+/* ---- Paged key / value cache (no counterpart in the reference, whose loop
+ * keeps one contiguous cache of one sequence, code/dflash.py:359-360, 488) ----
+ *
+ * The caller owns all the memory; the struct points at it.  A page holds
+ * page_size tokens of every head of one layer's keys or values, and the same
+ * page number is used in every layer.  Row b of the batch keeps position p in
+ * page table[b, p / page_size], entry p % page_size; -1 means no page.
+ * refs[p] counts the rows that hold page p; 0 means free.  Free pages are
+ * taken lowest number first, so equal calls give equal tables.
+ *   data    [layers, 2 (keys, values), pages, kv_heads, page_size, head_dim]
+ *   scratch dd_pages_scratch bytes, used by the dd_pages_* calls only
+ *   status  one word of DD_STATUS_* bits, set by the kernels, never cleared
+ * Calls on one cache must be ordered (one stream, or events between streams).
+ * Nothing here synchronises or allocates; everything can be captured. */
+typedef struct dd_paged_cache {
+  void* data;
+  int32_t* table;      /* [batch, row_pages] */
+  int64_t* length;     /* [batch]: tokens of each row */
+  int32_t* refs;       /* [pages] */
+  void* scratch;
+  uint32_t* status;
+  int32_t layers, batch, kv_heads, pages, page_size, head_dim, row_pages;
+  int32_t dtype;       /* DD_BF16, DD_FP16 or DD_F32 */
+  int32_t device;
+} dd_paged_cache;
+
+/* Bytes of scratch that the dd_pages_* calls need (also checks the shape):
+ * page_size 16, 32, 64 or 128; head_dim a multiple of 8, at most 256; batch
+ * at most 1024. */
+int dd_pages_scratch(const dd_paged_cache* c, uint64_t* bytes);
+
+/* Make positions length[b] .. upto[b] - 1 of every row writable: missing pages
+ * are taken from the free ones, and a page that other rows hold too and that
+ * these positions reach is replaced by a copy (the first of the rows that need
+ * it keeps the original when no row outside this call holds it).  upto [batch]
+ * int64, device.  Lengths do not change. */
+int dd_pages_reserve(const dd_paged_cache* c, const int64_t* upto, void* stream);
+
+/* length[b] = min(length[b], to[b]) (at least 0); pages wholly behind it are given back. */
+int dd_pages_crop(const dd_paged_cache* c, const int64_t* to, void* stream);
+
+/* Row b becomes a copy of row src[b] as it was before the call: it shares the
+ * pages below src's length and takes its length.  src[b] = b leaves the row,
+ * -1 empties it.  The same source may be named many times.  src [batch] int64, device. */
+int dd_pages_fork(const dd_paged_cache* c, const int64_t* src, void* stream);
+
+/* Move the pages in use to the lowest numbers (contents, tables and counts);
+ * the pages behind them are all free afterwards. */
+int dd_pages_compact(const dd_paged_cache* c, void* stream);
+
+/* One layer's new tokens into the cache: token t of row b, t < lens[b], has
+ * position p = start[b] + t.
+ *   q_out = rope(norm(q, q_norm), p), K[p] = rope(norm(k, k_norm), p), V[p] = v
+ * norm(x, w) = x / sqrt(mean(x^2) + eps) * w (left out where w is NULL); rope
+ * turns pair i of the first `rotary` values by the angle p * inv_freq[i] and
+ * scales it by `factor`; the pairs are (i, i + rotary / 2), or (2 i, 2 i + 1)
+ * with `interleaved`.  All in fp32 (the angle in fp64) with one rounding.
+ * q_out rows t >= lens[b] are zero.  A position without a page of its own is
+ * not written and sets a status bit.  Strides are in elements (batch, token,
+ * head); the last dimension is contiguous.  q (then q_out) may be NULL. */
+typedef struct dd_cache_write_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;                /* [batch, tokens, heads, head_dim] */
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int64_t* start;       /* [batch] */
+  const int64_t* lens;        /* [batch], or NULL: all `tokens` */
+  const void* q_norm;         /* [head_dim] or NULL */
+  const void* k_norm;
+  const float* inv_freq;      /* [rotary / 2], NULL when rotary = 0 */
+  float eps;
+  float factor;
+  int32_t layer, tokens, heads, rotary, interleaved;
+} dd_cache_write_args;
+int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* stream);
+
+/* Attention of the new tokens over one layer of the cache.  Query t of row b,
+ * t < lens[b], has position p = start[b] + t and sees the keys j < start[b] +
+ * lens[b] that have a page, with j <= p if `causal`, and with `window` > 0
+ * (causal only) p - j < window or j < sinks:
+ *   out = sum_j softmax_j(scale q . K[j]) V[j]
+ * Query heads h * heads / kv_heads ... share key head h.  A query that sees no
+ * key, and every t >= lens[b], gives zeros.  Keys that a query does not see
+ * have no effect on it, whatever they hold. */
+typedef struct dd_cache_attend_args {
+  const void* q;
+  void* out;                  /* [batch, tokens, heads, head_dim] */
+  int64_t q_stride[3];        /* batch, token, head, in elements */
+  const int64_t* start;       /* [batch] */
+  const int64_t* lens;        /* [batch], or NULL: all `tokens` */
+  void* workspace;            /* dd_cache_attend_workspace bytes, 16-byte aligned; not shared by overlapping calls */
+  uint64_t workspace_bytes;
+  float scale;
+  int32_t layer, tokens, heads, causal, window, sinks;
+} dd_cache_attend_args;
+int dd_cache_attend_workspace(const dd_paged_cache* c, const dd_cache_attend_args* a, uint64_t* bytes);
+int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void* stream);
 
 /* Launch kinds reported by dd_read_timing. */
 #define DD_PHASE_Z 1      /* z = parallel_hiddens @ W_z^T */
