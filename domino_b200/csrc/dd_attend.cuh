@@ -20,6 +20,7 @@ struct AttendParams {
   const int* table;
   const long long* start;
   const long long* lens;     // null: all tokens
+  unsigned* status;
   float scale;
   int batch, tokens, heads, kv_heads, dim, pages, page_size, row_pages;
   int causal, window, sinks;

@@ -1,0 +1,850 @@
+// dd_attend_tc.cuh -- paged attention on the tensor cores, for 16-bit caches
+// with heads of up to 128 values.
+//
+// The query rows of one key head (token t, head g of the group: row t G + g)
+// fill the 128 rows of a tile, so a block of 16 tokens with 4 heads a group
+// reads its keys once for 64 rows.  Per tile of 128 keys:
+//
+//   S = Q K^T       tcgen05, Q and K in shared memory, S in TMEM
+//   P = e^(S - m)   one thread per row: TMEM -> registers -> TMEM (16 bits)
+//   O += P V        tcgen05, P from TMEM, V in shared memory, O in TMEM
+//
+// Two streams, each with its own S, O and four softmax warps, keep the tensor
+// cores busy while the other stream's exponentials run.  With kPair they are
+// two query tiles over the same keys (long chunks: every key tile serves 256
+// rows); without, they take alternate key tiles of one query tile and are
+// joined at the end (few rows, bound by the bytes of the cache).
+//
+// Work is cut by key tiles, not by rows: the tiles of all (row of the batch,
+// query tile, key head) items are numbered through and every CTA takes an
+// equal run of them, so long and short rows balance and one row's long cache
+// spreads over all SMs.  An item that crosses CTAs leaves its pieces
+// (unnormalised O, m, l) in the workspace and attend_join_kernel adds them in
+// the order of the CTAs: no atomics, the same result every time.  Lengths are
+// read on the device, so the cut needs no host synchronisation.
+//
+// The running maximum moves only when a row's scores pass it by more than 8
+// (as powers of two): P then stays below 2^8 and the rescaling of O, a round
+// trip through TMEM, is rare.  m, l, S and O are fp32; P is rounded to the
+// cache's type, the one rounding besides the result's (its error is that of
+// one rounding of each weight).
+//
+// A masked key has weight 0, and 0 times a NaN is NaN in a matrix product.
+// So the values of keys that no row of the item sees are set to zero in
+// shared memory (pages behind the end, missing pages, the rest of a page);
+// a tile that only some rows see is searched for infinities and NaN, and an
+// item that holds one is computed again key by key (attend_row_exact).
+#pragma once
+
+#include "dd_attend.cuh"
+
+namespace dd {
+
+constexpr int kAttThreads = 384;  // 8 softmax warps, TMA producer, MMA issuer, 2 query loaders
+constexpr int kKeyTile = 128;
+constexpr int kMaxStages = 12;
+
+struct AttendWork {
+  int4* head;    // [grid]: item {entry, key head, last CTA} whose first piece this CTA holds and does not finish; entry -1: none
+  float* o;      // [grid][2][rows][dim_pad]
+  float2* ml;    // [grid][2][rows]
+};
+template <int kDim, bool kPair>
+constexpr size_t attend_work_bytes(int grid) {
+  return (size_t)grid * (16 + 2 * (kPair ? 256 : 128) * (sizeof(float) * kDim + 8));
+}
+
+// Key tiles of one (row of the batch, query tile): n_sink from 0, then from `first` on.
+struct TileSpan {
+  int n_sink, first, n;
+  int rows;              // query rows of the batch row (tokens x group)
+  long long start, lo, hi;  // position of token 0; keys that any row of the tile sees: [lo, hi) and below sinks
+  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
+};
+__device__ inline TileSpan tile_span(const AttendParams& a, int b, int qt, int tile_rows) {
+  TileSpan s;
+  const int group = a.heads / a.kv_heads;
+  const int n_new = (int)(a.lens ? min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens);
+  s.start = a.start[b];
+  s.rows = n_new * group;
+  s.n_sink = s.first = s.n = 0;
+  s.lo = s.hi = 0;
+  const int r0 = qt * tile_rows;
+  if (r0 >= s.rows) return s;
+  const long long p0 = s.start + r0 / group, p1 = s.start + (min(s.rows, r0 + tile_rows) - 1) / group;
+  const long long total = min(max(s.start + n_new, 0ll), (long long)a.row_pages * a.page_size);
+  s.hi = a.causal ? min(total, p1 + 1) : total;
+  if (s.hi <= 0) {
+    s.hi = 0;
+    return s;
+  }
+  s.lo = a.window > 0 ? max(p0 - a.window + 1, 0ll) : 0;
+  const int t_lo = (int)(s.lo / kKeyTile), t_hi = (int)((s.hi + kKeyTile - 1) / kKeyTile);
+  const long long sinks = min(min((long long)a.sinks, s.lo), s.hi);
+  s.n_sink = min((int)((sinks + kKeyTile - 1) / kKeyTile), t_lo);
+  s.first = t_lo;
+  s.n = s.n_sink + max(t_hi - t_lo, 0);
+  return s;
+}
+
+// A CTA's run of key tiles, item by item.
+struct Piece {
+  int e, b, qt, h, i0, i1;  // entry (b, qt), key head, tiles [i0, i1) of it
+  long long unit, end;      // number of tile i0; end of the CTA's run
+  TileSpan span;
+};
+struct PieceStart {
+  long long unit, end, rem;  // rem: tiles of the entry before `unit`
+  int e;
+};
+__device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
+  p.b = p.e / q_tiles;
+  p.qt = p.e - p.b * q_tiles;
+  p.span = tile_span(a, p.b, p.qt, tile_rows);
+}
+__device__ __forceinline__ bool piece_first(const AttendParams& a, const PieceStart& s, Piece& p, int q_tiles,
+                                            int tile_rows) {
+  p.unit = s.unit;
+  p.end = s.end;
+  if (p.unit >= p.end) return false;
+  p.e = s.e;
+  piece_enter(a, p, q_tiles, tile_rows);
+  p.h = (int)(s.rem / p.span.n);
+  p.i0 = (int)(s.rem - (long long)p.h * p.span.n);
+  p.i1 = (int)min((long long)p.span.n, p.i0 + (p.end - p.unit));
+  return true;
+}
+__device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
+  p.unit += p.i1 - p.i0;
+  if (p.unit >= p.end) return false;
+  if (++p.h == a.kv_heads) {
+    p.h = 0;
+    do {
+      ++p.e;
+      piece_enter(a, p, q_tiles, tile_rows);
+    } while (p.span.n == 0);
+  }
+  p.i0 = 0;
+  p.i1 = (int)min((long long)p.span.n, p.end - p.unit);
+  return true;
+}
+
+// Position of tile i's keys / values in a piece's load order, the order in
+// which the tensor cores take them.  n tiles.  Pair: K0 V0 K1 V1 ..  Single:
+// K0 K1 V0 K2 V1 K3 .., the two streams one tile apart.
+template <bool kPair>
+__device__ __forceinline__ int load_index_k(int i) {
+  return kPair ? 2 * i : i < 2 ? i : 2 * i - 1;
+}
+template <bool kPair>
+__device__ __forceinline__ int load_index_v(int i, int n) {
+  return kPair ? 2 * i + 1 : i + min(i + 2, n);
+}
+
+// 16-key groups of a key tile without a page, as bits 0 .. 7 (the producer
+// loads pages below hi only; groups behind it are masked by position).
+__device__ __forceinline__ unsigned missing_groups(const AttendParams& a, int b, int tile, int lane) {
+  const long long key = (long long)tile * kKeyTile + lane * 16;
+  bool bad = false;
+  if (lane < 8) {
+    const long long slot = key / a.page_size;
+    const int page = slot < a.row_pages ? a.table[(long long)b * a.row_pages + slot] : -1;
+    bad = page < 0 || page >= a.pages;
+  }
+  return __ballot_sync(0xffffffffu, bad);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+// Whether either half of a packed word is an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool non_finite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w >> 16 & e) == e;
+}
+
+// One query row over the tiles [i0, i1) of its item, key by key, the values
+// of masked keys untouched: the plain definition, for items with non-finite
+// values.  o gets the unnormalised sum, *m the maximum (log2 units), *l the sum.
+template <typename T, int kDim>
+__device__ __noinline__ void attend_row_exact(const AttendParams& a, const Piece& p, int row, float* o, float* m_out,
+                                              float* l_out) {
+  const int group = a.heads / a.kv_heads, t = row / group, g = row - t * group;
+  const long long pos = p.span.start + t;
+  const Visible v = visible(a, pos, min(max(p.span.start + p.span.rows / group, 0ll), (long long)a.row_pages * a.page_size));
+  const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + t * a.q_stride[1] + (p.h * group + g) * a.q_stride[2];
+  const float sl = a.scale * 1.4426950408889634f;
+  float m = -INFINITY, l = 0.0f;
+  for (int d = 0; d < kDim; ++d) o[d] = 0.0f;
+  for (int i = p.i0; i < p.i1; ++i) {
+    const long long j0 = (long long)p.span.tile(i) * kKeyTile;
+    for (long long j = j0; j < j0 + kKeyTile; ++j) {
+      if (j >= v.hi || (j < v.lo && j >= a.sinks)) continue;
+      const int page = a.table[(long long)p.b * a.row_pages + j / a.page_size];
+      if (page < 0 || page >= a.pages) continue;
+      const long long at = (((long long)page * a.kv_heads + p.h) * a.page_size + j % a.page_size) * a.dim;
+      const T* k = static_cast<const T*>(a.pool[0]) + at;
+      const T* vv = static_cast<const T*>(a.pool[1]) + at;
+      float s = 0.0f;
+      for (int d = 0; d < a.dim; ++d) s += io<T>::to_f(q[d]) * io<T>::to_f(k[d]);
+      s *= sl;
+      if (s > m) {
+        const float keep = exp2f(m - s);
+        l *= keep;
+        for (int d = 0; d < a.dim; ++d) o[d] *= keep;
+        m = s;
+      }
+      const float w = exp2f(s - (m == -INFINITY ? 0.0f : m));
+      l += w;
+      for (int d = 0; d < a.dim; ++d) o[d] += w * io<T>::to_f(vv[d]);
+    }
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+template <int kDim, bool kPair>
+struct AttendShape {
+  static constexpr int kTiles = kPair ? 2 : 1;      // query tiles
+  static constexpr int kRows = 128 * kTiles;
+  static constexpr int kHalves = kDim / 64;
+  static constexpr int kTileBytes = 128 * kDim * 2;  // a query tile, a K or V tile
+  static constexpr int kStages = (224 * 1024 - kTiles * kTileBytes) / kTileBytes < kMaxStages
+                                     ? (224 * 1024 - kTiles * kTileBytes) / kTileBytes
+                                     : kMaxStages;
+};
+
+// Behind the tiles in shared memory.
+struct AttendShared {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t s_full[2], p_full[2], o_full[2], q_full, q_empty, wg[2], both;
+  PieceStart first;
+  long long warp_units[kAttThreads / 32], total;
+  uint32_t tmem_base;
+  int abort_flag;
+  unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
+  float2 row_ml[2][128];
+};
+// All of the 227 KB; the tiles start on a 1024-byte boundary, and there is
+// room for the padding that takes (the window starts on one: none).
+constexpr int kAttSmem = 227 * 1024;
+constexpr int kAttPad = kAttSmem - 224 * 1024 - (int)sizeof(AttendShared);
+static_assert(kAttPad >= 0, "tiles and AttendShared must fit 227 KB");
+
+template <typename T, int kDim, bool kPair>
+__global__ void __launch_bounds__(kAttThreads, 1)
+    attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ AttendParams a, const __grid_constant__ AttendWork work) {
+  using Shape = AttendShape<kDim, kPair>;
+  extern __shared__ unsigned char smem_raw[];
+  const int pad = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
+  if (pad > kAttPad) {
+    if (threadIdx.x == 0) {
+      atomicOr(a.status, DD_STATUS_TIMEOUT);
+      work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    }
+    return;
+  }
+  unsigned char* sm_q = smem_raw + pad;
+  unsigned char* sm_ring = sm_q + Shape::kTiles * Shape::kTileBytes;
+  AttendShared& bar = *reinterpret_cast<AttendShared*>(sm_q + 224 * 1024);
+  PieceStart& first = bar.first;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.heads / a.kv_heads;
+  const int q_tiles = (int)(((long long)a.tokens * group + Shape::kRows - 1) / Shape::kRows);
+
+  if (tid == 0) {
+    bar.abort_flag = 0;
+    bar.redo[0] = bar.redo[1] = 0;
+    for (int i = 0; i < Shape::kStages; ++i) {
+      mbar_init(&bar.full[i], 1);
+      mbar_init(&bar.empty[i], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar.s_full[s], 1);
+      mbar_init(&bar.p_full[s], 128);
+      mbar_init(&bar.o_full[s], 1);
+      mbar_init(&bar.wg[s], 128);
+    }
+    mbar_init(&bar.q_full, 64);
+    mbar_init(&bar.q_empty, 1);
+    mbar_init(&bar.both, 256);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(&bar.tmem_base, 512);
+  pdl_wait_primary();
+
+  // the CTA's run of tiles
+  {
+    const int entries = a.batch * q_tiles, per = (entries + kAttThreads - 1) / kAttThreads;
+    const int e0 = tid * per, e1 = min(entries, e0 + per);
+    long long mine = 0;
+    for (int e = e0; e < e1; ++e) mine += tile_span(a, e / q_tiles, e % q_tiles, Shape::kRows).n;
+    mine *= a.kv_heads;
+    long long inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    if (lane == 31) bar.warp_units[warp] = inc;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttThreads / 32; ++w) {
+      if (w < warp) before += bar.warp_units[w];
+      total += bar.warp_units[w];
+    }
+    before += inc - mine;
+    const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+    if (u0 >= u1) {
+      if (tid == 0) {
+        first.unit = first.end = 0;
+        work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      }
+    } else if (u0 >= before && u0 < before + mine) {
+      long long at = before;
+      for (int e = e0; e < e1; ++e) {
+        const long long n = (long long)tile_span(a, e / q_tiles, e % q_tiles, Shape::kRows).n * a.kv_heads;
+        if (u0 < at + n) {
+          first.unit = u0;
+          first.end = u1;
+          first.rem = u0 - at;
+          first.e = e;
+          break;
+        }
+        at += n;
+      }
+    }
+    if (tid == 0) bar.total = total;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  const uint32_t tmem = bar.tmem_base;
+  volatile int* abort = &bar.abort_flag;
+  Piece p;
+  bool more = piece_first(a, first, p, q_tiles, Shape::kRows);
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- producer
+    const int pages_per_tile = kKeyTile / a.page_size;
+    const uint32_t page_bytes = a.page_size * 128u;  // of one 64-value half
+    long long cnt = 0;
+    bool ok = true;
+    if (lane == 0) {
+      prefetch_tmap(&map_k);
+      prefetch_tmap(&map_v);
+    }
+    auto load = [&](const CUtensorMap* map, int i) {
+      const int tile = p.span.tile(i);
+      const long long slot = (long long)tile * pages_per_tile + lane;
+      int page = -1;
+      if (lane < pages_per_tile && slot < a.row_pages && slot * a.page_size < p.span.hi) {
+        page = a.table[(long long)p.b * a.row_pages + slot];
+        if (page >= a.pages) page = -1;
+      }
+      const int st = (int)(cnt % Shape::kStages);
+      ok = mbar_wait_bounded(&bar.empty[st], ((cnt / Shape::kStages) & 1) ^ 1, abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], __popc(have) * page_bytes * Shape::kHalves);
+      __syncwarp();
+      if (page >= 0) {
+        unsigned char* dst = sm_ring + st * Shape::kTileBytes + lane * page_bytes;
+#pragma unroll
+        for (int hf = 0; hf < Shape::kHalves; ++hf)
+          tma_load_4d(dst + hf * 128 * 128, map, &bar.full[st], hf * 64, 0, p.h, page);
+      }
+      ++cnt;
+    };
+    for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+      const int n = p.i1 - p.i0;
+      if (kPair) {
+        for (int i = 0; i < n && ok; ++i) {
+          load(&map_k, p.i0 + i);
+          if (ok) load(&map_v, p.i0 + i);
+        }
+      } else {
+        load(&map_k, p.i0);
+        if (ok && n > 1) load(&map_k, p.i0 + 1);
+        for (int i = 0; i < n && ok; ++i) {
+          load(&map_v, p.i0 + i);
+          if (ok && i + 2 < n) load(&map_k, p.i0 + i + 2);
+        }
+      }
+    }
+    if (!ok) {  // leave no copy in flight behind this CTA
+      for (long long c = max(0ll, cnt - Shape::kStages); c < cnt; ++c)
+        for (int k = 0; k < 1000000 && !mbar_try_wait(&bar.full[c % Shape::kStages], (c / Shape::kStages) & 1); ++k) {
+        }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+      constexpr uint32_t idesc_s = idesc_f16(128, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
+      long long base = 0;
+      uint32_t n_pieces = 0, n_p[2] = {0, 0};
+      bool ok = true;
+      auto stage = [&](int idx) { return (int)((base + idx) % Shape::kStages); };
+      auto wait_load = [&](int idx) {
+        const long long c = base + idx;
+        ok = ok && mbar_wait_bounded(&bar.full[c % Shape::kStages], (c / Shape::kStages) & 1, abort);
+      };
+      auto qk = [&](int s, int idx) {
+        const uint32_t q = smem_u32(sm_q) + (kPair ? s * Shape::kTileBytes : 0);
+        const uint32_t k = smem_u32(sm_ring) + stage(idx) * Shape::kTileBytes;
+#pragma unroll
+        for (int d = 0; d < kDim / 16; ++d) {
+          const uint32_t off = (d / 4) * 128 * 128 + (d % 4) * 32;
+          mma_f16_ss(tmem + s * 128, smem_desc_k_sw128(q + off), smem_desc_k_sw128(k + off), idesc_s, d > 0);
+        }
+        mma_commit(&bar.s_full[s]);
+      };
+      auto pv = [&](int s, int idx, bool accumulate) {
+        const uint32_t v = smem_u32(sm_ring) + stage(idx) * Shape::kTileBytes;
+#pragma unroll
+        for (int d = 0; d < kKeyTile / 16; ++d)
+          mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + d * 8, smem_desc_mn_sw128(v + d * 2048, 128 * 128),
+                     idesc_o, accumulate || d > 0);
+      };
+      auto wait_p = [&](int s) {
+        ok = ok && mbar_wait_bounded(&bar.p_full[s], n_p[s]++ & 1, abort);
+        tc_fence_after();
+      };
+      for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+        const int n = p.i1 - p.i0;
+        ok = ok && mbar_wait_bounded(&bar.q_full, n_pieces++ & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        if (kPair) {
+          wait_load(load_index_k<true>(0));
+          if (!ok) break;
+          qk(0, load_index_k<true>(0));
+          qk(1, load_index_k<true>(0));
+          mma_commit(&bar.empty[stage(load_index_k<true>(0))]);
+          if (n == 1) mma_commit(&bar.q_empty);
+          for (int i = 0; i < n && ok; ++i) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              wait_p(s);
+              const int iv = load_index_v<true>(i, n), ik = load_index_k<true>(i + 1);
+              if (s == 0) wait_load(iv);
+              if (!ok) break;
+              pv(s, iv, i > 0);
+              if (s == 1) mma_commit(&bar.empty[stage(iv)]);
+              if (i + 1 < n) {
+                if (s == 0) wait_load(ik);
+                if (!ok) break;
+                qk(s, ik);
+                if (s == 1) {
+                  mma_commit(&bar.empty[stage(ik)]);
+                  if (i + 2 == n) mma_commit(&bar.q_empty);
+                }
+              } else {
+                mma_commit(&bar.o_full[s]);
+              }
+            }
+          }
+        } else {
+          for (int s = 0; s < min(2, n) && ok; ++s) {
+            wait_load(load_index_k<false>(s));
+            if (!ok) break;
+            qk(s, load_index_k<false>(s));
+            mma_commit(&bar.empty[stage(load_index_k<false>(s))]);
+          }
+          if (ok && n <= 2) mma_commit(&bar.q_empty);
+          for (int i = 0; i < n && ok; ++i) {
+            const int s = i & 1, iv = load_index_v<false>(i, n), ik = load_index_k<false>(i + 2);
+            wait_p(s);
+            wait_load(iv);
+            if (!ok) break;
+            pv(s, iv, i >= 2);
+            mma_commit(&bar.empty[stage(iv)]);
+            if (i + 2 < n) {
+              wait_load(ik);
+              if (!ok) break;
+              qk(s, ik);
+              mma_commit(&bar.empty[stage(ik)]);
+              if (i + 3 == n) mma_commit(&bar.q_empty);
+            } else {
+              mma_commit(&bar.o_full[s]);
+            }
+          }
+        }
+        base += 2 * n;
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 10) {
+    // ---------------------------------------------------------------- query loader, and the record for the join
+    const int id = tid - 320;
+    constexpr int kChunks = kDim / 8;  // 16-byte chunks of a row
+    const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0 &&
+                     a.q_stride[2] % 8 == 0;
+    const long long total = bar.total;
+    uint32_t n_pieces = 0;
+    int4 head = make_int4(-1, 0, 0, 0);
+    bool ok = true;
+    for (; more; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+      if (p.i0 == 0 && p.i1 < p.span.n) {
+        const long long end = p.unit + p.span.n;
+        int c = blockIdx.x + 1;
+        while (total * (c + 1) / gridDim.x < end) ++c;
+        // (with fewer tiles than CTAs some CTAs between are empty: the join needs the total)
+        head = make_int4(p.e, p.h, c, total < gridDim.x ? (int)total : 0);
+      }
+      ok = mbar_wait_bounded(&bar.q_empty, (n_pieces++ & 1) ^ 1, abort);
+      if (!ok) break;
+      const int r0 = p.qt * Shape::kRows, live = min(Shape::kRows, p.span.rows - r0);
+      const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0];
+      for (int c0 = id; c0 < live * kChunks; c0 += 64 * 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int c = c0 + 64 * k, row = c / kChunks, ch = c % kChunks;
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (row < live && ch * 8 < a.dim) {
+            const int t = (r0 + row) / group, g = (r0 + row) - t * group;
+            const T* src = q + t * a.q_stride[1] + (p.h * group + g) * a.q_stride[2] + ch * 8;
+            if (vec) {
+              v[k] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              alignas(16) T x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = src[i];
+              v[k] = *reinterpret_cast<const uint4*>(x);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int c = c0 + 64 * k, row = c / kChunks, ch = c % kChunks;
+          if (row < live)
+            *reinterpret_cast<uint4*>(sm_q + (row / 128) * Shape::kTileBytes + (ch / 8) * 128 * 128 + (row % 128) * 128 +
+                                      ((ch % 8) ^ (row % 8)) * 16) = v[k];
+        }
+      }
+      fence_proxy_async_shared();
+      mbar_arrive(&bar.q_full);
+    }
+    if (id == 0 && first.unit < first.end) work.head[blockIdx.x] = head;
+  } else {
+    // ---------------------------------------------------------------- softmax, one thread per query row
+    const int s = warp >> 2, row = tid & 127;
+    const uint32_t lanes = ((warp & 3) * 32u) << 16;
+    const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + lanes;
+    const float sl = a.scale * 1.4426950408889634f;
+    uint32_t n_s = 0, n_o[2] = {0, 0}, n_wg = 0, n_both = 0, n_pieces = 0;
+    long long base = 0;
+    bool ok = true;
+    for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+      const int n = p.i1 - p.i0;
+      ++n_pieces;
+      const int tile0 = p.qt * Shape::kRows + (kPair ? s * 128 : 0), r = tile0 + row;
+      const bool warp_live = tile0 + (warp & 3) * 32 < p.span.rows;
+      // keys that the row sees: [lo, hi) and, below hi, [0, sinks)
+      const long long pos = p.span.start + r / group;
+      long long hi = 0, lo = 0;
+      if (r < p.span.rows) {
+        hi = a.causal ? min(p.span.hi, pos + 1) : p.span.hi;
+        lo = a.window > 0 ? max(pos - a.window + 1, 0ll) : 0;
+      }
+      // rows of the item see all keys of [all_lo, all_hi)
+      const long long p_min = p.span.start + p.qt * Shape::kRows / group;
+      const long long p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * Shape::kRows) - 1) / group;
+      const long long all_hi = a.causal ? min(p.span.hi, p_min + 1) : p.span.hi;
+      const long long all_lo = a.window > 0 ? max(p_max - a.window + 1, 0ll) : 0;
+      float m = -INFINITY, l = 0.0f;
+      bool have_o = false;
+      for (int i = kPair ? 0 : s; i < n; i += kPair ? 1 : 2) {
+        const int tile = p.span.tile(p.i0 + i);
+        const long long key0 = (long long)tile * kKeyTile, key1 = key0 + kKeyTile;
+        const unsigned missing = key0 < p.span.hi ? missing_groups(a, p.b, tile, lane) : 0;
+        const bool whole = missing == 0 && key1 <= all_hi && (key0 >= all_lo || key1 <= a.sinks);
+        ok = mbar_wait_bounded(&bar.s_full[s], n_s++ & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        if (warp_live) {
+          uint32_t x[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x + 32 * c);
+          tmem_ld_wait();
+          if (!whole) {
+            const int hi_c = (int)min(max(hi - key0, 0ll), 128ll), lo_c = (int)min(max(lo - key0, 0ll), 128ll);
+            const int sink_c = (int)min(max((long long)a.sinks - key0, 0ll), 128ll);
+#pragma unroll
+            for (int c = 0; c < 128; ++c) {
+              const bool see = c < hi_c && (c >= lo_c || c < sink_c) && !(missing >> (c / 16) & 1);
+              if (!see) x[c] = 0xff800000u;  // -inf
+            }
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c]));
+          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          const bool moves = (mt - m) * sl > 8.0f;
+          if (__any_sync(0xffffffffu, moves)) {
+            const float m1 = moves ? mt : m;
+            const float keep = moves ? exp2_approx((m - m1) * sl) : 1.0f;
+            l *= keep;
+            m = m1;
+            if (have_o) {
+              for (int c = 0; c < kDim; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(t_o + s * kDim + c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                tmem_st32(t_o + s * kDim + c, o);
+              }
+            }
+          }
+          have_o = true;
+          const float sub = m == -INFINITY ? 0.0f : m * sl;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 128; c += 64) {
+            uint32_t w[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float p0 = exp2_approx(__uint_as_float(x[c + 2 * k]) * sl - sub);
+              const float p1 = exp2_approx(__uint_as_float(x[c + 2 * k + 1]) * sl - sub);
+              sum[k & 1] += p0;
+              sum[2 + (k & 1)] += p1;
+              w[k] = pack2<T>(p0, p1);
+            }
+            tmem_st32(t_s + c / 2, w);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+        }
+        if (!whole) {
+          const long long c = base + load_index_v<kPair>(i, n);
+          const int st = (int)(c % Shape::kStages);
+          ok = mbar_wait_bounded(&bar.full[st], (c / Shape::kStages) & 1, abort);
+          if (!ok) break;
+          // this thread's key: zero if no row of the item sees it; non-finite values that some rows see
+          const long long j = key0 + row;
+          unsigned char* v = sm_ring + st * Shape::kTileBytes + row * 128;
+          const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (row / 16) & 1);
+          if (!seen) {
+#pragma unroll
+            for (int hf = 0; hf < Shape::kHalves; ++hf)
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<uint4*>(v + hf * 128 * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_shared();
+          } else if (j >= all_hi || (j < all_lo && j >= a.sinks)) {
+            bool odd = false;
+#pragma unroll
+            for (int hf = 0; hf < Shape::kHalves; ++hf)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint4 w = *reinterpret_cast<const uint4*>(v + hf * 128 * 128 + k * 16);
+                odd = odd || non_finite2<T>(w.x) || non_finite2<T>(w.y) || non_finite2<T>(w.z) || non_finite2<T>(w.w);
+              }
+            if (odd) bar.redo[s] = n_pieces;
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&bar.p_full[s]);
+      }
+      if (!ok) break;
+      // the piece's result
+      const bool split = p.i0 > 0 || p.i1 < p.span.n;
+      const size_t slot = 2 * (size_t)blockIdx.x + (p.i0 == 0 ? 1 : 0);
+      const int t = r / group, g = r - t * group;
+      const bool in_chunk = r < a.tokens * group;
+      T* out = static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * group + g) * a.dim;
+      const int slot_row = (kPair ? s * 128 : 0) + row;
+      float* part = work.o + (slot * Shape::kRows + slot_row) * kDim;
+      float f[2], inv;
+      bool again;
+      if (kPair) {
+        ok = mbar_wait_bounded(&bar.o_full[s], n_o[s]++ & 1, abort);
+        if (!ok) break;
+        mbar_arrive(&bar.wg[s]);
+        ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
+        if (!ok) break;
+        again = bar.redo[s] == n_pieces;  // nobody searches the next piece before all have read this
+        mbar_arrive(&bar.wg[s]);
+        ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
+        if (!ok) break;
+        f[0] = f[1] = 1.0f;
+      } else {
+        bar.row_ml[s][row] = make_float2(m == -INFINITY ? -INFINITY : m * sl, l);
+        ok = mbar_wait_bounded(&bar.o_full[0], n_o[0]++ & 1, abort);
+        if (ok && n > 1) ok = mbar_wait_bounded(&bar.o_full[1], n_o[1]++ & 1, abort);
+        if (!ok) break;
+        mbar_arrive(&bar.both);
+        ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
+        if (!ok) break;
+        const float2 x0 = bar.row_ml[0][row], x1 = bar.row_ml[1][row];
+        again = bar.redo[0] == n_pieces || bar.redo[1] == n_pieces;
+        const float top = fmaxf(x0.x, x1.x);
+        f[0] = x0.x == -INFINITY ? 0.0f : exp2_approx(x0.x - top);
+        f[1] = x1.x == -INFINITY ? 0.0f : exp2_approx(x1.x - top);
+        l = x0.y * f[0] + x1.y * f[1];
+        m = top;
+      }
+      tc_fence_after();
+      if (kPair && m != -INFINITY) m *= sl;
+      inv = l == 0.0f ? 0.0f : 1.0f / l;
+      if (again) {
+        // (both streams' rows are the same without kPair: the first does them)
+        if ((kPair || s == 0) && in_chunk) {
+          const Piece here = p;
+          float o[kDim];
+          float m_x = -INFINITY, l_x = 0.0f;
+          for (int d = 0; d < kDim; ++d) o[d] = 0.0f;
+          if (r < p.span.rows) attend_row_exact<T, kDim>(a, here, r, o, &m_x, &l_x);
+          inv = l_x == 0.0f ? 0.0f : 1.0f / l_x;
+          if (split) {
+            for (int d = 0; d < kDim; ++d) part[d] = o[d];
+            work.ml[slot * Shape::kRows + slot_row] = make_float2(m_x, l_x);
+          } else {
+            for (int d = 0; d < a.dim; ++d) out[d] = io<T>::from_f(r < p.span.rows ? o[d] * inv : 0.0f);
+          }
+        }
+      } else {
+        if (split && (kPair || s == 0)) work.ml[slot * Shape::kRows + slot_row] = make_float2(m, l);
+        const float norm = split ? 1.0f : inv;
+        const int c_begin = kPair ? 0 : s * (kDim / 2), c_end = kPair ? kDim : c_begin + kDim / 2;
+        const float f0 = f[0] * norm, f1 = f[1] * norm;
+#pragma unroll 1
+        for (int c = c_begin; c < c_end; c += 32) {
+          float o[32];
+          if (warp_live) {
+            uint32_t x[32];
+            tmem_ld32(t_o + (kPair ? s * kDim : 0) + c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = f0 == 0.0f ? 0.0f : __uint_as_float(x[k]) * f0;
+            if (!kPair && n > 1) {
+              tmem_ld32(t_o + kDim + c, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] += f1 == 0.0f ? 0.0f : __uint_as_float(x[k]) * f1;
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0.0f;
+          }
+          if (!in_chunk) continue;
+          if (split) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          } else {
+            const bool live = r < p.span.rows;
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              if (c + k >= a.dim) break;
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (live)
+                w = make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),
+                               pack2<T>(o[k + 6], o[k + 7]));
+              *reinterpret_cast<uint4*>(out + c + k) = w;
+            }
+          }
+        }
+      }
+      if (!kPair) {  // both streams have read O, the maxima and the flags
+        tc_fence_before();
+        mbar_arrive(&bar.both);
+        ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
+        if (!ok) break;
+      }
+      base += 2 * n;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 512);
+  }
+  if (tid == 0 && bar.abort_flag) atomicOr(a.status, DD_STATUS_TIMEOUT);
+}
+
+// The items that cross CTAs: CTA c's record names an item whose first tiles it
+// holds; the rest is in slot 0 of the CTAs behind it.  A block takes 16 rows
+// (4 warps, 4 rows each).  Also the rows that no item covers: behind the end
+// of a short chunk, or with no key to see.
+constexpr int kJoinRows = 16;
+template <typename T, int kDim, bool kPair>
+__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendParams a,
+                                                          const __grid_constant__ AttendWork work) {
+  constexpr int kRows = AttendShape<kDim, kPair>::kRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.heads / a.kv_heads;
+  const int q_tiles = (int)(((long long)a.tokens * group + kRows - 1) / kRows);
+  pdl_wait_primary();
+  const int4 head = work.head[blockIdx.x];
+  if (head.x >= 0) {
+    const int b = head.x / q_tiles, qt = head.x - b * q_tiles, h = head.y, c0 = blockIdx.x, c1 = head.z;
+    const int rows = (int)(a.lens ? min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens) * group;
+    // CTAs without a tile (fewer tiles than CTAs) have left nothing
+    auto empty = [&](int c) {
+      return head.w > 0 && (long long)head.w * c / gridDim.x == (long long)head.w * (c + 1) / gridDim.x;
+    };
+    for (int k = warp; k < kJoinRows; k += 4) {
+      const int row = blockIdx.y * kJoinRows + k, r = qt * kRows + row;
+      if (r >= a.tokens * group) break;
+      const int t = r / group, g = r - t * group;
+      T* out = static_cast<T*>(a.out) + (((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim;
+      float o[kDim / 32] = {};
+      float top = -INFINITY, l = 0.0f;
+      if (r < rows) {
+        for (int c = c0 + lane; c <= c1; c += 32)
+          if (!empty(c)) top = fmaxf(top, work.ml[(2 * (size_t)c + (c == c0)) * kRows + row].x);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int c = c0; c <= c1; ++c) {
+          if (empty(c)) continue;
+          const size_t slot = 2 * (size_t)c + (c == c0);
+          const float2 ml = work.ml[slot * kRows + row];
+          const float* part = work.o + (slot * kRows + row) * kDim;
+          if (ml.y == 0.0f) continue;  // the piece holds no key that this row sees
+          const float w = exp2_approx(ml.x - (top == -INFINITY ? 0.0f : top));
+          l += ml.y * w;
+#pragma unroll
+          for (int i = 0; i < kDim / 32; ++i) o[i] += part[lane + 32 * i] * w;
+        }
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int i = 0; i < kDim / 32; ++i)
+        if (lane + 32 * i < a.dim) out[lane + 32 * i] = io<T>::from_f(o[i] * inv);
+    }
+  }
+  const int blocks = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
+  for (int e = me; e < a.batch * q_tiles; e += blocks) {
+    const int b = e / q_tiles, qt = e - b * q_tiles;
+    if (tile_span(a, b, qt, kRows).n) continue;
+    const int r1 = min((qt + 1) * kRows, a.tokens * group);
+    for (int r = qt * kRows; r < r1; ++r) {
+      const int t = r / group, g = r - t * group;
+      for (int i = threadIdx.x; i < a.kv_heads * a.dim; i += 128) {
+        const int h = i / a.dim, d = i - h * a.dim;
+        static_cast<T*>(a.out)[(((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + d] = io<T>::from_f(0.0f);
+      }
+    }
+  }
+}
+
+}  // namespace dd

@@ -6,9 +6,12 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <mutex>
+#include <type_traits>
 
 #include "../../include/domino_draft.h"
 #include "dd_attend.cuh"
+#include "dd_attend_tc.cuh"
 #include "dd_cache_write.cuh"
 #include "dd_common.h"
 #include "dd_pages.cuh"
@@ -165,6 +168,88 @@ int launch_write(const WriteParams& p, int batch, int tokens_per_cta, bool inter
              : launch_write<T, false>(p, batch, tokens_per_cta, interleaved, stream);
 }
 
+typedef CUresult (*PFN_encodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+PFN_encodeTiled encoder() {
+  static PFN_encodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<PFN_encodeTiled>(p) : nullptr;
+  }();
+  return fn;
+}
+
+// One layer's keys or values as [pages, kv_heads, page_size, head_dim], in
+// boxes of one head's page x 64 values with 128-byte swizzle.  Values behind
+// head_dim read as zero.
+int encode_pool(const dd_paged_cache* c, int layer, int kv, CUtensorMap* m) {
+  PFN_encodeTiled encode = encoder();
+  if (!encode) return global_fail(DD_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t row = (cuuint64_t)c->head_dim * 2;
+  cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->kv_heads, (cuuint64_t)c->pages};
+  cuuint64_t strides[3] = {row, row * c->page_size, row * c->page_size * c->kv_heads};
+  cuuint32_t box[4] = {64, (cuuint32_t)c->page_size, 1, 1}, one[4] = {1, 1, 1, 1};
+  CUresult r = encode(m, c->dtype == DD_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                      plane(c, layer, kv), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return global_fail(DD_ECUDA, "cuTensorMapEncodeTiled (page pool) failed (%d)", (int)r);
+  return DD_OK;
+}
+
+// Which kernel serves a call: the tensor cores take 16-bit caches with heads
+// of up to 128 values; pairs of query tiles from the second tile on.
+struct AttendPlan {
+  bool tensor, pair;
+  int dim;  // head_dim padded to 64 or 128
+};
+AttendPlan attend_plan(const dd_paged_cache* c, const dd_cache_attend_args* a) {
+  AttendPlan p;
+  p.tensor = c->dtype != DD_F32 && c->head_dim <= 128;
+  p.dim = c->head_dim <= 64 ? 64 : 128;
+  p.pair = (long long)a->tokens * (a->heads / c->kv_heads) > 128;
+  return p;
+}
+uint64_t attend_bytes(const AttendPlan& p, const DeviceInfo& dev) {
+  if (!p.tensor) return 0;
+  if (p.dim == 64) return p.pair ? attend_work_bytes<64, true>(dev.sms) : attend_work_bytes<64, false>(dev.sms);
+  return p.pair ? attend_work_bytes<128, true>(dev.sms) : attend_work_bytes<128, false>(dev.sms);
+}
+
+template <typename T, int kDim, bool kPair>
+int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendParams& p, const DeviceInfo& dev,
+                  void* stream) {
+  CUtensorMap mk, mv;
+  int rc = encode_pool(c, args->layer, 0, &mk);
+  if (!rc) rc = encode_pool(c, args->layer, 1, &mv);
+  if (rc) return rc;
+  static bool ready[64];
+  if (!ready[c->device]) {
+    DD_TRY(cudaFuncSetAttribute(attend_tc_kernel<T, kDim, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttSmem));
+    ready[c->device] = true;
+  }
+  constexpr int kRows = AttendShape<kDim, kPair>::kRows;
+  AttendWork w;
+  w.head = static_cast<int4*>(args->workspace);
+  w.o = reinterpret_cast<float*>(w.head + dev.sms);
+  w.ml = reinterpret_cast<float2*>(w.o + (size_t)dev.sms * 2 * kRows * kDim);
+  rc = launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(dev.sms), dim3(kAttThreads), kAttSmem, stream, mk, mv, p, w);
+  if (rc) return rc;
+  return launch("attend join", attend_join_kernel<T, kDim, kPair>, dim3(dev.sms, kRows / kJoinRows), dim3(128), 0, stream,
+                p, w);
+}
+template <typename T>
+int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendPlan& plan, const AttendParams& p,
+                  const DeviceInfo& dev, void* stream) {
+  if (plan.dim == 64)
+    return plan.pair ? launch_attend<T, 64, true>(c, args, p, dev, stream)
+                     : launch_attend<T, 64, false>(c, args, p, dev, stream);
+  return plan.pair ? launch_attend<T, 128, true>(c, args, p, dev, stream)
+                   : launch_attend<T, 128, false>(c, args, p, dev, stream);
+}
+
 int check_attend(const dd_paged_cache* c, const dd_cache_attend_args* a) {
   int rc = check_cache(c);
   if (rc) return rc;
@@ -305,7 +390,9 @@ int dd_cache_attend_workspace(const dd_paged_cache* c, const dd_cache_attend_arg
   int rc = check_attend(c, a);
   if (rc) return rc;
   if (!bytes) return global_fail(DD_EINVAL, "null argument");
-  *bytes = 0;
+  DeviceInfo dev;
+  if ((rc = device_info(c->device, &dev))) return rc;
+  *bytes = attend_bytes(attend_plan(c, a), dev);
   return DD_OK;
 }
 
@@ -338,6 +425,15 @@ int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void
   p.causal = a->causal != 0;
   p.window = a->window;
   p.sinks = a->sinks;
+  p.status = c->status;
+  const AttendPlan plan = attend_plan(c, a);
+  if (plan.tensor) {
+    if (!a->workspace || a->workspace_bytes < attend_bytes(plan, dev) || !aligned16(a->workspace))
+      return global_fail(DD_EINVAL, "dd_cache_attend: workspace of %llu bytes needed",
+                         (unsigned long long)attend_bytes(plan, dev));
+    if (c->dtype == DD_FP16) return launch_attend<__half>(c, a, plan, p, dev, stream);
+    return launch_attend<__nv_bfloat16>(c, a, plan, p, dev, stream);
+  }
   const long long units = (long long)c->batch * a->tokens * a->heads;
   const long long blocks = (units + kSimpleWarps - 1) / kSimpleWarps;
   if (blocks > 0x7fffffffll) return global_fail(DD_EINVAL, "dd_cache_attend: chunk too large");
