@@ -22,7 +22,8 @@ struct AttendParams {
   const long long* lens;     // null: all tokens
   unsigned* status;
   float scale;
-  int batch, tokens, heads, kv_heads, dim, pages, page_size, row_pages;
+  int batch, tokens, heads, kv_heads, dim, pages, page_size, page_shift, row_pages;  // page_size = 1 << page_shift
+  int group;                 // query heads per key head
   int causal, window, sinks;
 };
 

@@ -54,34 +54,31 @@ constexpr size_t attend_work_bytes(int grid) {
   return (size_t)grid * (16 + 2 * (kPair ? 256 : 128) * (sizeof(float) * kDim + 8));
 }
 
-// Key tiles of one (row of the batch, query tile): n_sink from 0, then from `first` on.
+// Key tiles of one (row of the batch, query tile): n_sink from 0, then from
+// `first` on.  Positions are 32-bit here: a row holds at most 2^30 tokens.
 struct TileSpan {
   int n_sink, first, n;
-  int rows;              // query rows of the batch row (tokens x group)
-  long long start, lo, hi;  // position of token 0; keys that any row of the tile sees: [lo, hi) and below sinks
+  int rows;           // query rows of the batch row (tokens x group)
+  int start, lo, hi;  // position of token 0; keys that any row of the tile sees: [lo, hi) and, below hi, the sinks
   __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
 };
-__device__ inline TileSpan tile_span(const AttendParams& a, int b, int qt, int tile_rows) {
+__device__ __forceinline__ TileSpan tile_span(const AttendParams& a, int b, int qt, int tile_rows) {
   TileSpan s;
-  const int group = a.heads / a.kv_heads;
-  const int n_new = (int)(a.lens ? min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens);
-  s.start = a.start[b];
-  s.rows = n_new * group;
+  const int n_new = a.lens ? (int)min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens;
+  s.start = (int)min(max(a.start[b], -(1ll << 30)), 1ll << 30);
+  s.rows = n_new * a.group;
   s.n_sink = s.first = s.n = 0;
   s.lo = s.hi = 0;
   const int r0 = qt * tile_rows;
   if (r0 >= s.rows) return s;
-  const long long p0 = s.start + r0 / group, p1 = s.start + (min(s.rows, r0 + tile_rows) - 1) / group;
-  const long long total = min(max(s.start + n_new, 0ll), (long long)a.row_pages * a.page_size);
-  s.hi = a.causal ? min(total, p1 + 1) : total;
-  if (s.hi <= 0) {
-    s.hi = 0;
-    return s;
-  }
-  s.lo = a.window > 0 ? max(p0 - a.window + 1, 0ll) : 0;
-  const int t_lo = (int)(s.lo / kKeyTile), t_hi = (int)((s.hi + kKeyTile - 1) / kKeyTile);
-  const long long sinks = min(min((long long)a.sinks, s.lo), s.hi);
-  s.n_sink = min((int)((sinks + kKeyTile - 1) / kKeyTile), t_lo);
+  const int p0 = s.start + r0 / a.group, p1 = s.start + (min(s.rows, r0 + tile_rows) - 1) / a.group;
+  const int total = min(max(s.start + n_new, 0), a.row_pages << a.page_shift);
+  s.hi = max(a.causal ? min(total, p1 + 1) : total, 0);
+  if (s.hi == 0) return s;
+  s.lo = a.window > 0 ? max(p0 - a.window + 1, 0) : 0;
+  const int t_lo = s.lo / kKeyTile, t_hi = (s.hi + kKeyTile - 1) / kKeyTile;
+  const int sinks = min(min(a.sinks, s.lo), s.hi);
+  s.n_sink = min((sinks + kKeyTile - 1) / kKeyTile, t_lo);
   s.first = t_lo;
   s.n = s.n_sink + max(t_hi - t_lo, 0);
   return s;
@@ -90,12 +87,11 @@ __device__ inline TileSpan tile_span(const AttendParams& a, int b, int qt, int t
 // A CTA's run of key tiles, item by item.
 struct Piece {
   int e, b, qt, h, i0, i1;  // entry (b, qt), key head, tiles [i0, i1) of it
-  long long unit, end;      // number of tile i0; end of the CTA's run
+  int left;                 // tiles of the run from i0 on
   TileSpan span;
 };
 struct PieceStart {
-  long long unit, end, rem;  // rem: tiles of the entry before `unit`
-  int e;
+  int units, e, h, i0;  // tiles of the run, and where it starts
 };
 __device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
   p.b = p.e / q_tiles;
@@ -104,19 +100,18 @@ __device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int
 }
 __device__ __forceinline__ bool piece_first(const AttendParams& a, const PieceStart& s, Piece& p, int q_tiles,
                                             int tile_rows) {
-  p.unit = s.unit;
-  p.end = s.end;
-  if (p.unit >= p.end) return false;
+  p.left = s.units;
+  if (p.left == 0) return false;
   p.e = s.e;
+  p.h = s.h;
+  p.i0 = s.i0;
   piece_enter(a, p, q_tiles, tile_rows);
-  p.h = (int)(s.rem / p.span.n);
-  p.i0 = (int)(s.rem - (long long)p.h * p.span.n);
-  p.i1 = (int)min((long long)p.span.n, p.i0 + (p.end - p.unit));
+  p.i1 = min(p.span.n, p.i0 + p.left);
   return true;
 }
 __device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
-  p.unit += p.i1 - p.i0;
-  if (p.unit >= p.end) return false;
+  p.left -= p.i1 - p.i0;
+  if (p.left == 0) return false;
   if (++p.h == a.kv_heads) {
     p.h = 0;
     do {
@@ -125,33 +120,34 @@ __device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int 
     } while (p.span.n == 0);
   }
   p.i0 = 0;
-  p.i1 = (int)min((long long)p.span.n, p.end - p.unit);
+  p.i1 = min(p.span.n, p.left);
   return true;
 }
 
-// Position of tile i's keys / values in a piece's load order, the order in
-// which the tensor cores take them.  n tiles.  Pair: K0 V0 K1 V1 ..  Single:
-// K0 K1 V0 K2 V1 K3 .., the two streams one tile apart.
-template <bool kPair>
-__device__ __forceinline__ int load_index_k(int i) {
-  return kPair ? 2 * i : i < 2 ? i : 2 * i - 1;
-}
+// The ring of key and value tiles.  Tiles are loaded in the order in which the
+// tensor cores take them: with kPair K0 V0 K1 V1 .., without K0 K1 V0 K2 V1 K3
+// .. (the two streams one tile apart), so producer and issuer walk it in step.
+template <int kStages>
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+// Position of tile i's values in a piece's load order; n tiles.
 template <bool kPair>
 __device__ __forceinline__ int load_index_v(int i, int n) {
   return kPair ? 2 * i + 1 : i + min(i + 2, n);
 }
 
-// 16-key groups of a key tile without a page, as bits 0 .. 7 (the producer
-// loads pages below hi only; groups behind it are masked by position).
-__device__ __forceinline__ unsigned missing_groups(const AttendParams& a, int b, int tile, int lane) {
-  const long long key = (long long)tile * kKeyTile + lane * 16;
-  bool bad = false;
-  if (lane < 8) {
-    const long long slot = key / a.page_size;
-    const int page = slot < a.row_pages ? a.table[(long long)b * a.row_pages + slot] : -1;
-    bad = page < 0 || page >= a.pages;
-  }
-  return __ballot_sync(0xffffffffu, bad);
+// Page of 16-key group `lane` (0 .. 7) of a key tile.
+__device__ __forceinline__ int group_page(const AttendParams& a, int b, int tile, int lane) {
+  const int slot = (tile * kKeyTile + lane * 16) >> a.page_shift;
+  return lane < 8 && slot < a.row_pages ? a.table[(long long)b * a.row_pages + slot] : -1;
 }
 
 template <typename T>
@@ -166,6 +162,14 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+// The n lowest bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+// Scores that are not seen become -infinity.
+__device__ __forceinline__ void mask32(uint32_t (&x)[32], uint32_t see) {
+  if (__all_sync(0xffffffffu, see == ~0u)) return;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) x[k] = see >> k & 1 ? x[k] : 0xff800000u;
+}
 // Whether either half of a packed word is an infinity or a NaN.
 template <typename T>
 __device__ __forceinline__ bool non_finite2(uint32_t w) {
@@ -179,9 +183,8 @@ __device__ __forceinline__ bool non_finite2(uint32_t w) {
 template <typename T, int kDim>
 __device__ __noinline__ void attend_row_exact(const AttendParams& a, const Piece& p, int row, float* o, float* m_out,
                                               float* l_out) {
-  const int group = a.heads / a.kv_heads, t = row / group, g = row - t * group;
-  const long long pos = p.span.start + t;
-  const Visible v = visible(a, pos, min(max(p.span.start + p.span.rows / group, 0ll), (long long)a.row_pages * a.page_size));
+  const int group = a.group, t = row / group, g = row - t * group;
+  const Visible v = visible(a, p.span.start + t, row_keys(a, p.b));
   const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + t * a.q_stride[1] + (p.h * group + g) * a.q_stride[2];
   const float sl = a.scale * 1.4426950408889634f;
   float m = -INFINITY, l = 0.0f;
@@ -190,9 +193,9 @@ __device__ __noinline__ void attend_row_exact(const AttendParams& a, const Piece
     const long long j0 = (long long)p.span.tile(i) * kKeyTile;
     for (long long j = j0; j < j0 + kKeyTile; ++j) {
       if (j >= v.hi || (j < v.lo && j >= a.sinks)) continue;
-      const int page = a.table[(long long)p.b * a.row_pages + j / a.page_size];
+      const int page = a.table[(long long)p.b * a.row_pages + (j >> a.page_shift)];
       if (page < 0 || page >= a.pages) continue;
-      const long long at = (((long long)page * a.kv_heads + p.h) * a.page_size + j % a.page_size) * a.dim;
+      const long long at = (((long long)page * a.kv_heads + p.h) * a.page_size + (j & (a.page_size - 1))) * a.dim;
       const T* k = static_cast<const T*>(a.pool[0]) + at;
       const T* vv = static_cast<const T*>(a.pool[1]) + at;
       float s = 0.0f;
@@ -229,7 +232,7 @@ struct AttendShared {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t s_full[2], p_full[2], o_full[2], q_full, q_empty, wg[2], both;
   PieceStart first;
-  long long warp_units[kAttThreads / 32], total;
+  long long warp_units[kAttThreads / 32], total, unit0;
   uint32_t tmem_base;
   int abort_flag;
   unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
@@ -260,8 +263,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   AttendShared& bar = *reinterpret_cast<AttendShared*>(sm_q + 224 * 1024);
   PieceStart& first = bar.first;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = a.heads / a.kv_heads;
-  const int q_tiles = (int)(((long long)a.tokens * group + Shape::kRows - 1) / Shape::kRows);
+  const int group = a.group;
+  const int q_tiles = (a.tokens * group + Shape::kRows - 1) / Shape::kRows;
 
   if (tid == 0) {
     bar.abort_flag = 0;
@@ -309,24 +312,28 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
     if (u0 >= u1) {
       if (tid == 0) {
-        first.unit = first.end = 0;
+        first.units = 0;
         work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
       }
     } else if (u0 >= before && u0 < before + mine) {
       long long at = before;
       for (int e = e0; e < e1; ++e) {
-        const long long n = (long long)tile_span(a, e / q_tiles, e % q_tiles, Shape::kRows).n * a.kv_heads;
-        if (u0 < at + n) {
-          first.unit = u0;
-          first.end = u1;
-          first.rem = u0 - at;
+        const int n = tile_span(a, e / q_tiles, e % q_tiles, Shape::kRows).n;
+        const long long rem = u0 - at;
+        if (rem < (long long)n * a.kv_heads) {
+          first.units = (int)(u1 - u0);
           first.e = e;
+          first.h = (int)(rem / n);
+          first.i0 = (int)(rem % n);
           break;
         }
-        at += n;
+        at += (long long)n * a.kv_heads;
       }
     }
-    if (tid == 0) bar.total = total;
+    if (tid == 0) {
+      bar.total = total;
+      bar.unit0 = u0;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -338,24 +345,26 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 
   if (warp == 8) {
     // ---------------------------------------------------------------- producer
-    const int pages_per_tile = kKeyTile / a.page_size;
+    const int pages_per_tile = kKeyTile >> a.page_shift;
     const uint32_t page_bytes = a.page_size * 128u;  // of one 64-value half
-    long long cnt = 0;
+    Ring<Shape::kStages> ring;
     bool ok = true;
     if (lane == 0) {
       prefetch_tmap(&map_k);
       prefetch_tmap(&map_v);
     }
-    auto load = [&](const CUtensorMap* map, int i) {
-      const int tile = p.span.tile(i);
-      const long long slot = (long long)tile * pages_per_tile + lane;
+    auto page_of = [&](int i) {
+      const int slot = p.span.tile(i) * pages_per_tile + lane;
       int page = -1;
-      if (lane < pages_per_tile && slot < a.row_pages && slot * a.page_size < p.span.hi) {
+      if (lane < pages_per_tile && slot < a.row_pages && (slot << a.page_shift) < p.span.hi) {
         page = a.table[(long long)p.b * a.row_pages + slot];
         if (page >= a.pages) page = -1;
       }
-      const int st = (int)(cnt % Shape::kStages);
-      ok = mbar_wait_bounded(&bar.empty[st], ((cnt / Shape::kStages) & 1) ^ 1, abort);
+      return page;
+    };
+    auto load = [&](const CUtensorMap* map, int page) {
+      const int st = ring.stage;
+      ok = mbar_wait_bounded(&bar.empty[st], ring.phase ^ 1, abort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
@@ -367,27 +376,35 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         for (int hf = 0; hf < Shape::kHalves; ++hf)
           tma_load_4d(dst + hf * 128 * 128, map, &bar.full[st], hf * 64, 0, p.h, page);
       }
-      ++cnt;
+      ring.next();
     };
+    // table entries are read one tile ahead of their use
     for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
-      const int n = p.i1 - p.i0;
       if (kPair) {
-        for (int i = 0; i < n && ok; ++i) {
-          load(&map_k, p.i0 + i);
-          if (ok) load(&map_v, p.i0 + i);
+        int page = page_of(p.i0);
+        for (int i = p.i0; i < p.i1 && ok; ++i) {
+          const int ahead = i + 1 < p.i1 ? page_of(i + 1) : -1;
+          load(&map_k, page);
+          if (ok) load(&map_v, page);
+          page = ahead;
         }
       } else {
-        load(&map_k, p.i0);
-        if (ok && n > 1) load(&map_k, p.i0 + 1);
-        for (int i = 0; i < n && ok; ++i) {
-          load(&map_v, p.i0 + i);
-          if (ok && i + 2 < n) load(&map_k, p.i0 + i + 2);
+        int page = page_of(p.i0), page1 = p.i0 + 1 < p.i1 ? page_of(p.i0 + 1) : -1;
+        load(&map_k, page);
+        if (ok && p.i0 + 1 < p.i1) load(&map_k, page1);
+        for (int i = p.i0; i < p.i1 && ok; ++i) {
+          const int ahead = i + 2 < p.i1 ? page_of(i + 2) : -1;
+          load(&map_v, page);
+          if (ok && i + 2 < p.i1) load(&map_k, ahead);
+          page = page1;
+          page1 = ahead;
         }
       }
     }
-    if (!ok) {  // leave no copy in flight behind this CTA
-      for (long long c = max(0ll, cnt - Shape::kStages); c < cnt; ++c)
-        for (int k = 0; k < 1000000 && !mbar_try_wait(&bar.full[c % Shape::kStages], (c / Shape::kStages) & 1); ++k) {
+    if (!ok) {  // leave no copy in flight behind this CTA: every stage's last load
+      Ring<Shape::kStages> r = ring;
+      for (int c = 0; c < Shape::kStages; ++c, r.next())
+        for (int k = 0; k < 1000000 && !mbar_try_wait(&bar.full[r.stage], r.phase ^ 1); ++k) {
         }
     }
   } else if (warp == 9) {
@@ -395,30 +412,32 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     if (lane == 0) {
       constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
       constexpr uint32_t idesc_s = idesc_f16(128, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
-      long long base = 0;
+      Ring<Shape::kStages> ring;
       uint32_t n_pieces = 0, n_p[2] = {0, 0};
       bool ok = true;
-      auto stage = [&](int idx) { return (int)((base + idx) % Shape::kStages); };
-      auto wait_load = [&](int idx) {
-        const long long c = base + idx;
-        ok = ok && mbar_wait_bounded(&bar.full[c % Shape::kStages], (c / Shape::kStages) & 1, abort);
+      // the stage of the next load, once it has landed
+      auto take = [&]() {
+        const int st = ring.stage;
+        ok = ok && mbar_wait_bounded(&bar.full[st], ring.phase, abort);
+        ring.next();
+        return st;
       };
-      auto qk = [&](int s, int idx) {
-        const uint32_t q = smem_u32(sm_q) + (kPair ? s * Shape::kTileBytes : 0);
-        const uint32_t k = smem_u32(sm_ring) + stage(idx) * Shape::kTileBytes;
+      const uint32_t ring0 = smem_u32(sm_ring), q0 = smem_u32(sm_q);
+      auto qk = [&](int s, int st) {
+        const uint64_t dq = smem_desc_k_sw128(q0 + (kPair ? s * Shape::kTileBytes : 0));
+        const uint64_t dk = smem_desc_k_sw128(ring0 + st * Shape::kTileBytes);
 #pragma unroll
         for (int d = 0; d < kDim / 16; ++d) {
-          const uint32_t off = (d / 4) * 128 * 128 + (d % 4) * 32;
-          mma_f16_ss(tmem + s * 128, smem_desc_k_sw128(q + off), smem_desc_k_sw128(k + off), idesc_s, d > 0);
+          const uint64_t off = ((d / 4) * 128 * 128 + (d % 4) * 32) >> 4;
+          mma_f16_ss(tmem + s * 128, dq + off, dk + off, idesc_s, d > 0);
         }
         mma_commit(&bar.s_full[s]);
       };
-      auto pv = [&](int s, int idx, bool accumulate) {
-        const uint32_t v = smem_u32(sm_ring) + stage(idx) * Shape::kTileBytes;
+      auto pv = [&](int s, int st, bool accumulate) {
+        const uint64_t dv = smem_desc_mn_sw128(ring0 + st * Shape::kTileBytes, 128 * 128);
 #pragma unroll
         for (int d = 0; d < kKeyTile / 16; ++d)
-          mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + d * 8, smem_desc_mn_sw128(v + d * 2048, 128 * 128),
-                     idesc_o, accumulate || d > 0);
+          mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + d * 8, dv + ((d * 2048) >> 4), idesc_o, accumulate || d > 0);
       };
       auto wait_p = [&](int s) {
         ok = ok && mbar_wait_bounded(&bar.p_full[s], n_p[s]++ & 1, abort);
@@ -430,27 +449,26 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         if (!ok) break;
         tc_fence_after();
         if (kPair) {
-          wait_load(load_index_k<true>(0));
+          int k = take(), v = 0;
           if (!ok) break;
-          qk(0, load_index_k<true>(0));
-          qk(1, load_index_k<true>(0));
-          mma_commit(&bar.empty[stage(load_index_k<true>(0))]);
+          qk(0, k);
+          qk(1, k);
+          mma_commit(&bar.empty[k]);
           if (n == 1) mma_commit(&bar.q_empty);
           for (int i = 0; i < n && ok; ++i) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
               wait_p(s);
-              const int iv = load_index_v<true>(i, n), ik = load_index_k<true>(i + 1);
-              if (s == 0) wait_load(iv);
+              if (s == 0 && ok) v = take();
               if (!ok) break;
-              pv(s, iv, i > 0);
-              if (s == 1) mma_commit(&bar.empty[stage(iv)]);
+              pv(s, v, i > 0);
+              if (s == 1) mma_commit(&bar.empty[v]);
               if (i + 1 < n) {
-                if (s == 0) wait_load(ik);
+                if (s == 0) k = take();
                 if (!ok) break;
-                qk(s, ik);
+                qk(s, k);
                 if (s == 1) {
-                  mma_commit(&bar.empty[stage(ik)]);
+                  mma_commit(&bar.empty[k]);
                   if (i + 2 == n) mma_commit(&bar.q_empty);
                 }
               } else {
@@ -460,31 +478,31 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           }
         } else {
           for (int s = 0; s < min(2, n) && ok; ++s) {
-            wait_load(load_index_k<false>(s));
+            const int k = take();
             if (!ok) break;
-            qk(s, load_index_k<false>(s));
-            mma_commit(&bar.empty[stage(load_index_k<false>(s))]);
+            qk(s, k);
+            mma_commit(&bar.empty[k]);
           }
           if (ok && n <= 2) mma_commit(&bar.q_empty);
           for (int i = 0; i < n && ok; ++i) {
-            const int s = i & 1, iv = load_index_v<false>(i, n), ik = load_index_k<false>(i + 2);
+            const int s = i & 1;
             wait_p(s);
-            wait_load(iv);
             if (!ok) break;
-            pv(s, iv, i >= 2);
-            mma_commit(&bar.empty[stage(iv)]);
+            const int v = take();
+            if (!ok) break;
+            pv(s, v, i >= 2);
+            mma_commit(&bar.empty[v]);
             if (i + 2 < n) {
-              wait_load(ik);
+              const int k = take();
               if (!ok) break;
-              qk(s, ik);
-              mma_commit(&bar.empty[stage(ik)]);
+              qk(s, k);
+              mma_commit(&bar.empty[k]);
               if (i + 3 == n) mma_commit(&bar.q_empty);
             } else {
               mma_commit(&bar.o_full[s]);
             }
           }
         }
-        base += 2 * n;
       }
     }
     __syncwarp();
@@ -500,7 +518,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     bool ok = true;
     for (; more; more = piece_next(a, p, q_tiles, Shape::kRows)) {
       if (p.i0 == 0 && p.i1 < p.span.n) {
-        const long long end = p.unit + p.span.n;
+        const long long end = bar.unit0 + (first.units - p.left) + p.span.n;
         int c = blockIdx.x + 1;
         while (total * (c + 1) / gridDim.x < end) ++c;
         // (with fewer tiles than CTAs some CTAs between are empty: the join needs the total)
@@ -540,7 +558,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       fence_proxy_async_shared();
       mbar_arrive(&bar.q_full);
     }
-    if (id == 0 && first.unit < first.end) work.head[blockIdx.x] = head;
+    if (id == 0 && first.units > 0) work.head[blockIdx.x] = head;
   } else {
     // ---------------------------------------------------------------- softmax, one thread per query row
     const int s = warp >> 2, row = tid & 127;
@@ -548,7 +566,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + lanes;
     const float sl = a.scale * 1.4426950408889634f;
     uint32_t n_s = 0, n_o[2] = {0, 0}, n_wg = 0, n_both = 0, n_pieces = 0;
-    long long base = 0;
+    int base = 0;  // loads before this piece, modulo two rounds of the ring
     bool ok = true;
     for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
       const int n = p.i1 - p.i0;
@@ -556,45 +574,49 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       const int tile0 = p.qt * Shape::kRows + (kPair ? s * 128 : 0), r = tile0 + row;
       const bool warp_live = tile0 + (warp & 3) * 32 < p.span.rows;
       // keys that the row sees: [lo, hi) and, below hi, [0, sinks)
-      const long long pos = p.span.start + r / group;
-      long long hi = 0, lo = 0;
+      int hi = 0, lo = 0;
       if (r < p.span.rows) {
+        const int pos = p.span.start + r / group;
         hi = a.causal ? min(p.span.hi, pos + 1) : p.span.hi;
-        lo = a.window > 0 ? max(pos - a.window + 1, 0ll) : 0;
+        lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
       }
       // rows of the item see all keys of [all_lo, all_hi)
-      const long long p_min = p.span.start + p.qt * Shape::kRows / group;
-      const long long p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * Shape::kRows) - 1) / group;
-      const long long all_hi = a.causal ? min(p.span.hi, p_min + 1) : p.span.hi;
-      const long long all_lo = a.window > 0 ? max(p_max - a.window + 1, 0ll) : 0;
+      const int p_min = p.span.start + p.qt * Shape::kRows / group;
+      const int p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * Shape::kRows) - 1) / group;
+      const int all_hi = a.causal ? min(p.span.hi, p_min + 1) : p.span.hi;
+      const int all_lo = a.window > 0 ? max(p_max - a.window + 1, 0) : 0;
       float m = -INFINITY, l = 0.0f;
       bool have_o = false;
-      for (int i = kPair ? 0 : s; i < n; i += kPair ? 1 : 2) {
+      constexpr int kStep = kPair ? 1 : 2;
+      int page = (kPair ? 0 : s) < n ? group_page(a, p.b, p.span.tile(p.i0 + (kPair ? 0 : s)), lane) : 0;
+      for (int i = kPair ? 0 : s; i < n; i += kStep) {
         const int tile = p.span.tile(p.i0 + i);
-        const long long key0 = (long long)tile * kKeyTile, key1 = key0 + kKeyTile;
-        const unsigned missing = key0 < p.span.hi ? missing_groups(a, p.b, tile, lane) : 0;
+        const int key0 = tile * kKeyTile, key1 = key0 + kKeyTile;
+        // 16-key groups without a page (read one tile ahead)
+        const unsigned missing = __ballot_sync(0xffffffffu, lane < 8 && (page < 0 || page >= a.pages));
+        if (i + kStep < n) page = group_page(a, p.b, p.span.tile(p.i0 + i + kStep), lane);
         const bool whole = missing == 0 && key1 <= all_hi && (key0 >= all_lo || key1 <= a.sinks);
         ok = mbar_wait_bounded(&bar.s_full[s], n_s++ & 1, abort);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          uint32_t x[128];
+          // bit k: the row sees key 32 c + k of the tile
+          auto see = [&](int c) {
+            const int k0 = key0 + 32 * c;
+            const uint32_t gap = (missing >> (2 * c) & 1) * 0xffffu | (missing >> (2 * c + 1) & 1) * 0xffff0000u;
+            return low_bits(hi - k0) & (~low_bits(lo - k0) | low_bits(a.sinks - k0)) & ~gap;
+          };
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            tmem_ld32(t_s + 32 * c, x);
+            tmem_ld_wait();
+            if (!whole) mask32(x, see(c));
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x + 32 * c);
-          tmem_ld_wait();
-          if (!whole) {
-            const int hi_c = (int)min(max(hi - key0, 0ll), 128ll), lo_c = (int)min(max(lo - key0, 0ll), 128ll);
-            const int sink_c = (int)min(max((long long)a.sinks - key0, 0ll), 128ll);
-#pragma unroll
-            for (int c = 0; c < 128; ++c) {
-              const bool see = c < hi_c && (c >= lo_c || c < sink_c) && !(missing >> (c / 16) & 1);
-              if (!see) x[c] = 0xff800000u;  // -inf
-            }
+            for (int k = 0; k < 32; ++k) top[k & 1] = fmaxf(top[k & 1], __uint_as_float(x[k]));
           }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c]));
-          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          const float mt = fmaxf(top[0], top[1]);
           const bool moves = (mt - m) * sl > 8.0f;
           if (__any_sync(0xffffffffu, moves)) {
             const float m1 = moves ? mt : m;
@@ -602,6 +624,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             l *= keep;
             m = m1;
             if (have_o) {
+#pragma unroll 1
               for (int c = 0; c < kDim; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(t_o + s * kDim + c, o);
@@ -614,34 +637,37 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           }
           have_o = true;
           const float sub = m == -INFINITY ? 0.0f : m * sl;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32], w[16];
+            tmem_ld32(t_s + 32 * c, x);
+            tmem_ld_wait();
+            if (!whole) mask32(x, see(c));
 #pragma unroll
-          for (int c = 0; c < 128; c += 64) {
-            uint32_t w[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float p0 = exp2_approx(__uint_as_float(x[c + 2 * k]) * sl - sub);
-              const float p1 = exp2_approx(__uint_as_float(x[c + 2 * k + 1]) * sl - sub);
-              sum[k & 1] += p0;
-              sum[2 + (k & 1)] += p1;
+            for (int k = 0; k < 16; ++k) {
+              const float p0 = exp2_approx(__uint_as_float(x[2 * k]) * sl - sub);
+              const float p1 = exp2_approx(__uint_as_float(x[2 * k + 1]) * sl - sub);
+              sum[0] += p0;
+              sum[1] += p1;
               w[k] = pack2<T>(p0, p1);
             }
-            tmem_st32(t_s + c / 2, w);
+            tmem_st16(t_s + 16 * c, w);  // over scores that have been read
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          l += sum[0] + sum[1];
           tmem_st_wait();
         }
         if (!whole) {
-          const long long c = base + load_index_v<kPair>(i, n);
-          const int st = (int)(c % Shape::kStages);
-          ok = mbar_wait_bounded(&bar.full[st], (c / Shape::kStages) & 1, abort);
+          const int c = (base + load_index_v<kPair>(i, n)) % (2 * Shape::kStages);
+          const int st = c % Shape::kStages;
+          ok = mbar_wait_bounded(&bar.full[st], c / Shape::kStages, abort);
           if (!ok) break;
           // this thread's key: zero if no row of the item sees it; non-finite values that some rows see
-          const long long j = key0 + row;
+          const int j = key0 + row;
           unsigned char* v = sm_ring + st * Shape::kTileBytes + row * 128;
           const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (row / 16) & 1);
           if (!seen) {
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < Shape::kHalves; ++hf)
 #pragma unroll
               for (int k = 0; k < 8; ++k)
@@ -649,7 +675,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             fence_proxy_async_shared();
           } else if (j >= all_hi || (j < all_lo && j >= a.sinks)) {
             bool odd = false;
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < Shape::kHalves; ++hf)
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
@@ -768,7 +794,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
       }
-      base += 2 * n;
+      base = (base + 2 * n) % (2 * Shape::kStages);
     }
   }
   tc_fence_before();
@@ -782,54 +808,63 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 }
 
 // The items that cross CTAs: CTA c's record names an item whose first tiles it
-// holds; the rest is in slot 0 of the CTAs behind it.  A block takes 16 rows
-// (4 warps, 4 rows each).  Also the rows that no item covers: behind the end
-// of a short chunk, or with no key to see.
-constexpr int kJoinRows = 16;
+// holds; the rest is in slot 0 of the CTAs behind it.  One warp per row: the
+// lanes read the pieces' (m, l) side by side, then the row is added up piece by
+// piece with several loads in flight.  Also the rows that no item covers:
+// behind the end of a short chunk, or with no key to see.
+constexpr int kJoinRows = 8;
 template <typename T, int kDim, bool kPair>
-__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendParams a,
-                                                          const __grid_constant__ AttendWork work) {
+__global__ void __launch_bounds__(32 * kJoinRows) attend_join_kernel(const __grid_constant__ AttendParams a,
+                                                                     const __grid_constant__ AttendWork work) {
   constexpr int kRows = AttendShape<kDim, kPair>::kRows;
+  constexpr int kVec = kDim / 32;  // values per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.heads / a.kv_heads;
-  const int q_tiles = (int)(((long long)a.tokens * group + kRows - 1) / kRows);
+  const int group = a.group;
+  const int q_tiles = (a.tokens * group + kRows - 1) / kRows;
   pdl_wait_primary();
   const int4 head = work.head[blockIdx.x];
   if (head.x >= 0) {
     const int b = head.x / q_tiles, qt = head.x - b * q_tiles, h = head.y, c0 = blockIdx.x, c1 = head.z;
     const int rows = (int)(a.lens ? min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens) * group;
-    // CTAs without a tile (fewer tiles than CTAs) have left nothing
-    auto empty = [&](int c) {
-      return head.w > 0 && (long long)head.w * c / gridDim.x == (long long)head.w * (c + 1) / gridDim.x;
-    };
-    for (int k = warp; k < kJoinRows; k += 4) {
-      const int row = blockIdx.y * kJoinRows + k, r = qt * kRows + row;
-      if (r >= a.tokens * group) break;
-      const int t = r / group, g = r - t * group;
-      T* out = static_cast<T*>(a.out) + (((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim;
-      float o[kDim / 32] = {};
-      float top = -INFINITY, l = 0.0f;
-      if (r < rows) {
-        for (int c = c0 + lane; c <= c1; c += 32)
-          if (!empty(c)) top = fmaxf(top, work.ml[(2 * (size_t)c + (c == c0)) * kRows + row].x);
+    const int row = blockIdx.y * kJoinRows + warp, r = qt * kRows + row;
+    if (r < a.tokens * group) {
+      float o[kVec] = {};
+      float m = -INFINITY, l = 0.0f;
+      for (int c = c0; r < rows && c <= c1; c += 32) {
+        // 32 pieces; CTAs without a tile (fewer tiles than CTAs) have left nothing
+        const int mine = c + lane;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (mine <= c1 && !(head.w > 0 && head.w * mine / (int)gridDim.x == head.w * (mine + 1) / (int)gridDim.x))
+          ml = work.ml[(2 * (size_t)mine + (mine == c0)) * kRows + row];
+        float top = ml.x;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        for (int c = c0; c <= c1; ++c) {
-          if (empty(c)) continue;
-          const size_t slot = 2 * (size_t)c + (c == c0);
-          const float2 ml = work.ml[slot * kRows + row];
-          const float* part = work.o + (slot * kRows + row) * kDim;
-          if (ml.y == 0.0f) continue;  // the piece holds no key that this row sees
-          const float w = exp2_approx(ml.x - (top == -INFINITY ? 0.0f : top));
-          l += ml.y * w;
+        const float m1 = fmaxf(m, top), base = m1 == -INFINITY ? 0.0f : m1;
+        const float keep = exp2_approx(m - base);
+        const float w = ml.y == 0.0f ? 0.0f : exp2_approx(ml.x - base);  // l = 0: no key of the piece is seen
+        float sum = ml.y * w;
 #pragma unroll
-          for (int i = 0; i < kDim / 32; ++i) o[i] += part[lane + 32 * i] * w;
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l = l * keep + sum;
+        m = m1;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) o[i] *= keep;
+        const int pieces = min(32, c1 - c + 1);
+#pragma unroll 4
+        for (int k = 0; k < pieces; ++k) {
+          const float wk = __shfl_sync(0xffffffffu, w, k);
+          if (wk == 0.0f) continue;
+          const float* part = work.o + ((2 * (size_t)(c + k) + (c + k == c0)) * kRows + row) * kDim + lane * kVec;
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) o[i] += part[i] * wk;
         }
       }
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int t = r / group, g = r - t * group;
+      T* out = static_cast<T*>(a.out) + (((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + lane * kVec;
+      if (lane * kVec < a.dim)
 #pragma unroll
-      for (int i = 0; i < kDim / 32; ++i)
-        if (lane + 32 * i < a.dim) out[lane + 32 * i] = io<T>::from_f(o[i] * inv);
+        for (int i = 0; i < kVec; ++i) out[i] = io<T>::from_f(o[i] * inv);
     }
   }
   const int blocks = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
@@ -839,7 +874,7 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
     const int r1 = min((qt + 1) * kRows, a.tokens * group);
     for (int r = qt * kRows; r < r1; ++r) {
       const int t = r / group, g = r - t * group;
-      for (int i = threadIdx.x; i < a.kv_heads * a.dim; i += 128) {
+      for (int i = threadIdx.x; i < a.kv_heads * a.dim; i += 32 * kJoinRows) {
         const int h = i / a.dim, d = i - h * a.dim;
         static_cast<T*>(a.out)[(((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + d] = io<T>::from_f(0.0f);
       }

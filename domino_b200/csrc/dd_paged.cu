@@ -79,6 +79,8 @@ int check_shape(const dd_paged_cache* c) {
     return global_fail(DD_EINVAL, "paged cache: pages x kv_heads must stay below 2^31");
   if ((long long)c->batch * c->row_pages > 0x7fffffffll)
     return global_fail(DD_EINVAL, "paged cache: batch x row_pages must stay below 2^31");
+  if ((long long)c->row_pages * c->page_size > (1ll << 30))
+    return global_fail(DD_EINVAL, "paged cache: a row holds at most 2^30 tokens");
   return DD_OK;
 }
 
@@ -237,7 +239,7 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, con
   w.ml = reinterpret_cast<float2*>(w.o + (size_t)dev.sms * 2 * kRows * kDim);
   rc = launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(dev.sms), dim3(kAttThreads), kAttSmem, stream, mk, mv, p, w);
   if (rc) return rc;
-  return launch("attend join", attend_join_kernel<T, kDim, kPair>, dim3(dev.sms, kRows / kJoinRows), dim3(128), 0, stream,
+  return launch("attend join", attend_join_kernel<T, kDim, kPair>, dim3(dev.sms, kRows / kJoinRows), dim3(32 * kJoinRows), 0, stream,
                 p, w);
 }
 template <typename T>
@@ -261,7 +263,7 @@ int check_attend(const dd_paged_cache* c, const dd_cache_attend_args* a) {
   if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return global_fail(DD_EINVAL, "cache attend: scale must be positive");
   if (a->window < 0 || a->sinks < 0 || (a->window == 0 && a->sinks > 0) || (a->window > 0 && !a->causal))
     return global_fail(DD_EINVAL, "cache attend: a window needs causal attention, sinks need a window");
-  if ((long long)a->tokens * (a->heads / c->kv_heads) > 0x3fffffffll || (long long)a->heads * c->head_dim > 0x7fffffffll)
+  if ((long long)a->tokens * (a->heads / c->kv_heads) > (1ll << 29) || (long long)a->heads * c->head_dim > 0x7fffffffll)
     return global_fail(DD_EINVAL, "cache attend: chunk too large");
   return DD_OK;
 }
@@ -418,13 +420,16 @@ int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void
   p.tokens = a->tokens;
   p.heads = a->heads;
   p.kv_heads = c->kv_heads;
+  p.group = a->heads / c->kv_heads;
   p.dim = c->head_dim;
   p.pages = c->pages;
   p.page_size = c->page_size;
+  while (1 << p.page_shift < c->page_size) ++p.page_shift;
   p.row_pages = c->row_pages;
   p.causal = a->causal != 0;
-  p.window = a->window;
-  p.sinks = a->sinks;
+  // nothing is further away than 2^30 positions
+  p.window = std::min(a->window, 1 << 30);
+  p.sinks = std::min(a->sinks, 1 << 30);
   p.status = c->status;
   const AttendPlan plan = attend_plan(c, a);
   if (plan.tensor) {
