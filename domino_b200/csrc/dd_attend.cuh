@@ -24,6 +24,7 @@ struct AttendParams {
   float scale;
   int batch, tokens, heads, kv_heads, dim, pages, page_size, page_shift, row_pages;  // page_size = 1 << page_shift
   int group;                 // query heads per key head
+  int copies;                // copies of the rows in a query tile of the tensor-core kernel: 1, 2 or 4
   int causal, window, sinks;
 };
 

@@ -43,6 +43,7 @@ namespace dd {
 constexpr int kAttThreads = 384;  // 8 softmax warps, TMA producer, MMA issuer, 2 query loaders
 constexpr int kKeyTile = 128;
 constexpr int kMaxStages = 12;
+constexpr int kMergeCols = 16, kMergeStride = kMergeCols + 1;  // of the buffer that joins streams and copies of rows
 
 struct AttendWork {
   int4* head;    // [grid]: item {entry, key head, last CTA} whose first piece this CTA holds and does not finish; entry -1: none
@@ -90,24 +91,10 @@ struct Piece {
   int left;                 // tiles of the run from i0 on
   TileSpan span;
 };
-struct PieceStart {
-  int units, e, h, i0;  // tiles of the run, and where it starts
-};
 __device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
   p.b = p.e / q_tiles;
   p.qt = p.e - p.b * q_tiles;
   p.span = tile_span(a, p.b, p.qt, tile_rows);
-}
-__device__ __forceinline__ bool piece_first(const AttendParams& a, const PieceStart& s, Piece& p, int q_tiles,
-                                            int tile_rows) {
-  p.left = s.units;
-  if (p.left == 0) return false;
-  p.e = s.e;
-  p.h = s.h;
-  p.i0 = s.i0;
-  piece_enter(a, p, q_tiles, tile_rows);
-  p.i1 = min(p.span.n, p.i0 + p.left);
-  return true;
 }
 __device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
   p.left -= p.i1 - p.i0;
@@ -122,6 +109,12 @@ __device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int 
   p.i0 = 0;
   p.i1 = min(p.span.n, p.left);
   return true;
+}
+
+// Where CTA c's run starts: c / grid of all tiles.
+__device__ __forceinline__ long long run_start(long long total, unsigned c, unsigned grid) {
+  if (total < 1 << 23 && grid < 256) return (unsigned)total * c / grid;  // 32-bit division
+  return total * c / grid;
 }
 
 // The ring of key and value tiles.  Tiles are loaded in the order in which the
@@ -222,21 +215,22 @@ struct AttendShape {
   static constexpr int kRows = 128 * kTiles;
   static constexpr int kHalves = kDim / 64;
   static constexpr int kTileBytes = 128 * kDim * 2;  // a query tile, a K or V tile
-  static constexpr int kStages = (224 * 1024 - kTiles * kTileBytes) / kTileBytes < kMaxStages
-                                     ? (224 * 1024 - kTiles * kTileBytes) / kTileBytes
-                                     : kMaxStages;
+  static constexpr int kMergeBytes = kPair ? 0 : 2 * 128 * kMergeStride * 4;
+  static constexpr int kFit = (224 * 1024 - kTiles * kTileBytes - kMergeBytes) / kTileBytes;
+  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
 };
 
 // Behind the tiles in shared memory.
 struct AttendShared {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t s_full[2], p_full[2], o_full[2], q_full, q_empty, wg[2], both;
-  PieceStart first;
+  Piece first;          // where the run starts; left = 0: the CTA has none
   long long warp_units[kAttThreads / 32], total, unit0;
   uint32_t tmem_base;
   int abort_flag;
   unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
   float2 row_ml[2][128];
+  float row_norm[128];
 };
 // All of the 227 KB; the tiles start on a 1024-byte boundary, and there is
 // room for the padding that takes (the window starts on one: none).
@@ -261,7 +255,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   unsigned char* sm_q = smem_raw + pad;
   unsigned char* sm_ring = sm_q + Shape::kTiles * Shape::kTileBytes;
   AttendShared& bar = *reinterpret_cast<AttendShared*>(sm_q + 224 * 1024);
-  PieceStart& first = bar.first;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.group;
   const int q_tiles = (a.tokens * group + Shape::kRows - 1) / Shape::kRows;
@@ -285,16 +278,24 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc(&bar.tmem_base, 512);
+  if (tid == 32 * 8) {
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
+  }
   pdl_wait_primary();
 
   // the CTA's run of tiles
   {
     const int entries = a.batch * q_tiles, per = (entries + kAttThreads - 1) / kAttThreads;
     const int e0 = tid * per, e1 = min(entries, e0 + per);
-    long long mine = 0;
-    for (int e = e0; e < e1; ++e) mine += tile_span(a, e / q_tiles, e % q_tiles, Shape::kRows).n;
-    mine *= a.kv_heads;
-    long long inc = mine;
+    Piece mine;
+    long long units = 0;
+    for (mine.e = e0; mine.e < e1; ++mine.e) {
+      piece_enter(a, mine, q_tiles, Shape::kRows);
+      units += mine.span.n;
+    }
+    units *= a.kv_heads;
+    long long inc = units;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long o = __shfl_up_sync(0xffffffffu, inc, d);
@@ -308,31 +309,31 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       if (w < warp) before += bar.warp_units[w];
       total += bar.warp_units[w];
     }
-    before += inc - mine;
-    const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
-    if (u0 >= u1) {
-      if (tid == 0) {
-        first.units = 0;
-        work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
-      }
-    } else if (u0 >= before && u0 < before + mine) {
-      long long at = before;
-      for (int e = e0; e < e1; ++e) {
-        const int n = tile_span(a, e / q_tiles, e % q_tiles, Shape::kRows).n;
-        const long long rem = u0 - at;
-        if (rem < (long long)n * a.kv_heads) {
-          first.units = (int)(u1 - u0);
-          first.e = e;
-          first.h = (int)(rem / n);
-          first.i0 = (int)(rem % n);
-          break;
-        }
-        at += (long long)n * a.kv_heads;
-      }
-    }
+    before += inc - units;
+    const long long u0 = run_start(total, blockIdx.x, gridDim.x), u1 = run_start(total, blockIdx.x + 1, gridDim.x);
     if (tid == 0) {
       bar.total = total;
       bar.unit0 = u0;
+    }
+    if (u0 >= u1) {
+      if (tid == 0) {
+        bar.first.left = 0;
+        work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      }
+    } else if (u0 >= before && u0 < before + units) {
+      // the run starts in this thread's entries (one entry as a rule: its span is still here)
+      long long rem = u0 - before;
+      for (mine.e = e0; mine.e < e1; ++mine.e) {
+        if (per > 1) piece_enter(a, mine, q_tiles, Shape::kRows);
+        const long long n = (long long)mine.span.n * a.kv_heads;
+        if (rem < n) break;
+        rem -= n;
+      }
+      mine.h = (int)rem / mine.span.n;  // rem < n tiles x heads of one entry
+      mine.i0 = (int)rem - mine.h * mine.span.n;
+      mine.left = (int)(u1 - u0);
+      mine.i1 = min(mine.span.n, mine.i0 + mine.left);
+      bar.first = mine;
     }
     tc_fence_before();
     __syncthreads();
@@ -340,8 +341,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   }
   const uint32_t tmem = bar.tmem_base;
   volatile int* abort = &bar.abort_flag;
-  Piece p;
-  bool more = piece_first(a, first, p, q_tiles, Shape::kRows);
+  Piece p = bar.first;
+  bool more = p.left > 0;
 
   if (warp == 8) {
     // ---------------------------------------------------------------- producer
@@ -349,10 +350,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     const uint32_t page_bytes = a.page_size * 128u;  // of one 64-value half
     Ring<Shape::kStages> ring;
     bool ok = true;
-    if (lane == 0) {
-      prefetch_tmap(&map_k);
-      prefetch_tmap(&map_v);
-    }
     auto page_of = [&](int i) {
       const int slot = p.span.tile(i) * pages_per_tile + lane;
       int page = -1;
@@ -508,57 +505,52 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     __syncwarp();
   } else if (warp >= 10) {
     // ---------------------------------------------------------------- query loader, and the record for the join
+    // 16-byte asynchronous copies, all of a piece's in flight at once; a thread
+    // keeps one chunk of the row and steps through the rows.
     const int id = tid - 320;
-    constexpr int kChunks = kDim / 8;  // 16-byte chunks of a row
+    constexpr int kChunks = kDim / 8, kRowStep = 64 / kChunks;
+    const int ch = id % kChunks;
     const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0 &&
                      a.q_stride[2] % 8 == 0;
-    const long long total = bar.total;
+    const int copy_rows = kPair ? Shape::kRows : 128 / a.copies;
     uint32_t n_pieces = 0;
     int4 head = make_int4(-1, 0, 0, 0);
     bool ok = true;
     for (; more; more = piece_next(a, p, q_tiles, Shape::kRows)) {
-      if (p.i0 == 0 && p.i1 < p.span.n) {
-        const long long end = bar.unit0 + (first.units - p.left) + p.span.n;
-        int c = blockIdx.x + 1;
-        while (total * (c + 1) / gridDim.x < end) ++c;
-        // (with fewer tiles than CTAs some CTAs between are empty: the join needs the total)
-        head = make_int4(p.e, p.h, c, total < gridDim.x ? (int)total : 0);
-      }
       ok = mbar_wait_bounded(&bar.q_empty, (n_pieces++ & 1) ^ 1, abort);
       if (!ok) break;
       const int r0 = p.qt * Shape::kRows, live = min(Shape::kRows, p.span.rows - r0);
-      const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0];
-      for (int c0 = id; c0 < live * kChunks; c0 += 64 * 8) {
-        uint4 v[8];
+      const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + (long long)p.h * group * a.q_stride[2] + ch * 8;
+      int row = id / kChunks, t = (r0 + row) / group, g = r0 + row - t * group;
+      for (; row < live; row += kRowStep) {
+        const T* src = q + t * a.q_stride[1] + g * a.q_stride[2];
+        const bool in = ch * 8 < a.dim;
+        for (int to = row; to < (kPair ? row + 1 : 128); to += copy_rows) {
+          unsigned char* dst = sm_q + (to / 128) * Shape::kTileBytes + (ch / 8) * 128 * 128 + (to % 128) * 128 +
+                               ((ch % 8) ^ (to % 8)) * 16;
+          if (vec) {
+            cp_async16(dst, in ? src : a.q, in ? 16 : 0);
+          } else {
+            alignas(16) T x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int c = c0 + 64 * k, row = c / kChunks, ch = c % kChunks;
-          v[k] = make_uint4(0, 0, 0, 0);
-          if (row < live && ch * 8 < a.dim) {
-            const int t = (r0 + row) / group, g = (r0 + row) - t * group;
-            const T* src = q + t * a.q_stride[1] + (p.h * group + g) * a.q_stride[2] + ch * 8;
-            if (vec) {
-              v[k] = *reinterpret_cast<const uint4*>(src);
-            } else {
-              alignas(16) T x[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] = src[i];
-              v[k] = *reinterpret_cast<const uint4*>(x);
-            }
+            for (int i = 0; i < 8; ++i) x[i] = in ? src[i] : io<T>::from_f(0.0f);
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
           }
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int c = c0 + 64 * k, row = c / kChunks, ch = c % kChunks;
-          if (row < live)
-            *reinterpret_cast<uint4*>(sm_q + (row / 128) * Shape::kTileBytes + (ch / 8) * 128 * 128 + (row % 128) * 128 +
-                                      ((ch % 8) ^ (row % 8)) * 16) = v[k];
-        }
+        for (g += kRowStep; g >= group; g -= group) ++t;
       }
+      cp_async_wait_all();
       fence_proxy_async_shared();
       mbar_arrive(&bar.q_full);
+      if (id == 0 && p.i0 == 0 && p.i1 < p.span.n) {
+        const long long end = bar.unit0 + (bar.first.left - p.left) + p.span.n;
+        int c = blockIdx.x + 1;
+        while (run_start(bar.total, c + 1, gridDim.x) < end) ++c;
+        // (with fewer tiles than CTAs some CTAs between are empty: the join needs the total)
+        head = make_int4(p.e, p.h, c, bar.total < gridDim.x ? (int)bar.total : 0);
+      }
     }
-    if (id == 0 && first.units > 0) work.head[blockIdx.x] = head;
+    if (id == 0 && bar.first.left > 0) work.head[blockIdx.x] = head;
   } else {
     // ---------------------------------------------------------------- softmax, one thread per query row
     const int s = warp >> 2, row = tid & 127;
@@ -568,11 +560,16 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     uint32_t n_s = 0, n_o[2] = {0, 0}, n_wg = 0, n_both = 0, n_pieces = 0;
     int base = 0;  // loads before this piece, modulo two rounds of the ring
     bool ok = true;
+    // Few rows: the tile holds `copies` copies of them, and copy c of a row
+    // takes part c of the tile's keys (P is zero elsewhere), so that all four
+    // warps share the exponentials.  The copies are joined like the streams.
+    const int copies = kPair ? 1 : a.copies, copy_rows = 128 / copies;
+    const int chunk0 = (row / copy_rows) * (4 / copies), chunk1 = chunk0 + 4 / copies;
     for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
       const int n = p.i1 - p.i0;
       ++n_pieces;
-      const int tile0 = p.qt * Shape::kRows + (kPair ? s * 128 : 0), r = tile0 + row;
-      const bool warp_live = tile0 + (warp & 3) * 32 < p.span.rows;
+      const int tile0 = p.qt * Shape::kRows + (kPair ? s * 128 : 0), r = tile0 + (kPair ? row : row % copy_rows);
+      const bool warp_live = r - lane < p.span.rows;
       // keys that the row sees: [lo, hi) and, below hi, [0, sinks)
       int hi = 0, lo = 0;
       if (r < p.span.rows) {
@@ -608,7 +605,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           };
           float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int c = chunk0; c < chunk1; ++c) {
             uint32_t x[32];
             tmem_ld32(t_s + 32 * c, x);
             tmem_ld_wait();
@@ -639,7 +636,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           const float sub = m == -INFINITY ? 0.0f : m * sl;
           float sum[2] = {0.0f, 0.0f};
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int c = chunk0; c < chunk1; ++c) {
             uint32_t x[32], w[16];
             tmem_ld32(t_s + 32 * c, x);
             tmem_ld_wait();
@@ -655,6 +652,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             tmem_st16(t_s + 16 * c, w);  // over scores that have been read
           }
           l += sum[0] + sum[1];
+          if (!kPair && copies > 1) {  // the other copies' keys
+            const uint32_t zero[16] = {};
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c)
+              if (c < chunk0 || c >= chunk1) tmem_st16(t_s + 16 * c, zero);
+          }
           tmem_st_wait();
         }
         if (!whole) {
@@ -662,28 +665,29 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           const int st = c % Shape::kStages;
           ok = mbar_wait_bounded(&bar.full[st], c / Shape::kStages, abort);
           if (!ok) break;
-          // this thread's key: zero if no row of the item sees it; non-finite values that some rows see
-          const int j = key0 + row;
-          unsigned char* v = sm_ring + st * Shape::kTileBytes + row * 128;
-          const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (row / 16) & 1);
-          if (!seen) {
+          // keys that no row of the item sees become zero; those that only some see are searched.
+          // Eight lanes a 128-byte row, four rows a step, 32 keys a warp.
+          unsigned char* v = sm_ring + st * Shape::kTileBytes + (lane % 8) * 16;
+          bool odd = false, wrote = false;
 #pragma unroll 1
-            for (int hf = 0; hf < Shape::kHalves; ++hf)
+          for (int k = (warp & 3) * 32 + lane / 8, k1 = k + 32; k < k1; k += 4) {
+            const int j = key0 + k;
+            const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (k / 16) & 1);
+            const bool search = seen && (j >= all_hi || (j < all_lo && j >= a.sinks));
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                *reinterpret_cast<uint4*>(v + hf * 128 * 128 + k * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_shared();
-          } else if (j >= all_hi || (j < all_lo && j >= a.sinks)) {
-            bool odd = false;
-#pragma unroll 1
-            for (int hf = 0; hf < Shape::kHalves; ++hf)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const uint4 w = *reinterpret_cast<const uint4*>(v + hf * 128 * 128 + k * 16);
+            for (int hf = 0; hf < Shape::kHalves; ++hf) {
+              uint4* at = reinterpret_cast<uint4*>(v + hf * 128 * 128 + k * 128);
+              if (!seen) {
+                *at = make_uint4(0, 0, 0, 0);
+                wrote = true;
+              } else if (search) {
+                const uint4 w = *at;
                 odd = odd || non_finite2<T>(w.x) || non_finite2<T>(w.y) || non_finite2<T>(w.z) || non_finite2<T>(w.w);
               }
-            if (odd) bar.redo[s] = n_pieces;
+            }
           }
+          if (wrote) fence_proxy_async_shared();
+          if (odd) bar.redo[s] = n_pieces;
         }
         tc_fence_before();
         mbar_arrive(&bar.p_full[s]);
@@ -692,13 +696,16 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       // the piece's result
       const bool split = p.i0 > 0 || p.i1 < p.span.n;
       const size_t slot = 2 * (size_t)blockIdx.x + (p.i0 == 0 ? 1 : 0);
-      const int t = r / group, g = r - t * group;
-      const bool in_chunk = r < a.tokens * group;
-      T* out = static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * group + g) * a.dim;
-      const int slot_row = (kPair ? s * 128 : 0) + row;
-      float* part = work.o + (slot * Shape::kRows + slot_row) * kDim;
-      float f[2], inv;
+      const int slot_row = kPair ? s * 128 + row : row;
+      float* part = work.o + slot * Shape::kRows * kDim;
+      float2* part_ml = work.ml + slot * Shape::kRows;
+      auto out_row = [&](int r) {
+        const int t = r / group, g = r - t * group;
+        return static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * group + g) * a.dim;
+      };
       bool again;
+      float f0 = 1.0f, f1 = 0.0f;  // weights of the streams' sums (kPair: only its own)
+      if (m != -INFINITY) m *= sl;
       if (kPair) {
         ok = mbar_wait_bounded(&bar.o_full[s], n_o[s]++ & 1, abort);
         if (!ok) break;
@@ -709,84 +716,121 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         mbar_arrive(&bar.wg[s]);
         ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
         if (!ok) break;
-        f[0] = f[1] = 1.0f;
       } else {
-        bar.row_ml[s][row] = make_float2(m == -INFINITY ? -INFINITY : m * sl, l);
+        bar.row_ml[s][row] = make_float2(m, l);
         ok = mbar_wait_bounded(&bar.o_full[0], n_o[0]++ & 1, abort);
         if (ok && n > 1) ok = mbar_wait_bounded(&bar.o_full[1], n_o[1]++ & 1, abort);
         if (!ok) break;
         mbar_arrive(&bar.both);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
-        const float2 x0 = bar.row_ml[0][row], x1 = bar.row_ml[1][row];
         again = bar.redo[0] == n_pieces || bar.redo[1] == n_pieces;
-        const float top = fmaxf(x0.x, x1.x);
-        f[0] = x0.x == -INFINITY ? 0.0f : exp2_approx(x0.x - top);
-        f[1] = x1.x == -INFINITY ? 0.0f : exp2_approx(x1.x - top);
-        l = x0.y * f[0] + x1.y * f[1];
-        m = top;
+        const float m0 = bar.row_ml[0][row].x, m1 = bar.row_ml[1][row].x;
+        m = -INFINITY;
+        for (int c = row % copy_rows; c < 128; c += copy_rows) m = fmaxf(m, fmaxf(bar.row_ml[0][c].x, bar.row_ml[1][c].x));
+        l = 0.0f;
+        for (int c = row % copy_rows; c < 128; c += copy_rows)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = bar.row_ml[k][c];
+            if (x.y != 0.0f) l += x.y * exp2_approx(x.x - m);
+          }
+        f0 = m0 == -INFINITY ? 0.0f : exp2_approx(m0 - m);
+        f1 = m1 == -INFINITY ? 0.0f : exp2_approx(m1 - m);
       }
       tc_fence_after();
-      if (kPair && m != -INFINITY) m *= sl;
-      inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (again) {
-        // (both streams' rows are the same without kPair: the first does them)
-        if ((kPair || s == 0) && in_chunk) {
+        if ((kPair || (s == 0 && row < copy_rows)) && r < a.tokens * group) {
           const Piece here = p;
-          float o[kDim];
-          float m_x = -INFINITY, l_x = 0.0f;
+          float o[kDim], m_x = -INFINITY, l_x = 0.0f;
           for (int d = 0; d < kDim; ++d) o[d] = 0.0f;
           if (r < p.span.rows) attend_row_exact<T, kDim>(a, here, r, o, &m_x, &l_x);
-          inv = l_x == 0.0f ? 0.0f : 1.0f / l_x;
+          const float inv_x = l_x == 0.0f ? 0.0f : 1.0f / l_x;
           if (split) {
-            for (int d = 0; d < kDim; ++d) part[d] = o[d];
-            work.ml[slot * Shape::kRows + slot_row] = make_float2(m_x, l_x);
+            for (int d = 0; d < kDim; ++d) part[(size_t)slot_row * kDim + d] = o[d];
+            part_ml[slot_row] = make_float2(m_x, l_x);
           } else {
-            for (int d = 0; d < a.dim; ++d) out[d] = io<T>::from_f(r < p.span.rows ? o[d] * inv : 0.0f);
+            T* out = out_row(r);
+            for (int d = 0; d < a.dim; ++d) out[d] = io<T>::from_f(r < p.span.rows ? o[d] * inv_x : 0.0f);
           }
         }
-      } else {
-        if (split && (kPair || s == 0)) work.ml[slot * Shape::kRows + slot_row] = make_float2(m, l);
+      } else if (kPair) {
+        const bool in_chunk = r < a.tokens * group, live = r < p.span.rows;
+        if (split) part_ml[slot_row] = make_float2(m, l);
         const float norm = split ? 1.0f : inv;
-        const int c_begin = kPair ? 0 : s * (kDim / 2), c_end = kPair ? kDim : c_begin + kDim / 2;
-        const float f0 = f[0] * norm, f1 = f[1] * norm;
+        T* out = out_row(r);
 #pragma unroll 1
-        for (int c = c_begin; c < c_end; c += 32) {
-          float o[32];
+        for (int c = 0; c < kDim; c += 32) {
+          uint32_t x[32];
           if (warp_live) {
-            uint32_t x[32];
-            tmem_ld32(t_o + (kPair ? s * kDim : 0) + c, x);
+            tmem_ld32(t_o + s * kDim + c, x);
             tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = f0 == 0.0f ? 0.0f : __uint_as_float(x[k]) * f0;
-            if (!kPair && n > 1) {
-              tmem_ld32(t_o + kDim + c, x);
-              tmem_ld_wait();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] += f1 == 0.0f ? 0.0f : __uint_as_float(x[k]) * f1;
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = 0.0f;
           }
           if (!in_chunk) continue;
+          float o[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = live && norm != 0.0f ? __uint_as_float(x[k]) * norm : 0.0f;
           if (split) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              *reinterpret_cast<float4*>(part + (size_t)slot_row * kDim + c + k) =
+                  make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           } else {
-            const bool live = r < p.span.rows;
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              if (c + k >= a.dim) break;
-              uint4 w = make_uint4(0, 0, 0, 0);
-              if (live)
-                w = make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),
+            for (int k = 0; k < 32; k += 8)
+              if (c + k < a.dim)
+                *reinterpret_cast<uint4*>(out + c + k) =
+                    make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),
                                pack2<T>(o[k + 6], o[k + 7]));
-              *reinterpret_cast<uint4*>(out + c + k) = w;
-            }
           }
         }
+      } else {
+        // Each stream's warps take half of the columns, 16 at a time: both
+        // streams' sums by row, the copies of a row through shared memory, and
+        // out with four lanes a row.
+        if (split && s == 0 && row < copy_rows) part_ml[row] = make_float2(m, l);
+        bar.row_norm[row] = inv;  // (both streams and all copies write the same)
+        float* merge = reinterpret_cast<float*>(sm_q + 224 * 1024 - Shape::kMergeBytes) + s * 128 * kMergeStride;
+        const int rows = min(p.span.rows, copy_rows), all_rows = min(a.tokens * group, copy_rows);
+#pragma unroll 1
+        for (int c = s * (kDim / 2); c < (s + 1) * (kDim / 2); c += kMergeCols) {
+          if (warp_live) {
+            uint32_t x[16], y[16];
+            tmem_ld16u(t_o + c, x);
+            if (n > 1) tmem_ld16u(t_o + kDim + c, y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float o = __uint_as_float(x[k]) * f0;
+              if (n > 1) o += __uint_as_float(y[k]) * f1;
+              merge[row * kMergeStride + k] = o;
+            }
+          }
+          mbar_arrive(&bar.wg[s]);
+          ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
+          if (!ok) break;
+          const int col = (row % 4) * 4;
+          for (int k = row / 4; k < all_rows; k += 32) {
+            float o[4] = {};
+            if (k < rows)
+              for (int from = k; from < 128; from += copy_rows)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] += merge[from * kMergeStride + col + i];
+            if (split) {
+              *reinterpret_cast<float4*>(part + (size_t)k * kDim + c + col) = make_float4(o[0], o[1], o[2], o[3]);
+            } else if (c + col < a.dim) {
+              const float norm = bar.row_norm[k];
+              *reinterpret_cast<uint2*>(out_row(k) + c + col) =
+                  norm == 0.0f ? make_uint2(0, 0)
+                               : make_uint2(pack2<T>(o[0] * norm, o[1] * norm), pack2<T>(o[2] * norm, o[3] * norm));
+            }
+          }
+          mbar_arrive(&bar.wg[s]);
+          ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
+          if (!ok) break;
+        }
+        if (!ok) break;
       }
       if (!kPair) {  // both streams have read O, the maxima and the flags
         tc_fence_before();

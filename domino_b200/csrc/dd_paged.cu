@@ -265,6 +265,10 @@ int check_attend(const dd_paged_cache* c, const dd_cache_attend_args* a) {
     return global_fail(DD_EINVAL, "cache attend: a window needs causal attention, sinks need a window");
   if ((long long)a->tokens * (a->heads / c->kv_heads) > (1ll << 29) || (long long)a->heads * c->head_dim > 0x7fffffffll)
     return global_fail(DD_EINVAL, "cache attend: chunk too large");
+  // the kernel counts key tiles of one row and head, and of one SM's share, in 32 bits
+  const double tiles = ((double)c->row_pages * c->page_size / 128 + 2) * c->kv_heads;
+  const double entries = (double)c->batch * ((double)a->tokens * (a->heads / c->kv_heads) / 128 + 1);
+  if (tiles > 1e9 || entries > 1e9 || tiles * entries > 1e11) return global_fail(DD_EINVAL, "cache attend: chunk too large");
   return DD_OK;
 }
 
@@ -432,6 +436,8 @@ int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void
   p.sinks = std::min(a->sinks, 1 << 30);
   p.status = c->status;
   const AttendPlan plan = attend_plan(c, a);
+  const long long rows = (long long)a->tokens * p.group;
+  p.copies = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
   if (plan.tensor) {
     if (!a->workspace || a->workspace_bytes < attend_bytes(plan, dev) || !aligned16(a->workspace))
       return global_fail(DD_EINVAL, "dd_cache_attend: workspace of %llu bytes needed",
