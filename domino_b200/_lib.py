@@ -38,8 +38,8 @@ EXPORTS = (
     "dd_get_exchange_buffer", "dd_ipc_export", "dd_ipc_open", "dd_ipc_close", "dd_set_vocab_shard",
     "dd_set_exchange_timeout", "dd_verify_accept", "dd_set_weight_layout", "dd_set_rollout_mode",
     "dd_set_trace", "dd_set_middle",
-    "dd_pages_scratch", "dd_pages_reserve", "dd_pages_crop", "dd_pages_fork", "dd_pages_compact",
-    "dd_cache_write", "dd_cache_attend_workspace", "dd_cache_attend",
+    "dd_cache_scratch", "dd_pages_reserve", "dd_pages_crop", "dd_pages_fork", "dd_pages_compact",
+    "dd_cache_write", "dd_cache_attend",
 )
 PHASES = {1: "z", 2: "zlm", 3: "gh", 4: "sgh", 5: "fc2", 6: "table", 7: "cell", 8: "gather", 9: "rollout"}
 
@@ -90,8 +90,7 @@ class DDCacheWriteArgs(ctypes.Structure):
 
 class DDCacheAttendArgs(ctypes.Structure):
     _fields_ = ([("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 3)]
-                + [(n, ctypes.c_void_p) for n in ("start", "lens", "workspace")]
-                + [("workspace_bytes", ctypes.c_uint64), ("scale", ctypes.c_float)]
+                + [(n, ctypes.c_void_p) for n in ("start", "lens")] + [("scale", ctypes.c_float)]
                 + [(n, ctypes.c_int32) for n in ("layer", "tokens", "heads", "causal", "window", "sinks")])
 
 
@@ -146,13 +145,12 @@ def load() -> ctypes.CDLL:
         lib.dd_set_middle.argtypes = [vp, ctypes.c_int]
         lib.dd_read_timing.argtypes = [vp, vp, vp, i32]
         cache, u64p = ctypes.POINTER(DDPagedCache), ctypes.POINTER(ctypes.c_uint64)
-        lib.dd_pages_scratch.argtypes = [cache, u64p]
+        lib.dd_cache_scratch.argtypes = [cache, u64p]
         lib.dd_pages_reserve.argtypes = [cache, vp, vp]
         lib.dd_pages_crop.argtypes = [cache, vp, vp]
         lib.dd_pages_fork.argtypes = [cache, vp, vp]
         lib.dd_pages_compact.argtypes = [cache, vp]
         lib.dd_cache_write.argtypes = [cache, ctypes.POINTER(DDCacheWriteArgs), vp]
-        lib.dd_cache_attend_workspace.argtypes = [cache, ctypes.POINTER(DDCacheAttendArgs), u64p]
         lib.dd_cache_attend.argtypes = [cache, ctypes.POINTER(DDCacheAttendArgs), vp]
         for name in EXPORTS:
             if name not in ("dd_last_error", "dd_version"):

@@ -19,9 +19,10 @@
 // query tile, key head) items are numbered through and every CTA takes an
 // equal run of them, so long and short rows balance and one row's long cache
 // spreads over all SMs.  An item that crosses CTAs leaves its pieces
-// (unnormalised O, m, l) in the workspace and attend_join_kernel adds them in
-// the order of the CTAs: no atomics, the same result every time.  Lengths are
-// read on the device, so the cut needs no host synchronisation.
+// (unnormalised O, m, l) in the workspace; the CTA that finishes last, found by
+// a counter that wraps back to zero, adds them in the order of the CTAs, so the
+// result is the same every time.  Lengths are read on the device, so the cut
+// needs no host synchronisation.
 //
 // The running maximum moves only when a row's scores pass it by more than 8
 // (as powers of two): P then stays below 2^8 and the rescaling of O, a round
@@ -40,19 +41,19 @@
 
 namespace dd {
 
-constexpr int kAttThreads = 384;  // 8 softmax warps, TMA producer, MMA issuer, 2 query loaders
+constexpr int kAttThreads = 384;  // 8 softmax warps, key producer, MMA issuer, value producer, query loader
 constexpr int kKeyTile = 128;
 constexpr int kMaxStages = 12;
-constexpr int kMergeCols = 16, kMergeStride = kMergeCols + 1;  // of the buffer that joins streams and copies of rows
+constexpr int kMergeCols = 16;  // of the two buffers of each stream's warps that join copies of rows
 
 struct AttendWork {
-  int4* head;    // [grid]: item {entry, key head, last CTA} whose first piece this CTA holds and does not finish; entry -1: none
-  float* o;      // [grid][2][rows][dim_pad]
-  float2* ml;    // [grid][2][rows]
+  unsigned* count;  // [kMaxAttendCtas], zero between calls: finished pieces of the item that starts in a CTA and leaves it
+  float* o;         // [grid][2][rows][dim_pad]: the piece that comes from the CTA before, and the one that goes on in the next
+  float2* ml;       // [grid][2][rows]
 };
-template <int kDim, bool kPair>
-constexpr size_t attend_work_bytes(int grid) {
-  return (size_t)grid * (16 + 2 * (kPair ? 256 : 128) * (sizeof(float) * kDim + 8));
+constexpr int kMaxAttendCtas = 160;
+__host__ __device__ constexpr size_t attend_work_bytes(int dim_pad, bool pair) {
+  return (size_t)kMaxAttendCtas * 2 * (pair ? 256 : 128) * (sizeof(float) * dim_pad + sizeof(float2));
 }
 
 // Key tiles of one (row of the batch, query tile): n_sink from 0, then from
@@ -85,20 +86,24 @@ __device__ __forceinline__ TileSpan tile_span(const AttendParams& a, int b, int 
   return s;
 }
 
-// A CTA's run of key tiles, item by item.
+// A CTA's share of the work, item by item.  Many items: the CTAs take equal runs
+// of units, where an item counts its tiles and, before them, kItemUnits for the
+// start and the end of an item.  Few items (at most a quarter of the CTAs): each
+// gets CTAs of its own in proportion to its tiles, so that nobody has two.
 struct Piece {
   int e, b, qt, h, i0, i1;  // entry (b, qt), key head, tiles [i0, i1) of it
-  int left;                 // tiles of the run from i0 on
+  int pos, left;            // unit of the item where the run enters it; units of the run from there on
   TileSpan span;
 };
+constexpr int kItemUnits = 3;
 __device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
   p.b = p.e / q_tiles;
   p.qt = p.e - p.b * q_tiles;
   p.span = tile_span(a, p.b, p.qt, tile_rows);
 }
 __device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
-  p.left -= p.i1 - p.i0;
-  if (p.left == 0) return false;
+  p.left -= p.span.n + kItemUnits - p.pos;
+  if (p.left <= kItemUnits) return false;  // the next item's first tile is another CTA's
   if (++p.h == a.kv_heads) {
     p.h = 0;
     do {
@@ -106,15 +111,25 @@ __device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int 
       piece_enter(a, p, q_tiles, tile_rows);
     } while (p.span.n == 0);
   }
-  p.i0 = 0;
-  p.i1 = min(p.span.n, p.left);
+  p.pos = p.i0 = 0;
+  p.i1 = min(p.span.n, p.left - kItemUnits);
   return true;
+}
+// CTAs for an item of n tiles when there are few items.
+__device__ __forceinline__ int item_ctas(const AttendParams& a, int n, long long tiles, int spare) {
+  if (n == 0) return 0;
+  return max(min((int)((long long)n * spare / tiles), n / a.min_tiles), 1);
 }
 
 // Where CTA c's run starts: c / grid of all tiles.
 __device__ __forceinline__ long long run_start(long long total, unsigned c, unsigned grid) {
   if (total < 1 << 23 && grid < 256) return (unsigned)total * c / grid;  // 32-bit division
   return total * c / grid;
+}
+
+// The CTA that holds tile g.
+__device__ __forceinline__ int run_of(long long total, long long g, unsigned grid) {
+  return (int)(((g + 1) * grid - 1) / total);
 }
 
 // The ring of key and value tiles.  Tiles are loaded in the order in which the
@@ -131,11 +146,40 @@ struct Ring {
     }
   }
 };
-// Position of tile i's values in a piece's load order; n tiles.
+// Position of tile i's keys / values in a piece's load order; n tiles.
+template <bool kPair>
+__device__ __forceinline__ int load_index_k(int i) {
+  return kPair ? 2 * i : i < 2 ? i : 2 * i - 1;
+}
 template <bool kPair>
 __device__ __forceinline__ int load_index_v(int i, int n) {
   return kPair ? 2 * i + 1 : i + min(i + 2, n);
 }
+
+// A row's table entries, 32 at a time with the next 32 on their way, one per lane.
+struct PageWindow {
+  int w = -2, now = -1, next = -1;
+  __device__ __forceinline__ int entry(const AttendParams& a, const Piece& p, int w32, int lane) const {
+    const int slot = w32 * 32 + lane;
+    int page = -1;
+    if (slot < a.row_pages && (slot << a.page_shift) < p.span.hi) {
+      page = a.table[(long long)p.b * a.row_pages + slot];
+      if (page >= a.pages) page = -1;
+    }
+    return page;
+  }
+  // Page of lane's part of a key tile (lanes below 128 / page_size; -1 elsewhere and where there is none).
+  __device__ __forceinline__ int get(const AttendParams& a, const Piece& p, int tile, int lane) {
+    const int per = kKeyTile >> a.page_shift, slot = tile * per, w32 = slot >> 5;
+    if (w32 != w) {
+      now = w32 == w + 1 ? next : entry(a, p, w32, lane);
+      next = entry(a, p, w32 + 1, lane);
+      w = w32;
+    }
+    const int page = __shfl_sync(0xffffffffu, now, (slot & 31) + lane);
+    return lane < per ? page : -1;
+  }
+};
 
 // Page of 16-key group `lane` (0 .. 7) of a key tile.
 __device__ __forceinline__ int group_page(const AttendParams& a, int b, int tile, int lane) {
@@ -154,6 +198,11 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+// One arrival for a whole warp, after all of its lanes got here.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 // The n lowest bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
@@ -209,13 +258,88 @@ __device__ __noinline__ void attend_row_exact(const AttendParams& a, const Piece
   *l_out = l;
 }
 
+// The pieces of one item, in slot 1 of CTA c0 and slot 0 of those behind it, by
+// 256 threads.  A warp takes four rows at a time: the lanes read the pieces'
+// (m, l) side by side, then the rows are added up piece by piece with sixteen
+// loads in flight (the reads come from L2 and one SM does them all).
+template <typename T, int kDim, int kRows>
+__device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork& work, const Piece& p, int c0, int c1,
+                                         int tid) {
+  constexpr int kVec = kDim / 32, kBatch = 4;  // values per lane, rows at a time
+  const int lane = tid & 31, r0 = p.qt * kRows, last = min(kRows, a.tokens * a.group - r0);
+  for (int row0 = tid >> 5; row0 < last; row0 += 8 * kBatch) {
+    float o[kBatch][kVec] = {}, m[kBatch], l[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
+    for (int c = c0; c <= c1; c += 32) {
+      const int mine = c + lane, pieces = min(32, c1 - c + 1);
+      float2 ml[kBatch];
+      float w[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int row = min(row0 + 8 * i, last - 1);
+        ml[i] = mine <= c1 ? __ldcg(&work.ml[(2 * (size_t)mine + (mine == c0)) * kRows + row]) : make_float2(-INFINITY, 0.0f);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        float top = ml[i].x;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float m1 = fmaxf(m[i], top), base = m1 == -INFINITY ? 0.0f : m1;
+        const float keep = exp2_approx(m[i] - base);
+        w[i] = exp2_approx(ml[i].x - base);
+        float sum = ml[i].y * w[i];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l[i] = l[i] * keep + sum;
+        m[i] = m1;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) o[i][v] *= keep;
+      }
+#pragma unroll 4
+      for (int k = 0; k < pieces; ++k) {
+        const float* part = work.o + (2 * (size_t)(c + k) + (c + k == c0)) * kRows * kDim + lane * kVec;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int row = min(row0 + 8 * i, last - 1);
+          const float wk = __shfl_sync(0xffffffffu, w[i], k);
+          float x[kVec];
+          if constexpr (kVec == 4)
+            *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(part + row * kDim));
+          else
+            *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(part + row * kDim));
+#pragma unroll
+          for (int v = 0; v < kVec; ++v) o[i][v] += x[v] * wk;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int row = row0 + 8 * i, r = r0 + row, t = r / a.group, g = r - t * a.group;
+      if (row >= last || lane * kVec >= a.dim) continue;
+      const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+      const bool live = r < p.span.rows;  // the pieces of rows behind the chunk's end hold anything
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) o[i][v] = live ? o[i][v] * inv : 0.0f;
+      T* out = static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * a.group + g) * a.dim + lane * kVec;
+      if constexpr (kVec == 4)
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o[i][0], o[i][1]), pack2<T>(o[i][2], o[i][3]));
+      else
+        *reinterpret_cast<uint32_t*>(out) = pack2<T>(o[i][0], o[i][1]);
+    }
+  }
+}
+
 template <int kDim, bool kPair>
 struct AttendShape {
   static constexpr int kTiles = kPair ? 2 : 1;      // query tiles
   static constexpr int kRows = 128 * kTiles;
   static constexpr int kHalves = kDim / 64;
   static constexpr int kTileBytes = 128 * kDim * 2;  // a query tile, a K or V tile
-  static constexpr int kMergeBytes = kPair ? 0 : 2 * 128 * kMergeStride * 4;
+  static constexpr int kMergeBytes = kPair ? 0 : 2 * 2 * 128 * kMergeCols * 4;
   static constexpr int kFit = (224 * 1024 - kTiles * kTileBytes - kMergeBytes) / kTileBytes;
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
 };
@@ -225,18 +349,59 @@ struct AttendShared {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t s_full[2], p_full[2], o_full[2], q_full, q_empty, wg[2], both;
   Piece first;          // where the run starts; left = 0: the CTA has none
-  long long warp_units[kAttThreads / 32], total, unit0;
+  long long total, unit0;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, few;
+  int join_c0, join_c1, join;  // CTAs that hold the split item; whether this CTA's piece finished last
   unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
-  float2 row_ml[2][128];
   float row_norm[128];
+  union {
+    float2 row_ml[2][128];
+    struct {  // while the work is cut
+      long long warp_sum[kAttThreads / 32], warp_x[kAttThreads / 32];
+      int warp_y[kAttThreads / 32];
+    };
+  };
 };
 // All of the 227 KB; the tiles start on a 1024-byte boundary, and there is
 // room for the padding that takes (the window starts on one: none).
 constexpr int kAttSmem = 227 * 1024;
 constexpr int kAttPad = kAttSmem - 224 * 1024 - (int)sizeof(AttendShared);
 static_assert(kAttPad >= 0, "tiles and AttendShared must fit 227 KB");
+
+// Over the block: `before` becomes the sum over the threads before this one and
+// `total` the sum over all; x and y become their sums over all.
+__device__ __forceinline__ void block_scan2(AttendShared& sh, long long& before, long long& total, long long& x, int& y,
+                                            int warp, int lane) {
+  long long inc = before;
+  const long long own = before;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += o;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, d);
+    y += __shfl_xor_sync(0xffffffffu, y, d);
+  }
+  __syncthreads();
+  if (lane == 31) {
+    sh.warp_sum[warp] = inc;
+    sh.warp_x[warp] = x;
+    sh.warp_y[warp] = y;
+  }
+  __syncthreads();
+  before = inc - own;
+  total = x = y = 0;
+#pragma unroll
+  for (int w = 0; w < kAttThreads / 32; ++w) {
+    if (w < warp) before += sh.warp_sum[w];
+    total += sh.warp_sum[w];
+    x += sh.warp_x[w];
+    y += sh.warp_y[w];
+  }
+}
 
 template <typename T, int kDim, bool kPair>
 __global__ void __launch_bounds__(kAttThreads, 1)
@@ -246,10 +411,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   const int pad = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
   if (pad > kAttPad) {
-    if (threadIdx.x == 0) {
-      atomicOr(a.status, DD_STATUS_TIMEOUT);
-      work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    }
+    if (threadIdx.x == 0) atomicOr(a.status, DD_STATUS_TIMEOUT);
     return;
   }
   unsigned char* sm_q = smem_raw + pad;
@@ -268,13 +430,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar.s_full[s], 1);
-      mbar_init(&bar.p_full[s], 128);
+      mbar_init(&bar.p_full[s], 4);  // one arrival per warp
       mbar_init(&bar.o_full[s], 1);
-      mbar_init(&bar.wg[s], 128);
+      mbar_init(&bar.wg[s], 4);
     }
-    mbar_init(&bar.q_full, 64);
+    mbar_init(&bar.q_full, 32);
     mbar_init(&bar.q_empty, 1);
-    mbar_init(&bar.both, 256);
+    mbar_init(&bar.both, 8);
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc(&bar.tmem_base, 512);
@@ -287,53 +449,88 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   // the CTA's run of tiles
   {
     const int entries = a.batch * q_tiles, per = (entries + kAttThreads - 1) / kAttThreads;
-    const int e0 = tid * per, e1 = min(entries, e0 + per);
+    const int e0 = tid * per, e1 = min(entries, e0 + per), grid = gridDim.x;
     Piece mine;
-    long long units = 0;
+    // sums over the block: tiles and items of one key head
+    long long tiles = 0;
+    int items = 0;
     for (mine.e = e0; mine.e < e1; ++mine.e) {
       piece_enter(a, mine, q_tiles, Shape::kRows);
-      units += mine.span.n;
+      tiles += mine.span.n;
+      items += mine.span.n > 0;
     }
-    units *= a.kv_heads;
-    long long inc = units;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
-    }
-    if (lane == 31) bar.warp_units[warp] = inc;
-    __syncthreads();
-    long long before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kAttThreads / 32; ++w) {
-      if (w < warp) before += bar.warp_units[w];
-      total += bar.warp_units[w];
-    }
-    before += inc - units;
-    const long long u0 = run_start(total, blockIdx.x, gridDim.x), u1 = run_start(total, blockIdx.x + 1, gridDim.x);
-    if (tid == 0) {
-      bar.total = total;
-      bar.unit0 = u0;
-    }
-    if (u0 >= u1) {
+    long long before = tiles + (long long)items * kItemUnits, total;  // units before this thread's entries, of all
+    const long long own = before;
+    block_scan2(bar, before, total, tiles, items, warp, lane);
+    before *= a.kv_heads;
+    total *= a.kv_heads;
+    const bool few = (long long)items * a.kv_heads * 4 <= grid;
+    int c0 = 0, c1 = 0;
+    bool found = false;
+    if (!few) {
+      const long long u0 = run_start(total, blockIdx.x, grid), u1 = run_start(total, blockIdx.x + 1, grid);
+      if (u0 < u1 && u0 >= before && u0 < before + own * a.kv_heads) {
+        // the run starts in this thread's entries (one entry as a rule: its span is still here)
+        long long rem = u0 - before;
+        int len = 0;
+        for (mine.e = e0; mine.e < e1; ++mine.e) {
+          if (per > 1) piece_enter(a, mine, q_tiles, Shape::kRows);
+          len = mine.span.n ? mine.span.n + kItemUnits : 0;
+          if (rem < (long long)len * a.kv_heads) break;
+          rem -= (long long)len * a.kv_heads;
+        }
+        mine.h = (int)rem / len;  // rem < tiles x heads of one entry
+        mine.pos = (int)rem - mine.h * len;
+        mine.left = (int)(u1 - u0);
+        mine.i0 = max(mine.pos - kItemUnits, 0);
+        mine.i1 = min(mine.span.n, mine.pos + mine.left - kItemUnits);
+        if (mine.i1 <= mine.i0) mine.left = 0;
+        found = true;
+      }
       if (tid == 0) {
-        bar.first.left = 0;
-        work.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        bar.total = total;
+        bar.unit0 = u0;
       }
-    } else if (u0 >= before && u0 < before + units) {
-      // the run starts in this thread's entries (one entry as a rule: its span is still here)
-      long long rem = u0 - before;
-      for (mine.e = e0; mine.e < e1; ++mine.e) {
-        if (per > 1) piece_enter(a, mine, q_tiles, Shape::kRows);
-        const long long n = (long long)mine.span.n * a.kv_heads;
-        if (rem < n) break;
-        rem -= n;
+    } else {
+      const int spare = grid - items * a.kv_heads;
+      tiles *= a.kv_heads;
+      long long ctas = 0, all, unused0 = 0;
+      int unused1 = 0;
+      for (int e = e0; e < e1; ++e) {
+        if (per > 1) {
+          mine.e = e;
+          piece_enter(a, mine, q_tiles, Shape::kRows);
+        }
+        ctas += item_ctas(a, mine.span.n, tiles, spare);
       }
-      mine.h = (int)rem / mine.span.n;  // rem < n tiles x heads of one entry
-      mine.i0 = (int)rem - mine.h * mine.span.n;
-      mine.left = (int)(u1 - u0);
-      mine.i1 = min(mine.span.n, mine.i0 + mine.left);
+      const long long mine_ctas = ctas;
+      block_scan2(bar, ctas, all, unused0, unused1, warp, lane);
+      if ((int)blockIdx.x >= ctas * a.kv_heads && (int)blockIdx.x < (ctas + mine_ctas) * a.kv_heads) {
+        int rem = blockIdx.x - (int)ctas * a.kv_heads, k = 1;
+        for (mine.e = e0; mine.e < e1; ++mine.e) {
+          if (per > 1) piece_enter(a, mine, q_tiles, Shape::kRows);
+          k = item_ctas(a, mine.span.n, tiles, spare);
+          if (rem < k * a.kv_heads) break;
+          rem -= k * a.kv_heads;
+        }
+        mine.h = rem / k;
+        const int part = rem - mine.h * k;
+        mine.i0 = (int)((long long)mine.span.n * part / k);
+        mine.i1 = (int)((long long)mine.span.n * (part + 1) / k);
+        mine.pos = 0;
+        mine.left = 1;  // one piece only
+        c0 = blockIdx.x - part;
+        c1 = c0 + k - 1;
+        found = true;
+      }
+    }
+    if (tid == 0) bar.first.left = 0;
+    __syncthreads();
+    if (found) {
       bar.first = mine;
+      bar.few = few;
+      bar.join_c0 = c0;
+      bar.join_c1 = c1;
     }
     tc_fence_before();
     __syncthreads();
@@ -344,184 +541,153 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   Piece p = bar.first;
   bool more = p.left > 0;
 
-  if (warp == 8) {
-    // ---------------------------------------------------------------- producer
-    const int pages_per_tile = kKeyTile >> a.page_shift;
+  if (warp == 8 || warp == 10) {
+    // ---------------------------------------------------------------- producers: keys, values
+    const bool keys = warp == 8;
+    const CUtensorMap* map = keys ? &map_k : &map_v;
     const uint32_t page_bytes = a.page_size * 128u;  // of one 64-value half
-    Ring<Shape::kStages> ring;
+    int base = 0;  // loads before this piece, modulo two rounds of the ring
     bool ok = true;
-    auto page_of = [&](int i) {
-      const int slot = p.span.tile(i) * pages_per_tile + lane;
-      int page = -1;
-      if (lane < pages_per_tile && slot < a.row_pages && (slot << a.page_shift) < p.span.hi) {
-        page = a.table[(long long)p.b * a.row_pages + slot];
-        if (page >= a.pages) page = -1;
-      }
-      return page;
-    };
-    auto load = [&](const CUtensorMap* map, int page) {
-      const int st = ring.stage;
-      ok = mbar_wait_bounded(&bar.empty[st], ring.phase ^ 1, abort);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], __popc(have) * page_bytes * Shape::kHalves);
-      __syncwarp();
-      if (page >= 0) {
-        unsigned char* dst = sm_ring + st * Shape::kTileBytes + lane * page_bytes;
-#pragma unroll
-        for (int hf = 0; hf < Shape::kHalves; ++hf)
-          tma_load_4d(dst + hf * 128 * 128, map, &bar.full[st], hf * 64, 0, p.h, page);
-      }
-      ring.next();
-    };
-    // table entries are read one tile ahead of their use
     for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
-      if (kPair) {
-        int page = page_of(p.i0);
-        for (int i = p.i0; i < p.i1 && ok; ++i) {
-          const int ahead = i + 1 < p.i1 ? page_of(i + 1) : -1;
-          load(&map_k, page);
-          if (ok) load(&map_v, page);
-          page = ahead;
-        }
-      } else {
-        int page = page_of(p.i0), page1 = p.i0 + 1 < p.i1 ? page_of(p.i0 + 1) : -1;
-        load(&map_k, page);
-        if (ok && p.i0 + 1 < p.i1) load(&map_k, page1);
-        for (int i = p.i0; i < p.i1 && ok; ++i) {
-          const int ahead = i + 2 < p.i1 ? page_of(i + 2) : -1;
-          load(&map_v, page);
-          if (ok && i + 2 < p.i1) load(&map_k, ahead);
-          page = page1;
-          page1 = ahead;
+      const int n = p.i1 - p.i0;
+      PageWindow window;
+      for (int i = 0; i < n; ++i) {
+        const int page = window.get(a, p, p.span.tile(p.i0 + i), lane);
+        const int c = (base + (keys ? load_index_k<kPair>(i) : load_index_v<kPair>(i, n))) % (2 * Shape::kStages);
+        const int st = c >= Shape::kStages ? c - Shape::kStages : c;
+        ok = mbar_wait_bounded(&bar.empty[st], (c >= Shape::kStages) ^ 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], __popc(have) * page_bytes * Shape::kHalves);
+        __syncwarp();
+        if (page >= 0) {
+          unsigned char* dst = sm_ring + st * Shape::kTileBytes + lane * page_bytes;
+#pragma unroll
+          for (int hf = 0; hf < Shape::kHalves; ++hf)
+            tma_load_4d(dst + hf * 128 * 128, map, &bar.full[st], hf * 64, 0, p.h, page);
         }
       }
+      base = (base + 2 * n) % (2 * Shape::kStages);
     }
-    if (!ok) {  // leave no copy in flight behind this CTA: every stage's last load
-      Ring<Shape::kStages> r = ring;
-      for (int c = 0; c < Shape::kStages; ++c, r.next())
-        for (int k = 0; k < 1000000 && !mbar_try_wait(&bar.full[r.stage], r.phase ^ 1); ++k) {
-        }
+    if (!ok) {  // leave no copy in flight behind this CTA: time for all of them to land
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 10 * 1000 * 1000) {
+      }
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-      constexpr uint32_t idesc_s = idesc_f16(128, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
-      Ring<Shape::kStages> ring;
-      uint32_t n_pieces = 0, n_p[2] = {0, 0};
-      bool ok = true;
-      // the stage of the next load, once it has landed
-      auto take = [&]() {
-        const int st = ring.stage;
-        ok = ok && mbar_wait_bounded(&bar.full[st], ring.phase, abort);
-        ring.next();
-        return st;
-      };
-      const uint32_t ring0 = smem_u32(sm_ring), q0 = smem_u32(sm_q);
-      auto qk = [&](int s, int st) {
-        const uint64_t dq = smem_desc_k_sw128(q0 + (kPair ? s * Shape::kTileBytes : 0));
-        const uint64_t dk = smem_desc_k_sw128(ring0 + st * Shape::kTileBytes);
+    // The whole warp walks the schedule and one elected lane issues: descriptors
+    // then stay in uniform registers (issued from inside a lane's own branch,
+    // each MMA cost about 100 cycles and the issue bound the kernel).
+    constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr uint32_t idesc_s = idesc_f16(128, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
+    Ring<Shape::kStages> ring;
+    uint32_t n_pieces = 0, n_p[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+      ok = ok && mbar_wait_bounded(b, parity, abort);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    // the stage of the next load, once it has landed
+    auto take = [&]() {
+      const int st = ring.stage;
+      wait(&bar.full[st], ring.phase);
+      ring.next();
+      return st;
+    };
+    const uint32_t ring0 = smem_u32(sm_ring), q0 = smem_u32(sm_q);
+    // S of stream s from the keys in stage st, and which buffers are free once it is done
+    auto qk = [&](int s, int st, bool free_stage, bool free_q) {
+      const uint64_t dq = smem_desc_k_sw128(q0 + (kPair ? s * Shape::kTileBytes : 0));
+      const uint64_t dk = smem_desc_k_sw128(ring0 + st * Shape::kTileBytes);
+      if (elect_one()) {
 #pragma unroll
         for (int d = 0; d < kDim / 16; ++d) {
           const uint64_t off = ((d / 4) * 128 * 128 + (d % 4) * 32) >> 4;
           mma_f16_ss(tmem + s * 128, dq + off, dk + off, idesc_s, d > 0);
         }
         mma_commit(&bar.s_full[s]);
-      };
-      auto pv = [&](int s, int st, bool accumulate) {
-        const uint64_t dv = smem_desc_mn_sw128(ring0 + st * Shape::kTileBytes, 128 * 128);
+        if (free_stage) mma_commit(&bar.empty[st]);
+        if (free_q) mma_commit(&bar.q_empty);
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int s, int st, bool accumulate, bool free_stage, bool last) {
+      const uint64_t dv = smem_desc_mn_sw128(ring0 + st * Shape::kTileBytes, 128 * 128);
+      if (elect_one()) {
 #pragma unroll
         for (int d = 0; d < kKeyTile / 16; ++d)
           mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + d * 8, dv + ((d * 2048) >> 4), idesc_o, accumulate || d > 0);
-      };
-      auto wait_p = [&](int s) {
-        ok = ok && mbar_wait_bounded(&bar.p_full[s], n_p[s]++ & 1, abort);
-        tc_fence_after();
-      };
-      for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
-        const int n = p.i1 - p.i0;
-        ok = ok && mbar_wait_bounded(&bar.q_full, n_pieces++ & 1, abort);
+        if (free_stage) mma_commit(&bar.empty[st]);
+        if (last) mma_commit(&bar.o_full[s]);
+      }
+      __syncwarp();
+    };
+    auto wait_p = [&](int s) {
+      wait(&bar.p_full[s], n_p[s]++ & 1);
+      tc_fence_after();
+    };
+    for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+      const int n = p.i1 - p.i0;
+      wait(&bar.q_full, n_pieces++ & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (kPair) {
+        int k = take(), v = 0;
         if (!ok) break;
-        tc_fence_after();
-        if (kPair) {
-          int k = take(), v = 0;
-          if (!ok) break;
-          qk(0, k);
-          qk(1, k);
-          mma_commit(&bar.empty[k]);
-          if (n == 1) mma_commit(&bar.q_empty);
-          for (int i = 0; i < n && ok; ++i) {
+        qk(0, k, false, false);
+        qk(1, k, true, n == 1);
+        for (int i = 0; i < n && ok; ++i) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              wait_p(s);
-              if (s == 0 && ok) v = take();
-              if (!ok) break;
-              pv(s, v, i > 0);
-              if (s == 1) mma_commit(&bar.empty[v]);
-              if (i + 1 < n) {
-                if (s == 0) k = take();
-                if (!ok) break;
-                qk(s, k);
-                if (s == 1) {
-                  mma_commit(&bar.empty[k]);
-                  if (i + 2 == n) mma_commit(&bar.q_empty);
-                }
-              } else {
-                mma_commit(&bar.o_full[s]);
-              }
-            }
-          }
-        } else {
-          for (int s = 0; s < min(2, n) && ok; ++s) {
-            const int k = take();
-            if (!ok) break;
-            qk(s, k);
-            mma_commit(&bar.empty[k]);
-          }
-          if (ok && n <= 2) mma_commit(&bar.q_empty);
-          for (int i = 0; i < n && ok; ++i) {
-            const int s = i & 1;
+          for (int s = 0; s < 2; ++s) {
             wait_p(s);
+            if (s == 0 && ok) v = take();
             if (!ok) break;
-            const int v = take();
-            if (!ok) break;
-            pv(s, v, i >= 2);
-            mma_commit(&bar.empty[v]);
-            if (i + 2 < n) {
-              const int k = take();
+            pv(s, v, i > 0, s == 1, i + 1 == n);
+            if (i + 1 < n) {
+              if (s == 0) k = take();
               if (!ok) break;
-              qk(s, k);
-              mma_commit(&bar.empty[k]);
-              if (i + 3 == n) mma_commit(&bar.q_empty);
-            } else {
-              mma_commit(&bar.o_full[s]);
+              qk(s, k, s == 1, s == 1 && i + 2 == n);
             }
+          }
+        }
+      } else {
+        for (int s = 0; s < min(2, n) && ok; ++s) {
+          const int k = take();
+          if (ok) qk(s, k, true, s + 1 == n);
+        }
+        for (int i = 0; i < n && ok; ++i) {
+          const int s = i & 1;
+          wait_p(s);
+          if (!ok) break;
+          const int v = take();
+          if (!ok) break;
+          pv(s, v, i >= 2, true, i + 2 >= n);
+          if (i + 2 < n) {
+            const int k = take();
+            if (ok) qk(s, k, true, i + 3 == n);
           }
         }
       }
     }
-    __syncwarp();
-  } else if (warp >= 10) {
-    // ---------------------------------------------------------------- query loader, and the record for the join
+  } else if (warp == 11) {
+    // ---------------------------------------------------------------- query loader, and the rows of no item
     // 16-byte asynchronous copies, all of a piece's in flight at once; a thread
     // keeps one chunk of the row and steps through the rows.
-    const int id = tid - 320;
-    constexpr int kChunks = kDim / 8, kRowStep = 64 / kChunks;
-    const int ch = id % kChunks;
+    constexpr int kChunks = kDim / 8, kRowStep = 32 / kChunks;
+    const int ch = lane % kChunks;
     const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0 &&
                      a.q_stride[2] % 8 == 0;
     const int copy_rows = kPair ? Shape::kRows : 128 / a.copies;
     uint32_t n_pieces = 0;
-    int4 head = make_int4(-1, 0, 0, 0);
     bool ok = true;
     for (; more; more = piece_next(a, p, q_tiles, Shape::kRows)) {
       ok = mbar_wait_bounded(&bar.q_empty, (n_pieces++ & 1) ^ 1, abort);
       if (!ok) break;
       const int r0 = p.qt * Shape::kRows, live = min(Shape::kRows, p.span.rows - r0);
       const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + (long long)p.h * group * a.q_stride[2] + ch * 8;
-      int row = id / kChunks, t = (r0 + row) / group, g = r0 + row - t * group;
+      int row = lane / kChunks, t = (r0 + row) / group, g = r0 + row - t * group;
       for (; row < live; row += kRowStep) {
         const T* src = q + t * a.q_stride[1] + g * a.q_stride[2];
         const bool in = ch * 8 < a.dim;
@@ -542,15 +708,21 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       cp_async_wait_all();
       fence_proxy_async_shared();
       mbar_arrive(&bar.q_full);
-      if (id == 0 && p.i0 == 0 && p.i1 < p.span.n) {
-        const long long end = bar.unit0 + (bar.first.left - p.left) + p.span.n;
-        int c = blockIdx.x + 1;
-        while (run_start(bar.total, c + 1, gridDim.x) < end) ++c;
-        // (with fewer tiles than CTAs some CTAs between are empty: the join needs the total)
-        head = make_int4(p.e, p.h, c, bar.total < gridDim.x ? (int)bar.total : 0);
+    }
+    // query tiles with nothing to see or behind the end of a short chunk: zeros
+    for (int e = blockIdx.x; e < a.batch * q_tiles; e += gridDim.x) {
+      const int b = e / q_tiles, qt = e - b * q_tiles;
+      if (tile_span(a, b, qt, Shape::kRows).n) continue;
+      const int r1 = min((qt + 1) * Shape::kRows, a.tokens * group);
+      for (int r = qt * Shape::kRows; r < r1; ++r) {
+        const int t = r / group, g = r - t * group;
+        for (int i = lane; i < a.kv_heads * (a.dim / 8); i += 32) {
+          const int h = i / (a.dim / 8), d = (i - h * (a.dim / 8)) * 8;
+          T* out = static_cast<T*>(a.out) + (((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + d;
+          *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
+        }
       }
     }
-    if (id == 0 && bar.first.left > 0) work.head[blockIdx.x] = head;
   } else {
     // ---------------------------------------------------------------- softmax, one thread per query row
     const int s = warp >> 2, row = tid & 127;
@@ -559,7 +731,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     const float sl = a.scale * 1.4426950408889634f;
     uint32_t n_s = 0, n_o[2] = {0, 0}, n_wg = 0, n_both = 0, n_pieces = 0;
     int base = 0;  // loads before this piece, modulo two rounds of the ring
-    bool ok = true;
+    bool ok = true, pending = false;
     // Few rows: the tile holds `copies` copies of them, and copy c of a row
     // takes part c of the tile's keys (P is zero elsewhere), so that all four
     // warps share the exponentials.  The copies are joined like the streams.
@@ -689,8 +861,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           if (wrote) fence_proxy_async_shared();
           if (odd) bar.redo[s] = n_pieces;
         }
+        if (!kPair && pending) {
+          ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
+          if (!ok) break;
+          pending = false;
+        }
         tc_fence_before();
-        mbar_arrive(&bar.p_full[s]);
+        warp_arrive(&bar.p_full[s], lane);
       }
       if (!ok) break;
       // the piece's result
@@ -709,19 +886,24 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       if (kPair) {
         ok = mbar_wait_bounded(&bar.o_full[s], n_o[s]++ & 1, abort);
         if (!ok) break;
-        mbar_arrive(&bar.wg[s]);
+        warp_arrive(&bar.wg[s], lane);
         ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
         if (!ok) break;
         again = bar.redo[s] == n_pieces;  // nobody searches the next piece before all have read this
-        mbar_arrive(&bar.wg[s]);
+        warp_arrive(&bar.wg[s], lane);
         ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
         if (!ok) break;
       } else {
+        if (pending) {  // (a stream without a tile in this piece)
+          ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
+          if (!ok) break;
+          pending = false;
+        }
         bar.row_ml[s][row] = make_float2(m, l);
         ok = mbar_wait_bounded(&bar.o_full[0], n_o[0]++ & 1, abort);
         if (ok && n > 1) ok = mbar_wait_bounded(&bar.o_full[1], n_o[1]++ & 1, abort);
         if (!ok) break;
-        mbar_arrive(&bar.both);
+        warp_arrive(&bar.both, lane);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
         again = bar.redo[0] == n_pieces || bar.redo[1] == n_pieces;
@@ -790,53 +972,81 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         // streams' sums by row, the copies of a row through shared memory, and
         // out with four lanes a row.
         if (split && s == 0 && row < copy_rows) part_ml[row] = make_float2(m, l);
-        bar.row_norm[row] = inv;  // (both streams and all copies write the same)
-        float* merge = reinterpret_cast<float*>(sm_q + 224 * 1024 - Shape::kMergeBytes) + s * 128 * kMergeStride;
+        bar.row_norm[row] = r < p.span.rows ? inv : 0.0f;  // (both streams write the same)
+        float4* merge = reinterpret_cast<float4*>(sm_q + 224 * 1024 - Shape::kMergeBytes) + s * 2 * 128 * 4;
         const int rows = min(p.span.rows, copy_rows), all_rows = min(a.tokens * group, copy_rows);
 #pragma unroll 1
-        for (int c = s * (kDim / 2); c < (s + 1) * (kDim / 2); c += kMergeCols) {
+        for (int c = s * (kDim / 2), c_end = c + kDim / 2; c < c_end; c += kMergeCols) {
           if (warp_live) {
             uint32_t x[16], y[16];
             tmem_ld16u(t_o + c, x);
             if (n > 1) tmem_ld16u(t_o + kDim + c, y);
             tmem_ld_wait();
+            float o[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              float o = __uint_as_float(x[k]) * f0;
-              if (n > 1) o += __uint_as_float(y[k]) * f1;
-              merge[row * kMergeStride + k] = o;
+              o[k] = __uint_as_float(x[k]) * f0;
+              if (n > 1) o[k] += __uint_as_float(y[k]) * f1;
             }
-          }
-          mbar_arrive(&bar.wg[s]);
-          ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
-          if (!ok) break;
-          const int col = (row % 4) * 4;
-          for (int k = row / 4; k < all_rows; k += 32) {
-            float o[4] = {};
-            if (k < rows)
-              for (int from = k; from < 128; from += copy_rows)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += merge[from * kMergeStride + col + i];
-            if (split) {
-              *reinterpret_cast<float4*>(part + (size_t)k * kDim + c + col) = make_float4(o[0], o[1], o[2], o[3]);
-            } else if (c + col < a.dim) {
-              const float norm = bar.row_norm[k];
-              *reinterpret_cast<uint2*>(out_row(k) + c + col) =
-                  norm == 0.0f ? make_uint2(0, 0)
-                               : make_uint2(pack2<T>(o[0] * norm, o[1] * norm), pack2<T>(o[2] * norm, o[3] * norm));
-            }
+            for (int k = 0; k < 4; ++k)  // 16-byte parts of the row, turned by the row against bank conflicts
+              merge[row * 4 + (k ^ (row >> 1 & 3))] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
-          mbar_arrive(&bar.wg[s]);
+          warp_arrive(&bar.wg[s], lane);
           ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
           if (!ok) break;
+          const int part4 = row % 4, col = c + part4 * 4;
+          for (int k = row / 4; k < all_rows; k += 32) {
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k < rows)
+              for (int from = k; from < 128; from += copy_rows) {
+                const float4 x = merge[from * 4 + (part4 ^ (from >> 1 & 3))];
+                o.x += x.x;
+                o.y += x.y;
+                o.z += x.z;
+                o.w += x.w;
+              }
+            if (split) {
+              *reinterpret_cast<float4*>(part + (size_t)k * kDim + col) = o;
+            } else if (col < a.dim) {
+              const float norm = bar.row_norm[k];
+              *reinterpret_cast<uint2*>(out_row(k) + col) =
+                  norm == 0.0f ? make_uint2(0, 0) : make_uint2(pack2<T>(o.x * norm, o.y * norm), pack2<T>(o.z * norm, o.w * norm));
+            }
+          }
+          // the other buffer next: the wait in between keeps the two apart
+          merge = reinterpret_cast<float4*>(sm_q + 224 * 1024 - Shape::kMergeBytes) + s * 2 * 128 * 4 +
+                  ((c / kMergeCols) & 1 ? 0 : 128 * 4);
         }
         if (!ok) break;
       }
-      if (!kPair) {  // both streams have read O, the maxima and the flags
-        tc_fence_before();
-        mbar_arrive(&bar.both);
+      if (split) {
+        // the piece is in the workspace; whoever brings the last one adds them up
+        __threadfence();
+        warp_arrive(&bar.both, lane);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
+        if (tid == 0) {
+          if (!bar.few) {
+            const long long g0 = bar.unit0 + (bar.first.left - p.left) - p.pos + kItemUnits;
+            bar.join_c0 = run_of(bar.total, g0, gridDim.x);
+            bar.join_c1 = run_of(bar.total, g0 + p.span.n - 1, gridDim.x);
+          }
+          const unsigned others = bar.join_c1 - bar.join_c0;
+          const unsigned done = atomicInc(&work.count[bar.join_c0], others);
+          __threadfence();
+          bar.join = done == others;
+        }
+        warp_arrive(&bar.both, lane);
+        ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
+        if (!ok) break;
+        const Piece here = p;
+        if (bar.join) join_pieces<T, kDim, Shape::kRows>(a, work, here, bar.join_c0, bar.join_c1, tid);
+      }
+      if (!kPair) {  // O, the maxima and the flags have been read; the next piece's first P waits for the other stream's
+        tc_fence_before();
+        warp_arrive(&bar.both, lane);
+        pending = true;
       }
       base = (base + 2 * n) % (2 * Shape::kStages);
     }
@@ -849,81 +1059,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     tmem_dealloc(tmem, 512);
   }
   if (tid == 0 && bar.abort_flag) atomicOr(a.status, DD_STATUS_TIMEOUT);
-}
-
-// The items that cross CTAs: CTA c's record names an item whose first tiles it
-// holds; the rest is in slot 0 of the CTAs behind it.  One warp per row: the
-// lanes read the pieces' (m, l) side by side, then the row is added up piece by
-// piece with several loads in flight.  Also the rows that no item covers:
-// behind the end of a short chunk, or with no key to see.
-constexpr int kJoinRows = 8;
-template <typename T, int kDim, bool kPair>
-__global__ void __launch_bounds__(32 * kJoinRows) attend_join_kernel(const __grid_constant__ AttendParams a,
-                                                                     const __grid_constant__ AttendWork work) {
-  constexpr int kRows = AttendShape<kDim, kPair>::kRows;
-  constexpr int kVec = kDim / 32;  // values per lane
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.group;
-  const int q_tiles = (a.tokens * group + kRows - 1) / kRows;
-  pdl_wait_primary();
-  const int4 head = work.head[blockIdx.x];
-  if (head.x >= 0) {
-    const int b = head.x / q_tiles, qt = head.x - b * q_tiles, h = head.y, c0 = blockIdx.x, c1 = head.z;
-    const int rows = (int)(a.lens ? min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens) * group;
-    const int row = blockIdx.y * kJoinRows + warp, r = qt * kRows + row;
-    if (r < a.tokens * group) {
-      float o[kVec] = {};
-      float m = -INFINITY, l = 0.0f;
-      for (int c = c0; r < rows && c <= c1; c += 32) {
-        // 32 pieces; CTAs without a tile (fewer tiles than CTAs) have left nothing
-        const int mine = c + lane;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (mine <= c1 && !(head.w > 0 && head.w * mine / (int)gridDim.x == head.w * (mine + 1) / (int)gridDim.x))
-          ml = work.ml[(2 * (size_t)mine + (mine == c0)) * kRows + row];
-        float top = ml.x;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float m1 = fmaxf(m, top), base = m1 == -INFINITY ? 0.0f : m1;
-        const float keep = exp2_approx(m - base);
-        const float w = ml.y == 0.0f ? 0.0f : exp2_approx(ml.x - base);  // l = 0: no key of the piece is seen
-        float sum = ml.y * w;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        l = l * keep + sum;
-        m = m1;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) o[i] *= keep;
-        const int pieces = min(32, c1 - c + 1);
-#pragma unroll 4
-        for (int k = 0; k < pieces; ++k) {
-          const float wk = __shfl_sync(0xffffffffu, w, k);
-          if (wk == 0.0f) continue;
-          const float* part = work.o + ((2 * (size_t)(c + k) + (c + k == c0)) * kRows + row) * kDim + lane * kVec;
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) o[i] += part[i] * wk;
-        }
-      }
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int t = r / group, g = r - t * group;
-      T* out = static_cast<T*>(a.out) + (((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + lane * kVec;
-      if (lane * kVec < a.dim)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) out[i] = io<T>::from_f(o[i] * inv);
-    }
-  }
-  const int blocks = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
-  for (int e = me; e < a.batch * q_tiles; e += blocks) {
-    const int b = e / q_tiles, qt = e - b * q_tiles;
-    if (tile_span(a, b, qt, kRows).n) continue;
-    const int r1 = min((qt + 1) * kRows, a.tokens * group);
-    for (int r = qt * kRows; r < r1; ++r) {
-      const int t = r / group, g = r - t * group;
-      for (int i = threadIdx.x; i < a.kv_heads * a.dim; i += 32 * kJoinRows) {
-        const int h = i / a.dim, d = i - h * a.dim;
-        static_cast<T*>(a.out)[(((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + d] = io<T>::from_f(0.0f);
-      }
-    }
-  }
 }
 
 }  // namespace dd

@@ -101,6 +101,27 @@ char* plane(const dd_paged_cache* c, int layer, int kv) {
   return static_cast<char*>(c->data) + (2ll * layer + kv) * plane_bytes(c);
 }
 
+// The cache's scratch: counters of dd_cache_attend (zero between calls), the
+// page calls' lists, and the attention's pieces.
+struct Scratch {
+  unsigned* count;
+  void* pages;
+  float* partial;
+  size_t bytes;
+};
+Scratch scratch_of(const dd_paged_cache* c) {
+  const size_t lists = (page_scratch_bytes(c->pages, c->batch, c->row_pages) + 255) / 256 * 256;
+  const size_t counters = (kMaxAttendCtas * sizeof(unsigned) + 255) / 256 * 256;
+  char* p = static_cast<char*>(c->scratch);
+  Scratch s;
+  s.count = reinterpret_cast<unsigned*>(p);
+  s.pages = p + counters;
+  s.partial = reinterpret_cast<float*>(p + counters + lists);
+  s.bytes = counters + lists;
+  if (c->dtype != DD_F32 && c->head_dim <= 128) s.bytes += attend_work_bytes(c->head_dim <= 64 ? 64 : 128, true);
+  return s;
+}
+
 // Launch with programmatic stream serialisation: the kernel may be scheduled
 // while its predecessor drains; every kernel here waits for it first thing.
 template <typename... K, typename... A>
@@ -138,7 +159,7 @@ struct PageCall {
 int page_call(const dd_paged_cache* c, const void* arg, const char* what, const DeviceScope& scope, PageCall* p) {
   if (!arg) return global_fail(DD_EINVAL, "%s: null argument", what);
   if (!scope.ok) return global_fail(DD_ECUDA, "%s: cannot select device %d", what, c->device);
-  p->s = page_scratch(c->scratch, c->pages, c->batch);
+  p->s = page_scratch(scratch_of(c).pages, c->pages, c->batch);
   return device_info(c->device, &p->dev);
 }
 
@@ -214,12 +235,6 @@ AttendPlan attend_plan(const dd_paged_cache* c, const dd_cache_attend_args* a) {
   p.pair = (long long)a->tokens * (a->heads / c->kv_heads) > 128;
   return p;
 }
-uint64_t attend_bytes(const AttendPlan& p, const DeviceInfo& dev) {
-  if (!p.tensor) return 0;
-  if (p.dim == 64) return p.pair ? attend_work_bytes<64, true>(dev.sms) : attend_work_bytes<64, false>(dev.sms);
-  return p.pair ? attend_work_bytes<128, true>(dev.sms) : attend_work_bytes<128, false>(dev.sms);
-}
-
 template <typename T, int kDim, bool kPair>
 int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendParams& p, const DeviceInfo& dev,
                   void* stream) {
@@ -232,15 +247,14 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, con
     DD_TRY(cudaFuncSetAttribute(attend_tc_kernel<T, kDim, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttSmem));
     ready[c->device] = true;
   }
+  const Scratch scratch = scratch_of(c);
   constexpr int kRows = AttendShape<kDim, kPair>::kRows;
+  const int grid = std::min(dev.sms, kMaxAttendCtas);
   AttendWork w;
-  w.head = static_cast<int4*>(args->workspace);
-  w.o = reinterpret_cast<float*>(w.head + dev.sms);
-  w.ml = reinterpret_cast<float2*>(w.o + (size_t)dev.sms * 2 * kRows * kDim);
-  rc = launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(dev.sms), dim3(kAttThreads), kAttSmem, stream, mk, mv, p, w);
-  if (rc) return rc;
-  return launch("attend join", attend_join_kernel<T, kDim, kPair>, dim3(dev.sms, kRows / kJoinRows), dim3(32 * kJoinRows), 0, stream,
-                p, w);
+  w.count = scratch.count;
+  w.o = scratch.partial;
+  w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * kRows * kDim);
+  return launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(grid), dim3(kAttThreads), kAttSmem, stream, mk, mv, p, w);
 }
 template <typename T>
 int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendPlan& plan, const AttendParams& p,
@@ -276,11 +290,11 @@ int check_attend(const dd_paged_cache* c, const dd_cache_attend_args* a) {
 
 extern "C" {
 
-int dd_pages_scratch(const dd_paged_cache* c, uint64_t* bytes) {
+int dd_cache_scratch(const dd_paged_cache* c, uint64_t* bytes) {
   int rc = check_shape(c);
   if (rc) return rc;
   if (!bytes) return global_fail(DD_EINVAL, "null argument");
-  *bytes = page_scratch_bytes(c->pages, c->batch, c->row_pages);
+  *bytes = scratch_of(c).bytes;
   return DD_OK;
 }
 
@@ -392,16 +406,6 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
   return launch_write<__nv_bfloat16>(p, c->batch, per_cta, il, vec, stream);
 }
 
-int dd_cache_attend_workspace(const dd_paged_cache* c, const dd_cache_attend_args* a, uint64_t* bytes) {
-  int rc = check_attend(c, a);
-  if (rc) return rc;
-  if (!bytes) return global_fail(DD_EINVAL, "null argument");
-  DeviceInfo dev;
-  if ((rc = device_info(c->device, &dev))) return rc;
-  *bytes = attend_bytes(attend_plan(c, a), dev);
-  return DD_OK;
-}
-
 int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void* stream) {
   int rc = check_attend(c, a);
   if (rc) return rc;
@@ -438,10 +442,8 @@ int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void
   const AttendPlan plan = attend_plan(c, a);
   const long long rows = (long long)a->tokens * p.group;
   p.copies = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+  p.min_tiles = 3;
   if (plan.tensor) {
-    if (!a->workspace || a->workspace_bytes < attend_bytes(plan, dev) || !aligned16(a->workspace))
-      return global_fail(DD_EINVAL, "dd_cache_attend: workspace of %llu bytes needed",
-                         (unsigned long long)attend_bytes(plan, dev));
     if (c->dtype == DD_FP16) return launch_attend<__half>(c, a, plan, p, dev, stream);
     return launch_attend<__nv_bfloat16>(c, a, plan, p, dev, stream);
   }

@@ -137,7 +137,7 @@ class PagedKVCache:
                                     dtype=_DTYPES[dtype])
         self._cp = ctypes.byref(self._c)
         need = ctypes.c_uint64()
-        rc = self._lib.dd_pages_scratch(self._cp, ctypes.byref(need))
+        rc = self._lib.dd_cache_scratch(self._cp, ctypes.byref(need))
         if rc < 0:
             raise ValueError(self._lib.dd_last_error(None).decode(errors="replace"))
         device = torch.device(device)
@@ -153,11 +153,10 @@ class PagedKVCache:
         self.length = torch.zeros(self.batch, dtype=torch.long, device=device)
         self.refs = torch.zeros(self.pages, dtype=torch.int32, device=device)
         self._status = torch.zeros(1, dtype=torch.int32, device=device)
-        self._scratch = torch.empty(need.value, dtype=torch.uint8, device=device)
+        self._scratch = torch.zeros(need.value, dtype=torch.uint8, device=device)
         c = self._c
         c.data, c.table, c.length, c.refs = (x.data_ptr() for x in (self.data, self.table, self.length, self.refs))
         c.scratch, c.status, c.device = self._scratch.data_ptr(), self._status.data_ptr(), device.index
-        self._workspace: dict = {}
 
     # ---------------------------------------------------------------- checks
     def _stream(self) -> int:
@@ -272,16 +271,7 @@ class PagedKVCache:
         a.scale = self.head_dim ** -0.5 if scale is None else scale
         a.q = q.data_ptr()
         a.q_stride[:] = q.stride()[:3]
-        key = (tokens, heads)
-        need = self._workspace.get(key)
-        if need is None:
-            n = ctypes.c_uint64()
-            self._check(self._lib.dd_cache_attend_workspace(self._cp, ctypes.byref(a), ctypes.byref(n)), "dd_cache_attend")
-            need = self._workspace[key] = n.value
         out = torch.empty(self.batch, tokens, heads, self.head_dim, dtype=self.dtype, device=self.device)
-        # from PyTorch's allocator for each call: a captured call keeps its own
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        a.workspace, a.workspace_bytes = (work.data_ptr() if need else None), need
         a.out = out.data_ptr()
         self._check(self._lib.dd_cache_attend(self._cp, ctypes.byref(a), self._stream()), "dd_cache_attend")
         return out
@@ -314,4 +304,6 @@ class PagedKVCache:
         """Synchronise and return (and clear) the ``DD_STATUS_*`` bits that calls have set."""
         s = int(self._status.item())
         self._status.zero_()
+        if s & _lib.DD_STATUS_TIMEOUT:  # an attention gave up half-way: its counters start anew
+            self._scratch.zero_()
         return s

@@ -291,7 +291,7 @@ int dd_set_trace(dd_handle* h, const dd_trace* t);
  * refs[p] counts the rows that hold page p; 0 means free.  Free pages are
  * taken lowest number first, so equal calls give equal tables.
  *   data    [layers, 2 (keys, values), pages, kv_heads, page_size, head_dim]
- *   scratch dd_pages_scratch bytes, used by the dd_pages_* calls only
+ *   scratch dd_cache_scratch bytes, 16-byte aligned, zero before the first call
  *   status  one word of DD_STATUS_* bits, set by the kernels, never cleared
  * Calls on one cache must be ordered (one stream, or events between streams).
  * Nothing here synchronises or allocates; everything can be captured. */
@@ -307,10 +307,10 @@ typedef struct dd_paged_cache {
   int32_t device;
 } dd_paged_cache;
 
-/* Bytes of scratch that the dd_pages_* calls need (also checks the shape):
+/* Bytes of scratch that the calls on a cache share (also checks the shape):
  * page_size 16, 32, 64 or 128; head_dim a multiple of 8, at most 256; batch
- * at most 1024. */
-int dd_pages_scratch(const dd_paged_cache* c, uint64_t* bytes);
+ * at most 1024; row_pages * page_size at most 2^30. */
+int dd_cache_scratch(const dd_paged_cache* c, uint64_t* bytes);
 
 /* Make positions length[b] .. upto[b] - 1 of every row writable: missing pages
  * are taken from the free ones, and a page that other rows hold too and that
@@ -365,19 +365,17 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
  *   out = sum_j softmax_j(scale q . K[j]) V[j]
  * Query heads h * heads / kv_heads ... share key head h.  A query that sees no
  * key, and every t >= lens[b], gives zeros.  Keys that a query does not see
- * have no effect on it, whatever they hold. */
+ * have no effect on it, whatever they hold.  start[b] outside +-2^30 counts as
+ * that bound.  bf16 / fp16 heads of up to 128 values run on the tensor cores. */
 typedef struct dd_cache_attend_args {
   const void* q;
   void* out;                  /* [batch, tokens, heads, head_dim] */
   int64_t q_stride[3];        /* batch, token, head, in elements */
   const int64_t* start;       /* [batch] */
   const int64_t* lens;        /* [batch], or NULL: all `tokens` */
-  void* workspace;            /* dd_cache_attend_workspace bytes, 16-byte aligned; not shared by overlapping calls */
-  uint64_t workspace_bytes;
   float scale;
   int32_t layer, tokens, heads, causal, window, sinks;
 } dd_cache_attend_args;
-int dd_cache_attend_workspace(const dd_paged_cache* c, const dd_cache_attend_args* a, uint64_t* bytes);
 int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void* stream);
 
 /* Launch kinds reported by dd_read_timing. */

@@ -64,7 +64,7 @@ def check_attend(c, out, q, keys, values, start, lens, causal=True, window=0, si
     seen = [torch.ones(k.shape[1], dtype=torch.bool) for k in keys] if seen is None else seen
     ref = R.attend(q.cpu(), keys, values, seen, start, lens, causal, window, sinks, scale)
     out = out.double().cpu()
-    assert torch.isfinite(out).all()
+    assert bool(torch.isfinite(out).all()), (~torch.isfinite(out)).nonzero()[:5].tolist()
     eps = torch.finfo(c.dtype).eps / 2
     for b in range(c.batch):
         vmax = values[b].abs().max().item() if values[b].numel() else 0.0
@@ -74,7 +74,7 @@ def check_attend(c, out, q, keys, values, start, lens, causal=True, window=0, si
         err = (out[b] - ref[b]).abs().max().item()
         assert err <= tol, (b, err, tol)
         n = min(int(lens[b]), q.shape[1])
-        assert (out[b, n:] == 0).all()
+        assert bool((out[b, n:] == 0).all())
     return ref
 
 

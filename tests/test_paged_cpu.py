@@ -31,11 +31,11 @@ def full(**kw):
 @pytest.mark.parametrize("bad", [dict(layers=0), dict(batch=0), dict(batch=1025), dict(kv_heads=0), dict(pages=0),
                                  dict(row_pages=0), dict(page_size=48), dict(page_size=8), dict(page_size=256),
                                  dict(head_dim=0), dict(head_dim=12), dict(head_dim=264), dict(dtype=7),
-                                 dict(pages=1 << 30, kv_heads=4), dict(batch=1024, row_pages=1 << 22)])
+                                 dict(pages=1 << 30, kv_heads=4), dict(batch=1024, row_pages=1 << 22), dict(row_pages=(1 << 24) + 1)])
 def test_cache_shapes_refused(lib, bad):
     from domino_b200 import PagedKVCache, _lib
     n = ctypes.c_uint64()
-    assert lib.dd_pages_scratch(ctypes.byref(shape(**bad)), ctypes.byref(n)) == _lib.DD_EINVAL
+    assert lib.dd_cache_scratch(ctypes.byref(shape(**bad)), ctypes.byref(n)) == _lib.DD_EINVAL
     assert b"paged cache" in lib.dd_last_error(None)
     if "dtype" not in bad:
         args = dict(layers=1, batch=2, kv_heads=2, pages=4, head_dim=64, dtype=torch.bfloat16, device="cuda", row_pages=2)
