@@ -25,6 +25,8 @@ struct AttendParams {
   int batch, tokens, heads, kv_heads, dim, pages, page_size, page_shift, row_pages;  // page_size = 1 << page_shift
   int group;                 // query heads per key head
   int copies;                // copies of the rows in a query tile of the tensor-core kernel: 1, 2 or 4
+  int tile_rows, item_rows;  // rows of a query tile (whole tokens, at most 128) and of the tiles of one item
+  int q_tma;                 // the queries' layout allows TMA
   int min_tiles;             // key tiles that a CTA of that kernel takes at least
   int causal, window, sinks;
 };

@@ -44,10 +44,6 @@ namespace dd {
 constexpr int kAttThreads = 384;  // 8 softmax warps, key producer, MMA issuer, value producer, query loader
 constexpr int kKeyTile = 128;
 constexpr int kMaxStages = 12;
-#ifndef POLY
-#define POLY 3
-#endif
-constexpr int kPolyOf8 = POLY;  // of 8 pairs of exponentials
 constexpr int kMergeCols = 16;  // of the two buffers of each stream's warps that join copies of rows
 
 struct AttendWork {
@@ -208,33 +204,6 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
-// 2^x for two values, x in [-126, 127], on the FMA units: x = n + f with |f| <=
-// 1/2 (adding 1.5 * 2^23 rounds to the integer n, whose low bits then stand in
-// the sum), 2^f by a polynomial with the smallest largest relative error on
-// that interval (fitted for this; 7.5e-5 with degree 3 for bf16 weights, 2.6e-6
-// with degree 4 for fp16), and n added to the exponent.
-template <typename T>
-__device__ __forceinline__ void exp2_poly2(uint64_t x, float& p0, float& p1) {
-  const uint64_t round = pack_f32x2(12582912.0f, 12582912.0f), unround = pack_f32x2(-12582912.0f, -12582912.0f);
-  const uint64_t n = add_f32x2(x, round);
-  const uint64_t f = fma_f32x2(add_f32x2(n, unround), pack_f32x2(-1.0f, -1.0f), x);
-  uint64_t y;
-  if constexpr (std::is_same<T, __half>::value) {
-    y = fma_f32x2(f, pack_f32x2(0.0095701017f, 0.0095701017f), pack_f32x2(0.0559178603f, 0.0559178603f));
-    y = fma_f32x2(y, f, pack_f32x2(0.2402474483f, 0.2402474483f));
-    y = fma_f32x2(y, f, pack_f32x2(0.6931218147f, 0.6931218147f));
-    y = fma_f32x2(y, f, pack_f32x2(0.9999992614f, 0.9999992614f));
-  } else {
-    y = fma_f32x2(f, pack_f32x2(0.0551716672f, 0.0551716672f), pack_f32x2(0.2426111221f, 0.2426111221f));
-    y = fma_f32x2(y, f, pack_f32x2(0.6932609858f, 0.6932609858f));
-    y = fma_f32x2(y, f, pack_f32x2(0.9999280736f, 0.9999280736f));
-  }
-  float y0, y1, n0, n1;
-  unpack_f32x2(y, y0, y1);
-  unpack_f32x2(n, n0, n1);
-  p0 = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
-  p1 = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
-}
 // The n lowest bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 // Scores that are not seen become -infinity.
@@ -297,7 +266,7 @@ template <typename T, int kDim, int kRows>
 __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork& work, const Piece& p, int c0, int c1,
                                          int tid) {
   constexpr int kVec = kDim / 32, kBatch = 4;  // values per lane, rows at a time
-  const int lane = tid & 31, r0 = p.qt * kRows, last = min(kRows, a.tokens * a.group - r0);
+  const int lane = tid & 31, r0 = p.qt * a.item_rows, last = min(a.item_rows, a.tokens * a.group - r0);
   for (int row0 = tid >> 5; row0 < last; row0 += 8 * kBatch) {
     float o[kBatch][kVec] = {}, m[kBatch], l[kBatch];
 #pragma unroll
@@ -369,6 +338,7 @@ struct AttendShape {
   static constexpr int kTiles = kPair ? 2 : 1;      // query tiles
   static constexpr int kRows = 128 * kTiles;
   static constexpr int kHalves = kDim / 64;
+  static constexpr int kParts = kPair ? 2 : 1;      // parts of a key tile with scores and weights of their own
   static constexpr int kTileBytes = 128 * kDim * 2;  // a query tile, a K or V tile
   static constexpr int kMergeBytes = kPair ? 0 : 2 * 2 * 128 * kMergeCols * 4;
   static constexpr int kFit = (224 * 1024 - kTiles * kTileBytes - kMergeBytes) / kTileBytes;
@@ -378,7 +348,7 @@ struct AttendShape {
 // Behind the tiles in shared memory.
 struct AttendShared {
   uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t s_full[2], p_full[2], o_full[2], q_full, q_empty, wg[2], both;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], o_full[2], q_full, q_empty, wg[2], both;
   Piece first;          // where the run starts; left = 0: the CTA has none
   long long total, unit0;
   uint32_t tmem_base;
@@ -437,7 +407,8 @@ __device__ __forceinline__ void block_scan2(AttendShared& sh, long long& before,
 template <typename T, int kDim, bool kPair>
 __global__ void __launch_bounds__(kAttThreads, 1)
     attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const __grid_constant__ AttendParams a, const __grid_constant__ AttendWork work) {
+                     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ AttendParams a,
+                     const __grid_constant__ AttendWork work) {
   using Shape = AttendShape<kDim, kPair>;
   extern __shared__ unsigned char smem_raw[];
   const int pad = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
@@ -450,7 +421,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   AttendShared& bar = *reinterpret_cast<AttendShared*>(sm_q + 224 * 1024);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.group;
-  const int q_tiles = (a.tokens * group + Shape::kRows - 1) / Shape::kRows;
+  const int q_tiles = (a.tokens * group + a.item_rows - 1) / a.item_rows;
 
   if (tid == 0) {
     bar.abort_flag = 0;
@@ -460,12 +431,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       mbar_init(&bar.empty[i], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bar.s_full[s], 1);
-      mbar_init(&bar.p_full[s], 4);  // one arrival per warp
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&bar.s_full[s][k], 1);
+        mbar_init(&bar.p_full[s][k], 4);  // one arrival per warp
+      }
+      mbar_init(&bar.pv_done[s], 1);
       mbar_init(&bar.o_full[s], 1);
       mbar_init(&bar.wg[s], 4);
     }
-    mbar_init(&bar.q_full, 32);
+    mbar_init(&bar.q_full, 1);
     mbar_init(&bar.q_empty, 1);
     mbar_init(&bar.both, 8);
     fence_mbar_init();
@@ -486,7 +460,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     long long tiles = 0;
     int items = 0;
     for (mine.e = e0; mine.e < e1; ++mine.e) {
-      piece_enter(a, mine, q_tiles, Shape::kRows);
+      piece_enter(a, mine, q_tiles, a.item_rows);
       tiles += mine.span.n;
       items += mine.span.n > 0;
     }
@@ -505,7 +479,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         long long rem = u0 - before;
         int len = 0;
         for (mine.e = e0; mine.e < e1; ++mine.e) {
-          if (per > 1) piece_enter(a, mine, q_tiles, Shape::kRows);
+          if (per > 1) piece_enter(a, mine, q_tiles, a.item_rows);
           len = mine.span.n ? mine.span.n + kItemUnits : 0;
           if (rem < (long long)len * a.kv_heads) break;
           rem -= (long long)len * a.kv_heads;
@@ -530,7 +504,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       for (int e = e0; e < e1; ++e) {
         if (per > 1) {
           mine.e = e;
-          piece_enter(a, mine, q_tiles, Shape::kRows);
+          piece_enter(a, mine, q_tiles, a.item_rows);
         }
         ctas += item_ctas(a, mine.span.n, tiles, spare);
       }
@@ -539,7 +513,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       if ((int)blockIdx.x >= ctas * a.kv_heads && (int)blockIdx.x < (ctas + mine_ctas) * a.kv_heads) {
         int rem = blockIdx.x - (int)ctas * a.kv_heads, k = 1;
         for (mine.e = e0; mine.e < e1; ++mine.e) {
-          if (per > 1) piece_enter(a, mine, q_tiles, Shape::kRows);
+          if (per > 1) piece_enter(a, mine, q_tiles, a.item_rows);
           k = item_ctas(a, mine.span.n, tiles, spare);
           if (rem < k * a.kv_heads) break;
           rem -= k * a.kv_heads;
@@ -579,7 +553,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     const uint32_t page_bytes = a.page_size * 128u;  // of one 64-value half
     int base = 0;  // loads before this piece, modulo two rounds of the ring
     bool ok = true;
-    for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+    for (; more && ok; more = piece_next(a, p, q_tiles, a.item_rows)) {
       const int n = p.i1 - p.i0;
       PageWindow window;
       for (int i = 0; i < n; ++i) {
@@ -612,9 +586,10 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // then stay in uniform registers (issued from inside a lane's own branch,
     // each MMA cost about 100 cycles and the issue bound the kernel).
     constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t idesc_s = idesc_f16(128, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
+    constexpr int kPartKeys = kKeyTile / Shape::kParts;
+    constexpr uint32_t idesc_s = idesc_f16(kPartKeys, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
     Ring<Shape::kStages> ring;
-    uint32_t n_pieces = 0, n_p[2] = {0, 0};
+    uint32_t n_pieces = 0, n_p[2] = {0, 0};  // tiles whose weights stream s has delivered
     bool ok = true;
     auto wait = [&](uint64_t* b, uint32_t parity) {
       ok = ok && mbar_wait_bounded(b, parity, abort);
@@ -628,124 +603,148 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       return st;
     };
     const uint32_t ring0 = smem_u32(sm_ring), q0 = smem_u32(sm_q);
-    // S of stream s from the keys in stage st, and which buffers are free once it is done
-    auto qk = [&](int s, int st, bool free_stage, bool free_q) {
+    // Scores of stream s from a part of the keys in stage st, and which buffers are free once they are done.
+    auto qk = [&](int s, int part, int st, bool free_stage, bool free_q) {
       const uint64_t dq = smem_desc_k_sw128(q0 + (kPair ? s * Shape::kTileBytes : 0));
-      const uint64_t dk = smem_desc_k_sw128(ring0 + st * Shape::kTileBytes);
+      const uint64_t dk = smem_desc_k_sw128(ring0 + st * Shape::kTileBytes + part * kPartKeys * 128);
       if (elect_one()) {
 #pragma unroll
         for (int d = 0; d < kDim / 16; ++d) {
           const uint64_t off = ((d / 4) * 128 * 128 + (d % 4) * 32) >> 4;
-          mma_f16_ss(tmem + s * 128, dq + off, dk + off, idesc_s, d > 0);
+          mma_f16_ss(tmem + s * 128 + part * kPartKeys, dq + off, dk + off, idesc_s, d > 0);
         }
-        mma_commit(&bar.s_full[s]);
+        mma_commit(&bar.s_full[s][part]);
         if (free_stage) mma_commit(&bar.empty[st]);
         if (free_q) mma_commit(&bar.q_empty);
       }
       __syncwarp();
     };
-    auto pv = [&](int s, int st, bool accumulate, bool free_stage, bool last) {
-      const uint64_t dv = smem_desc_mn_sw128(ring0 + st * Shape::kTileBytes, 128 * 128);
+    auto pv = [&](int s, int part, int st, bool accumulate, bool free_stage, bool last) {
+      const uint64_t dv = smem_desc_mn_sw128(ring0 + st * Shape::kTileBytes + part * kPartKeys * 128, 128 * 128);
       if (elect_one()) {
 #pragma unroll
-        for (int d = 0; d < kKeyTile / 16; ++d)
-          mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + d * 8, dv + ((d * 2048) >> 4), idesc_o, accumulate || d > 0);
+        for (int d = 0; d < kPartKeys / 16; ++d)
+          mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + part * kPartKeys + d * 8, dv + ((d * 2048) >> 4), idesc_o,
+                     accumulate || d > 0);
+        if (Shape::kParts > 1) mma_commit(&bar.pv_done[s]);
         if (free_stage) mma_commit(&bar.empty[st]);
         if (last) mma_commit(&bar.o_full[s]);
       }
       __syncwarp();
     };
-    auto wait_p = [&](int s) {
-      wait(&bar.p_full[s], n_p[s]++ & 1);
+    auto wait_p = [&](int s, int part) {
+      wait(&bar.p_full[s][part], (part + 1 == Shape::kParts ? n_p[s]++ : n_p[s]) & 1);
       tc_fence_after();
     };
-    for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+    for (; more && ok; more = piece_next(a, p, q_tiles, a.item_rows)) {
       const int n = p.i1 - p.i0;
       wait(&bar.q_full, n_pieces++ & 1);
       if (!ok) break;
       tc_fence_after();
       if (kPair) {
+        constexpr int kSteps = 2 * Shape::kParts;
         int k = take(), v = 0;
         if (!ok) break;
-        qk(0, k, false, false);
-        qk(1, k, true, n == 1);
+        // parts outside, streams inside: while one stream's exponentials of a
+        // part run, the tensor cores have its other part and the other stream
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) qk(u & 1, u >> 1, k, u == kSteps - 1, u == kSteps - 1 && n == 1);
         for (int i = 0; i < n && ok; ++i) {
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            wait_p(s);
-            if (s == 0 && ok) v = take();
+          for (int u = 0; u < kSteps; ++u) {
+            const int s = u & 1, part = u >> 1;
+            wait_p(s, part);
+            if (u == 0 && ok) v = take();
             if (!ok) break;
-            pv(s, v, i > 0, s == 1, i + 1 == n);
+            pv(s, part, v, i > 0 || part > 0, u == kSteps - 1, i + 1 == n && part + 1 == Shape::kParts);
             if (i + 1 < n) {
-              if (s == 0) k = take();
+              if (u == 0) k = take();
               if (!ok) break;
-              qk(s, k, s == 1, s == 1 && i + 2 == n);
+              qk(s, part, k, u == kSteps - 1, u == kSteps - 1 && i + 2 == n);
             }
           }
         }
       } else {
         for (int s = 0; s < min(2, n) && ok; ++s) {
           const int k = take();
-          if (ok) qk(s, k, true, s + 1 == n);
+          if (ok) qk(s, 0, k, true, s + 1 == n);
         }
         for (int i = 0; i < n && ok; ++i) {
           const int s = i & 1;
-          wait_p(s);
+          wait_p(s, 0);
           if (!ok) break;
           const int v = take();
           if (!ok) break;
-          pv(s, v, i >= 2, true, i + 2 >= n);
+          pv(s, 0, v, i >= 2, true, i + 2 >= n);
           if (i + 2 < n) {
             const int k = take();
-            if (ok) qk(s, k, true, i + 3 == n);
+            if (ok) qk(s, 0, k, true, i + 3 == n);
           }
         }
       }
     }
   } else if (warp == 11) {
     // ---------------------------------------------------------------- query loader, and the rows of no item
-    // 16-byte asynchronous copies, all of a piece's in flight at once; a thread
-    // keeps one chunk of the row and steps through the rows.
+    // A tile holds whole tokens (128 / group of them), so one box of [tokens,
+    // heads of the group, 64 values] fills it.  Where q's layout does not allow
+    // TMA: 16-byte asynchronous copies, a thread keeping one chunk of the rows,
+    // or plain loads.
     constexpr int kChunks = kDim / 8, kRowStep = 32 / kChunks;
     const int ch = lane % kChunks;
     const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride[0] % 8 == 0 && a.q_stride[1] % 8 == 0 &&
                      a.q_stride[2] % 8 == 0;
-    const int copy_rows = kPair ? Shape::kRows : 128 / a.copies;
+    const int copies = kPair ? 1 : a.copies, copy_rows = 128 / copies, live_rows = kPair ? 128 : copy_rows;
     uint32_t n_pieces = 0;
     bool ok = true;
-    for (; more; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+    for (; more; more = piece_next(a, p, q_tiles, a.item_rows)) {
       ok = mbar_wait_bounded(&bar.q_empty, (n_pieces++ & 1) ^ 1, abort);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const int r0 = p.qt * Shape::kRows, live = min(Shape::kRows, p.span.rows - r0);
-      const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + (long long)p.h * group * a.q_stride[2] + ch * 8;
-      int row = lane / kChunks, t = (r0 + row) / group, g = r0 + row - t * group;
-      for (; row < live; row += kRowStep) {
-        const T* src = q + t * a.q_stride[1] + g * a.q_stride[2];
-        const bool in = ch * 8 < a.dim;
-        for (int to = row; to < (kPair ? row + 1 : 128); to += copy_rows) {
-          unsigned char* dst = sm_q + (to / 128) * Shape::kTileBytes + (ch / 8) * 128 * 128 + (to % 128) * 128 +
-                               ((ch % 8) ^ (to % 8)) * 16;
-          if (vec) {
-            cp_async16(dst, in ? src : a.q, in ? 16 : 0);
-          } else {
-            alignas(16) T x[8];
+      const int r0 = p.qt * a.item_rows;
+      if (a.q_tma) {
+        const int box = copy_rows / group;  // tokens
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&bar.q_full, Shape::kTiles * copies * Shape::kHalves * box * group * 128);
+          for (int i = 0; i < Shape::kTiles * copies; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = in ? src[i] : io<T>::from_f(0.0f);
-            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
-          }
+            for (int hf = 0; hf < Shape::kHalves; ++hf)
+              tma_load_4d(sm_q + (kPair ? i * Shape::kTileBytes : i * copy_rows * 128) + hf * 128 * 128, &map_q, &bar.q_full,
+                          hf * 64, p.h * group, r0 / group + (kPair ? i * box : 0), p.b);
         }
-        for (g += kRowStep; g >= group; g -= group) ++t;
+        __syncwarp();
+        continue;
+      }
+      const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + (long long)p.h * group * a.q_stride[2] + ch * 8;
+      const bool in = ch * 8 < a.dim;
+      for (int tile = 0; tile < Shape::kTiles; ++tile) {
+        const int first_row = r0 + tile * a.tile_rows, rows = min(min(a.tile_rows, live_rows), p.span.rows - first_row);
+        int row = lane / kChunks, t = (first_row + row) / group, g = first_row + row - t * group;
+        for (; row < rows; row += kRowStep) {
+          const T* src = q + t * a.q_stride[1] + g * a.q_stride[2];
+          for (int to = row; to < 128; to += live_rows) {
+            unsigned char* dst = sm_q + tile * Shape::kTileBytes + (ch / 8) * 128 * 128 + to * 128 + ((ch % 8) ^ (to % 8)) * 16;
+            if (vec) {
+              cp_async16(dst, in ? src : a.q, in ? 16 : 0);
+            } else {
+              alignas(16) T x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = in ? src[i] : io<T>::from_f(0.0f);
+              *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
+            }
+          }
+          for (g += kRowStep; g >= group; g -= group) ++t;
+        }
       }
       cp_async_wait_all();
       fence_proxy_async_shared();
-      mbar_arrive(&bar.q_full);
+      warp_arrive(&bar.q_full, lane);
     }
     // query tiles with nothing to see or behind the end of a short chunk: zeros
     for (int e = blockIdx.x; e < a.batch * q_tiles; e += gridDim.x) {
       const int b = e / q_tiles, qt = e - b * q_tiles;
-      if (tile_span(a, b, qt, Shape::kRows).n) continue;
-      const int r1 = min((qt + 1) * Shape::kRows, a.tokens * group);
-      for (int r = qt * Shape::kRows; r < r1; ++r) {
+      if (tile_span(a, b, qt, a.item_rows).n) continue;
+      const int r1 = min((qt + 1) * a.item_rows, a.tokens * group);
+      for (int r = qt * a.item_rows; r < r1; ++r) {
         const int t = r / group, g = r - t * group;
         for (int i = lane; i < a.kv_heads * (a.dim / 8); i += 32) {
           const int h = i / (a.dim / 8), d = (i - h * (a.dim / 8)) * 8;
@@ -756,12 +755,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax, one thread per query row
+    constexpr int kPartKeys = kKeyTile / Shape::kParts;
     constexpr int kCols = kPair ? 2 : 1;  // groups of 32 columns in registers at a time
     const int s = warp >> 2, row = tid & 127;
     const uint32_t lanes = ((warp & 3) * 32u) << 16;
     const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + lanes;
     const float sl = a.scale * 1.4426950408889634f;
-    uint32_t n_s = 0, n_o[2] = {0, 0}, n_wg = 0, n_both = 0, n_pieces = 0;
+    uint32_t n_s = 0, n_part = 0, n_o[2] = {0, 0}, n_wg = 0, n_both = 0, n_pieces = 0;
     int base = 0;  // loads before this piece, modulo two rounds of the ring
     bool ok = true, pending = false;
     // Few rows: the tile holds `copies` copies of them, and copy c of a row
@@ -769,37 +769,48 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // warps share the exponentials.  The copies are joined like the streams.
     const int copies = kPair ? 1 : a.copies, copy_rows = 128 / copies;
     const int chunk0 = (row / copy_rows) * (4 / copies), chunk1 = chunk0 + 4 / copies;
-    for (; more && ok; more = piece_next(a, p, q_tiles, Shape::kRows)) {
+    for (; more && ok; more = piece_next(a, p, q_tiles, a.item_rows)) {
       const int n = p.i1 - p.i0;
       ++n_pieces;
-      const int tile0 = p.qt * Shape::kRows + (kPair ? s * 128 : 0), r = tile0 + (kPair ? row : row % copy_rows);
-      const bool warp_live = r - lane < p.span.rows;
+      const int tile0 = p.qt * a.item_rows + (kPair ? s * a.tile_rows : 0), in_tile = kPair ? row : row % copy_rows;
+      const int rows_here = min(p.span.rows - tile0, a.tile_rows);  // live rows of the tile
+      const int r = tile0 + in_tile;
+      const bool live = in_tile < rows_here, warp_live = in_tile - lane < rows_here;
       // keys that the row sees: [lo, hi) and, below hi, [0, sinks)
       int hi = 0, lo = 0;
-      if (r < p.span.rows) {
+      if (live) {
         const int pos = p.span.start + r / group;
         hi = a.causal ? min(p.span.hi, pos + 1) : p.span.hi;
         lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
       }
       // rows of the item see all keys of [all_lo, all_hi)
-      const int p_min = p.span.start + p.qt * Shape::kRows / group;
-      const int p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * Shape::kRows) - 1) / group;
+      const int p_min = p.span.start + p.qt * a.item_rows / group;
+      const int p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * a.item_rows) - 1) / group;
       const int all_hi = a.causal ? min(p.span.hi, p_min + 1) : p.span.hi;
       const int all_lo = a.window > 0 ? max(p_max - a.window + 1, 0) : 0;
       float m = -INFINITY, l = 0.0f;
       bool have_o = false;
       constexpr int kStep = kPair ? 1 : 2;
       int page = (kPair ? 0 : s) < n ? group_page(a, p.b, p.span.tile(p.i0 + (kPair ? 0 : s)), lane) : 0;
-      for (int i = kPair ? 0 : s; i < n; i += kStep) {
+      if (!kPair && pending) {  // the last piece's O, maxima and flags have been read by all
+        ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
+        if (!ok) break;
+        pending = false;
+      }
+      for (int i = kPair ? 0 : s; i < n && ok; i += kStep) {
         const int tile = p.span.tile(p.i0 + i);
-        const int key0 = tile * kKeyTile, key1 = key0 + kKeyTile;
         // 16-key groups without a page (read one tile ahead)
         const unsigned missing = __ballot_sync(0xffffffffu, lane < 8 && (page < 0 || page >= a.pages));
         if (i + kStep < n) page = group_page(a, p.b, p.span.tile(p.i0 + i + kStep), lane);
-        const bool whole = missing == 0 && key1 <= all_hi && (key0 >= all_lo || key1 <= a.sinks);
-        ok = mbar_wait_bounded(&bar.s_full[s], n_s++ & 1, abort);
+#pragma unroll 1
+        for (int part = 0; part < Shape::kParts; ++part, ++n_part) {
+        const int key0 = tile * kKeyTile, part0 = key0 + part * kPartKeys, part1 = part0 + kPartKeys;
+        const bool whole = missing == 0 && part1 <= all_hi && (part0 >= all_lo || part1 <= a.sinks);
+        ok = mbar_wait_bounded(&bar.s_full[s][part], n_s & 1, abort);
         if (!ok) break;
+        if (part + 1 == Shape::kParts) ++n_s;
         tc_fence_after();
+        const int chunk_a = kPair ? part * (kPartKeys / 32) : chunk0, chunk_b = kPair ? chunk_a + kPartKeys / 32 : chunk1;
         if (warp_live) {
           // bit k: the row sees key 32 c + k of the tile
           auto see = [&](int c) {
@@ -807,16 +818,21 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             const uint32_t gap = (missing >> (2 * c) & 1) * 0xffffu | (missing >> (2 * c + 1) & 1) * 0xffff0000u;
             return low_bits(hi - k0) & (~low_bits(lo - k0) | low_bits(a.sinks - k0)) & ~gap;
           };
-          float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c = chunk0; c < chunk1; c += kCols) {
-            uint32_t x[32 * kCols];
+          // kCols x 32 scores in registers at a time; where that is not all of
+          // the thread's, they are read again for the exponentials.
+          uint32_t x[32 * kCols];
+          auto fetch = [&](int c) {
 #pragma unroll
             for (int d = 0; d < kCols; ++d) tmem_ld32(t_s + 32 * (c + d), x + 32 * d);
             tmem_ld_wait();
+            if (!whole)
 #pragma unroll
-            for (int d = 0; d < kCols; ++d)
-              if (!whole) mask32(x + 32 * d, see(c + d));
+              for (int d = 0; d < kCols; ++d) mask32(x + 32 * d, see(c + d));
+          };
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = chunk_a; c < chunk_b; c += kCols) {
+            fetch(c);
 #pragma unroll
             for (int k = 0; k < 32 * kCols; k += 4) {
               top[0] = max3_nan(top[0], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
@@ -832,6 +848,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             l *= keep;
             m = m1;
             if (have_o) {
+              // (the scores of part k come after the products of part k - 2; those of k - 1 may still run)
+              if (Shape::kParts > 1) ok = mbar_wait_bounded(&bar.pv_done[s], (n_part - 1) & 1, abort);
+              if (Shape::kParts > 1) tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < kDim; c += 32) {
                 uint32_t o[32];
@@ -845,38 +864,30 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           }
           have_o = true;
           const float sub = m == -INFINITY ? 0.0f : m * sl;
-          uint64_t sum = 0;  // (two fp32 zeros)
+          uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
           const uint64_t sl2 = pack_f32x2(sl, sl), sub2 = pack_f32x2(-sub, -sub);
 #pragma unroll 1
-          for (int c = chunk0; c < chunk1; c += kCols) {
-            uint32_t x[32 * kCols];
-#pragma unroll
-            for (int d = 0; d < kCols; ++d) tmem_ld32(t_s + 32 * (c + d), x + 32 * d);
-            tmem_ld_wait();
+          for (int c = chunk_a; c < chunk_b; c += kCols) {
+            if (chunk_b - chunk_a > kCols) fetch(c);
 #pragma unroll
             for (int d = 0; d < kCols; ++d) {
               uint32_t w[16];
-              if (!whole) mask32(x + 32 * d, see(c + d));
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
                 const uint64_t e = fma_f32x2(pack_f32x2(__uint_as_float(x[32 * d + 2 * k]), __uint_as_float(x[32 * d + 2 * k + 1])),
                                              sl2, sub2);
-                float e0, e1, p0, p1;
+                float e0, e1;
                 unpack_f32x2(e, e0, e1);
-                if (k % 8 < kPolyOf8) {
-                  exp2_poly2<T>(pack_f32x2(fmaxf(e0, -126.0f), fmaxf(e1, -126.0f)), p0, p1);
-                } else {
-                  p0 = exp2_approx(e0);
-                  p1 = exp2_approx(e1);
-                }
-                sum = add_f32x2(sum, pack_f32x2(p0, p1));
+                const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
+                sum[k & 3] = add_f32x2(sum[k & 3], pack_f32x2(p0, p1));
                 w[k] = pack2<T>(p0, p1);
               }
-              tmem_st16(t_s + 16 * (c + d), w);  // over scores that have been read
+              // over scores that have been read, a part's weights within its own columns
+              tmem_st16(t_s + (kPair ? part * kPartKeys + 16 * (c + d - chunk_a) : 16 * (c + d)), w);
             }
           }
           float sum0, sum1;
-          unpack_f32x2(sum, sum0, sum1);
+          unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), sum0, sum1);
           l += sum0 + sum1;
           if (!kPair && copies > 1) {  // the other copies' keys
             const uint32_t zero[16] = {};
@@ -892,11 +903,11 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           ok = mbar_wait_bounded(&bar.full[st], c / Shape::kStages, abort);
           if (!ok) break;
           // keys that no row of the item sees become zero; those that only some see are searched.
-          // Eight lanes a 128-byte row, four rows a step, 32 keys a warp.
+          // Eight lanes a 128-byte row, four rows a step.
           unsigned char* v = sm_ring + st * Shape::kTileBytes + (lane % 8) * 16;
           bool odd = false, wrote = false;
 #pragma unroll 1
-          for (int k = (warp & 3) * 32 + lane / 8, k1 = k + 32; k < k1; k += 4) {
+          for (int k = part * kPartKeys + (warp & 3) * (kPartKeys / 4) + lane / 8, k1 = k + kPartKeys / 4; k < k1; k += 4) {
             const int j = key0 + k;
             const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (k / 16) & 1);
             const bool search = seen && (j >= all_hi || (j < all_lo && j >= a.sinks));
@@ -915,19 +926,16 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           if (wrote) fence_proxy_async_shared();
           if (odd) bar.redo[s] = n_pieces;
         }
-        if (!kPair && pending) {
-          ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
-          if (!ok) break;
-          pending = false;
-        }
         tc_fence_before();
-        warp_arrive(&bar.p_full[s], lane);
+        warp_arrive(&bar.p_full[s][part], lane);
+        }
       }
       if (!ok) break;
       // the piece's result
       const bool split = p.i0 > 0 || p.i1 < p.span.n;
       const size_t slot = 2 * (size_t)blockIdx.x + (p.i0 == 0 ? 1 : 0);
-      const int slot_row = kPair ? s * 128 + row : row;
+      const int slot_row = (kPair ? s * a.tile_rows : 0) + in_tile;
+      const bool in_chunk = in_tile < a.tile_rows && r < a.tokens * group;
       float* part = work.o + slot * Shape::kRows * kDim;
       float2* part_ml = work.ml + slot * Shape::kRows;
       auto out_row = [&](int r) {
@@ -948,11 +956,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
         if (!ok) break;
       } else {
-        if (pending) {  // (a stream without a tile in this piece)
-          ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
-          if (!ok) break;
-          pending = false;
-        }
         bar.row_ml[s][row] = make_float2(m, l);
         ok = mbar_wait_bounded(&bar.o_full[0], n_o[0]++ & 1, abort);
         if (ok && n > 1) ok = mbar_wait_bounded(&bar.o_full[1], n_o[1]++ & 1, abort);
@@ -977,23 +980,22 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (again) {
-        if ((kPair || (s == 0 && row < copy_rows)) && r < a.tokens * group) {
+        if ((kPair || (s == 0 && row < copy_rows)) && in_chunk) {
           const Piece here = p;
           float o[kDim], m_x = -INFINITY, l_x = 0.0f;
           for (int d = 0; d < kDim; ++d) o[d] = 0.0f;
-          if (r < p.span.rows) attend_row_exact<T, kDim>(a, here, r, o, &m_x, &l_x);
+          if (live) attend_row_exact<T, kDim>(a, here, r, o, &m_x, &l_x);
           const float inv_x = l_x == 0.0f ? 0.0f : 1.0f / l_x;
           if (split) {
             for (int d = 0; d < kDim; ++d) part[(size_t)slot_row * kDim + d] = o[d];
             part_ml[slot_row] = make_float2(m_x, l_x);
           } else {
             T* out = out_row(r);
-            for (int d = 0; d < a.dim; ++d) out[d] = io<T>::from_f(r < p.span.rows ? o[d] * inv_x : 0.0f);
+            for (int d = 0; d < a.dim; ++d) out[d] = io<T>::from_f(live ? o[d] * inv_x : 0.0f);
           }
         }
       } else if (kPair) {
-        const bool in_chunk = r < a.tokens * group, live = r < p.span.rows;
-        if (split) part_ml[slot_row] = make_float2(m, l);
+        if (split && in_tile < a.tile_rows) part_ml[slot_row] = make_float2(m, l);
         const float norm = split ? 1.0f : inv;
         T* out = out_row(r);
 #pragma unroll 1
@@ -1026,9 +1028,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         // streams' sums by row, the copies of a row through shared memory, and
         // out with four lanes a row.
         if (split && s == 0 && row < copy_rows) part_ml[row] = make_float2(m, l);
-        bar.row_norm[row] = r < p.span.rows ? inv : 0.0f;  // (both streams write the same)
+        bar.row_norm[row] = live ? inv : 0.0f;  // (both streams write the same)
         float4* merge = reinterpret_cast<float4*>(sm_q + 224 * 1024 - Shape::kMergeBytes) + s * 2 * 128 * 4;
-        const int rows = min(p.span.rows, copy_rows), all_rows = min(a.tokens * group, copy_rows);
+        const int rows = min(rows_here, copy_rows), all_rows = min(a.tokens * group, copy_rows);
 #pragma unroll 1
         for (int c = s * (kDim / 2), c_end = c + kDim / 2; c < c_end; c += kMergeCols) {
           if (warp_live) {

@@ -222,6 +222,26 @@ int encode_pool(const dd_paged_cache* c, int layer, int kv, CUtensorMap* m) {
   return DD_OK;
 }
 
+// The queries as [batch, tokens, heads, head_dim] in boxes of `box` tokens x
+// one key head's group of heads x 64 values; false where TMA cannot read them.
+bool encode_queries(const dd_paged_cache* c, const dd_cache_attend_args* a, int group, int box, CUtensorMap* m) {
+  PFN_encodeTiled encode = encoder();
+  if (!encode || box < 1 || group > 128 || !aligned16(a->q)) return false;
+  // the stride of a dimension of one is free
+  long long st[3] = {a->heads == 1 ? c->head_dim : a->q_stride[2], 0, 0};
+  st[1] = a->tokens == 1 ? st[0] * a->heads : a->q_stride[1];
+  st[2] = c->batch == 1 ? st[1] * a->tokens : a->q_stride[0];
+  for (long long x : st)
+    if (x <= 0 || x % 8 || x * 2 >= 1ll << 40) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)a->heads, (cuuint64_t)a->tokens, (cuuint64_t)c->batch};
+  cuuint64_t strides[3] = {(cuuint64_t)st[0] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[2] * 2};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)group, (cuuint32_t)box, 1}, one[4] = {1, 1, 1, 1};
+  return encode(m, c->dtype == DD_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                const_cast<void*>(a->q), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Which kernel serves a call: the tensor cores take 16-bit caches with heads
 // of up to 128 values; pairs of query tiles from the second tile on.
 struct AttendPlan {
@@ -236,9 +256,9 @@ AttendPlan attend_plan(const dd_paged_cache* c, const dd_cache_attend_args* a) {
   return p;
 }
 template <typename T, int kDim, bool kPair>
-int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendParams& p, const DeviceInfo& dev,
+int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, AttendParams p, const DeviceInfo& dev,
                   void* stream) {
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq{};
   int rc = encode_pool(c, args->layer, 0, &mk);
   if (!rc) rc = encode_pool(c, args->layer, 1, &mv);
   if (rc) return rc;
@@ -247,6 +267,9 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, con
     DD_TRY(cudaFuncSetAttribute(attend_tc_kernel<T, kDim, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttSmem));
     ready[c->device] = true;
   }
+  p.tile_rows = p.group <= 128 ? 128 / p.group * p.group : 128;
+  p.item_rows = p.tile_rows * (kPair ? 2 : 1);
+  p.q_tma = encode_queries(c, args, p.group, (kPair ? 128 : 128 / p.copies) / p.group, &mq);
   const Scratch scratch = scratch_of(c);
   constexpr int kRows = AttendShape<kDim, kPair>::kRows;
   const int grid = std::min(dev.sms, kMaxAttendCtas);
@@ -254,7 +277,7 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, con
   w.count = scratch.count;
   w.o = scratch.partial;
   w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * kRows * kDim);
-  return launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(grid), dim3(kAttThreads), kAttSmem, stream, mk, mv, p, w);
+  return launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(grid), dim3(kAttThreads), kAttSmem, stream, mk, mv, mq, p, w);
 }
 template <typename T>
 int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendPlan& plan, const AttendParams& p,
