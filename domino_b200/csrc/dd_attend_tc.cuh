@@ -37,100 +37,14 @@
 // item that holds one is computed again key by key (attend_row_exact).
 #pragma once
 
-#include "dd_attend.cuh"
+#include "dd_attend_cut.cuh"
 
 namespace dd {
 
 constexpr int kAttThreads = 384;  // 8 softmax warps, key producer, MMA issuer, value producer, query loader
-constexpr int kKeyTile = 128;
+constexpr int kMaxTensorCtas = 160;
 constexpr int kMaxStages = 12;
 constexpr int kMergeCols = 16;  // of the two buffers of each stream's warps that join copies of rows
-
-struct AttendWork {
-  unsigned* count;  // [kMaxAttendCtas], zero between calls: finished pieces of the item that starts in a CTA and leaves it
-  float* o;         // [grid][2][rows][dim_pad]: the piece that comes from the CTA before, and the one that goes on in the next
-  float2* ml;       // [grid][2][rows]
-};
-constexpr int kMaxAttendCtas = 160;
-__host__ __device__ constexpr size_t attend_work_bytes(int dim_pad, bool pair) {
-  return (size_t)kMaxAttendCtas * 2 * (pair ? 256 : 128) * (sizeof(float) * dim_pad + sizeof(float2));
-}
-
-// Key tiles of one (row of the batch, query tile): n_sink from 0, then from
-// `first` on.  Positions are 32-bit here: a row holds at most 2^30 tokens.
-struct TileSpan {
-  int n_sink, first, n;
-  int rows;           // query rows of the batch row (tokens x group)
-  int start, lo, hi;  // position of token 0; keys that any row of the tile sees: [lo, hi) and, below hi, the sinks
-  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
-};
-__device__ __forceinline__ TileSpan tile_span(const AttendParams& a, int b, int qt, int tile_rows) {
-  TileSpan s;
-  const int n_new = a.lens ? (int)min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens;
-  s.start = (int)min(max(a.start[b], -(1ll << 30)), 1ll << 30);
-  s.rows = n_new * a.group;
-  s.n_sink = s.first = s.n = 0;
-  s.lo = s.hi = 0;
-  const int r0 = qt * tile_rows;
-  if (r0 >= s.rows) return s;
-  const int p0 = s.start + r0 / a.group, p1 = s.start + (min(s.rows, r0 + tile_rows) - 1) / a.group;
-  const int total = min(max(s.start + n_new, 0), a.row_pages << a.page_shift);
-  s.hi = max(a.causal ? min(total, p1 + 1) : total, 0);
-  if (s.hi == 0) return s;
-  s.lo = a.window > 0 ? max(p0 - a.window + 1, 0) : 0;
-  const int t_lo = s.lo / kKeyTile, t_hi = (s.hi + kKeyTile - 1) / kKeyTile;
-  const int sinks = min(min(a.sinks, s.lo), s.hi);
-  s.n_sink = min((sinks + kKeyTile - 1) / kKeyTile, t_lo);
-  s.first = t_lo;
-  s.n = s.n_sink + max(t_hi - t_lo, 0);
-  return s;
-}
-
-// A CTA's share of the work, item by item.  Many items: the CTAs take equal runs
-// of units, where an item counts its tiles and, before them, kItemUnits for the
-// start and the end of an item.  Few items (at most a quarter of the CTAs): each
-// gets CTAs of its own in proportion to its tiles, so that nobody has two.
-struct Piece {
-  int e, b, qt, h, i0, i1;  // entry (b, qt), key head, tiles [i0, i1) of it
-  int pos, left;            // unit of the item where the run enters it; units of the run from there on
-  TileSpan span;
-};
-constexpr int kItemUnits = 3;
-__device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
-  p.b = p.e / q_tiles;
-  p.qt = p.e - p.b * q_tiles;
-  p.span = tile_span(a, p.b, p.qt, tile_rows);
-}
-__device__ __forceinline__ bool piece_next(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
-  p.left -= p.span.n + kItemUnits - p.pos;
-  if (p.left <= kItemUnits) return false;  // the next item's first tile is another CTA's
-  if (++p.h == a.kv_heads) {
-    p.h = 0;
-    do {
-      ++p.e;
-      piece_enter(a, p, q_tiles, tile_rows);
-    } while (p.span.n == 0);
-  }
-  p.pos = p.i0 = 0;
-  p.i1 = min(p.span.n, p.left - kItemUnits);
-  return true;
-}
-// CTAs for an item of n tiles when there are few items.
-__device__ __forceinline__ int item_ctas(const AttendParams& a, int n, long long tiles, int spare) {
-  if (n == 0) return 0;
-  return max(min((int)((long long)n * spare / tiles), n / a.min_tiles), 1);
-}
-
-// Where CTA c's run starts: c / grid of all tiles.
-__device__ __forceinline__ long long run_start(long long total, unsigned c, unsigned grid) {
-  if (total < 1 << 23 && grid < 256) return (unsigned)total * c / grid;  // 32-bit division
-  return total * c / grid;
-}
-
-// The CTA that holds tile g.
-__device__ __forceinline__ int run_of(long long total, long long g, unsigned grid) {
-  return (int)(((g + 1) * grid - 1) / total);
-}
 
 // The ring of key and value tiles.  Tiles are loaded in the order in which the
 // tensor cores take them: with kPair K0 V0 K1 V1 .., without K0 K1 V0 K2 V1 K3
@@ -187,18 +101,6 @@ __device__ __forceinline__ int group_page(const AttendParams& a, int b, int tile
   return lane < 8 && slot < a.row_pages ? a.table[(long long)b * a.row_pages + slot] : -1;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
 // One arrival for a whole warp, after all of its lanes got here.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
@@ -258,81 +160,6 @@ __device__ __noinline__ void attend_row_exact(const AttendParams& a, const Piece
   *l_out = l;
 }
 
-// The pieces of one item, in slot 1 of CTA c0 and slot 0 of those behind it, by
-// 256 threads.  A warp takes four rows at a time: the lanes read the pieces'
-// (m, l) side by side, then the rows are added up piece by piece with sixteen
-// loads in flight (the reads come from L2 and one SM does them all).
-template <typename T, int kDim, int kRows>
-__device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork& work, const Piece& p, int c0, int c1,
-                                         int tid) {
-  constexpr int kVec = kDim / 32, kBatch = 4;  // values per lane, rows at a time
-  const int lane = tid & 31, r0 = p.qt * a.item_rows, last = min(a.item_rows, a.tokens * a.group - r0);
-  for (int row0 = tid >> 5; row0 < last; row0 += 8 * kBatch) {
-    float o[kBatch][kVec] = {}, m[kBatch], l[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.0f;
-    }
-    for (int c = c0; c <= c1; c += 32) {
-      const int mine = c + lane, pieces = min(32, c1 - c + 1);
-      float2 ml[kBatch];
-      float w[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int row = min(row0 + 8 * i, last - 1);
-        ml[i] = mine <= c1 ? __ldcg(&work.ml[(2 * (size_t)mine + (mine == c0)) * kRows + row]) : make_float2(-INFINITY, 0.0f);
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        float top = ml[i].x;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float m1 = fmaxf(m[i], top), base = m1 == -INFINITY ? 0.0f : m1;
-        const float keep = exp2_approx(m[i] - base);
-        w[i] = exp2_approx(ml[i].x - base);
-        float sum = ml[i].y * w[i];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        l[i] = l[i] * keep + sum;
-        m[i] = m1;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) o[i][v] *= keep;
-      }
-#pragma unroll 4
-      for (int k = 0; k < pieces; ++k) {
-        const float* part = work.o + (2 * (size_t)(c + k) + (c + k == c0)) * kRows * kDim + lane * kVec;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int row = min(row0 + 8 * i, last - 1);
-          const float wk = __shfl_sync(0xffffffffu, w[i], k);
-          float x[kVec];
-          if constexpr (kVec == 4)
-            *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(part + row * kDim));
-          else
-            *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(part + row * kDim));
-#pragma unroll
-          for (int v = 0; v < kVec; ++v) o[i][v] += x[v] * wk;
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int row = row0 + 8 * i, r = r0 + row, t = r / a.group, g = r - t * a.group;
-      if (row >= last || lane * kVec >= a.dim) continue;
-      const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-      const bool live = r < p.span.rows;  // the pieces of rows behind the chunk's end hold anything
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) o[i][v] = live ? o[i][v] * inv : 0.0f;
-      T* out = static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * a.group + g) * a.dim + lane * kVec;
-      if constexpr (kVec == 4)
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o[i][0], o[i][1]), pack2<T>(o[i][2], o[i][3]));
-      else
-        *reinterpret_cast<uint32_t*>(out) = pack2<T>(o[i][0], o[i][1]);
-    }
-  }
-}
-
 template <int kDim, bool kPair>
 struct AttendShape {
   static constexpr int kTiles = kPair ? 2 : 1;      // query tiles
@@ -349,19 +176,14 @@ struct AttendShape {
 struct AttendShared {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2], o_full[2], q_full, q_empty, wg[2], both;
-  Piece first;          // where the run starts; left = 0: the CTA has none
-  long long total, unit0;
   uint32_t tmem_base;
-  int abort_flag, few;
-  int join_c0, join_c1, join;  // CTAs that hold the split item; whether this CTA's piece finished last
+  int abort_flag;
+  CutShared cut;
   unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
   float row_norm[128];
   union {
     float2 row_ml[2][128];
-    struct {  // while the work is cut
-      long long warp_sum[kAttThreads / 32], warp_x[kAttThreads / 32];
-      int warp_y[kAttThreads / 32];
-    };
+    CutScan scan;  // while the work is cut
   };
 };
 // All of the 227 KB; the tiles start on a 1024-byte boundary, and there is
@@ -369,40 +191,6 @@ struct AttendShared {
 constexpr int kAttSmem = 227 * 1024;
 constexpr int kAttPad = kAttSmem - 224 * 1024 - (int)sizeof(AttendShared);
 static_assert(kAttPad >= 0, "tiles and AttendShared must fit 227 KB");
-
-// Over the block: `before` becomes the sum over the threads before this one and
-// `total` the sum over all; x and y become their sums over all.
-__device__ __forceinline__ void block_scan2(AttendShared& sh, long long& before, long long& total, long long& x, int& y,
-                                            int warp, int lane) {
-  long long inc = before;
-  const long long own = before;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += o;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    x += __shfl_xor_sync(0xffffffffu, x, d);
-    y += __shfl_xor_sync(0xffffffffu, y, d);
-  }
-  __syncthreads();
-  if (lane == 31) {
-    sh.warp_sum[warp] = inc;
-    sh.warp_x[warp] = x;
-    sh.warp_y[warp] = y;
-  }
-  __syncthreads();
-  before = inc - own;
-  total = x = y = 0;
-#pragma unroll
-  for (int w = 0; w < kAttThreads / 32; ++w) {
-    if (w < warp) before += sh.warp_sum[w];
-    total += sh.warp_sum[w];
-    x += sh.warp_x[w];
-    y += sh.warp_y[w];
-  }
-}
 
 template <typename T, int kDim, bool kPair>
 __global__ void __launch_bounds__(kAttThreads, 1)
@@ -451,99 +239,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   }
   pdl_wait_primary();
 
-  // the CTA's run of tiles
-  {
-    const int entries = a.batch * q_tiles, per = (entries + kAttThreads - 1) / kAttThreads;
-    const int e0 = tid * per, e1 = min(entries, e0 + per), grid = gridDim.x;
-    Piece mine;
-    // sums over the block: tiles and items of one key head
-    long long tiles = 0;
-    int items = 0;
-    for (mine.e = e0; mine.e < e1; ++mine.e) {
-      piece_enter(a, mine, q_tiles, a.item_rows);
-      tiles += mine.span.n;
-      items += mine.span.n > 0;
-    }
-    long long before = tiles + (long long)items * kItemUnits, total;  // units before this thread's entries, of all
-    const long long own = before;
-    block_scan2(bar, before, total, tiles, items, warp, lane);
-    before *= a.kv_heads;
-    total *= a.kv_heads;
-    const bool few = (long long)items * a.kv_heads * 4 <= grid;
-    int c0 = 0, c1 = 0;
-    bool found = false;
-    if (!few) {
-      const long long u0 = run_start(total, blockIdx.x, grid), u1 = run_start(total, blockIdx.x + 1, grid);
-      if (u0 < u1 && u0 >= before && u0 < before + own * a.kv_heads) {
-        // the run starts in this thread's entries (one entry as a rule: its span is still here)
-        long long rem = u0 - before;
-        int len = 0;
-        for (mine.e = e0; mine.e < e1; ++mine.e) {
-          if (per > 1) piece_enter(a, mine, q_tiles, a.item_rows);
-          len = mine.span.n ? mine.span.n + kItemUnits : 0;
-          if (rem < (long long)len * a.kv_heads) break;
-          rem -= (long long)len * a.kv_heads;
-        }
-        mine.h = (int)rem / len;  // rem < tiles x heads of one entry
-        mine.pos = (int)rem - mine.h * len;
-        mine.left = (int)(u1 - u0);
-        mine.i0 = max(mine.pos - kItemUnits, 0);
-        mine.i1 = min(mine.span.n, mine.pos + mine.left - kItemUnits);
-        if (mine.i1 <= mine.i0) mine.left = 0;
-        found = true;
-      }
-      if (tid == 0) {
-        bar.total = total;
-        bar.unit0 = u0;
-      }
-    } else {
-      const int spare = grid - items * a.kv_heads;
-      tiles *= a.kv_heads;
-      long long ctas = 0, all, unused0 = 0;
-      int unused1 = 0;
-      for (int e = e0; e < e1; ++e) {
-        if (per > 1) {
-          mine.e = e;
-          piece_enter(a, mine, q_tiles, a.item_rows);
-        }
-        ctas += item_ctas(a, mine.span.n, tiles, spare);
-      }
-      const long long mine_ctas = ctas;
-      block_scan2(bar, ctas, all, unused0, unused1, warp, lane);
-      if ((int)blockIdx.x >= ctas * a.kv_heads && (int)blockIdx.x < (ctas + mine_ctas) * a.kv_heads) {
-        int rem = blockIdx.x - (int)ctas * a.kv_heads, k = 1;
-        for (mine.e = e0; mine.e < e1; ++mine.e) {
-          if (per > 1) piece_enter(a, mine, q_tiles, a.item_rows);
-          k = item_ctas(a, mine.span.n, tiles, spare);
-          if (rem < k * a.kv_heads) break;
-          rem -= k * a.kv_heads;
-        }
-        mine.h = rem / k;
-        const int part = rem - mine.h * k;
-        mine.i0 = (int)((long long)mine.span.n * part / k);
-        mine.i1 = (int)((long long)mine.span.n * (part + 1) / k);
-        mine.pos = 0;
-        mine.left = 1;  // one piece only
-        c0 = blockIdx.x - part;
-        c1 = c0 + k - 1;
-        found = true;
-      }
-    }
-    if (tid == 0) bar.first.left = 0;
-    __syncthreads();
-    if (found) {
-      bar.first = mine;
-      bar.few = few;
-      bar.join_c0 = c0;
-      bar.join_c1 = c1;
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-  }
+  cut_work<kAttThreads>(a, bar.cut, bar.scan, q_tiles, tid);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   const uint32_t tmem = bar.tmem_base;
   volatile int* abort = &bar.abort_flag;
-  Piece p = bar.first;
+  Piece p = bar.cut.first;
   bool more = p.left > 0;
 
   if (warp == 8 || warp == 10) {
@@ -739,20 +441,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       fence_proxy_async_shared();
       warp_arrive(&bar.q_full, lane);
     }
-    // query tiles with nothing to see or behind the end of a short chunk: zeros
-    for (int e = blockIdx.x; e < a.batch * q_tiles; e += gridDim.x) {
-      const int b = e / q_tiles, qt = e - b * q_tiles;
-      if (tile_span(a, b, qt, a.item_rows).n) continue;
-      const int r1 = min((qt + 1) * a.item_rows, a.tokens * group);
-      for (int r = qt * a.item_rows; r < r1; ++r) {
-        const int t = r / group, g = r - t * group;
-        for (int i = lane; i < a.kv_heads * (a.dim / 8); i += 32) {
-          const int h = i / (a.dim / 8), d = (i - h * (a.dim / 8)) * 8;
-          T* out = static_cast<T*>(a.out) + (((long long)b * a.tokens + t) * a.heads + h * group + g) * a.dim + d;
-          *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
-        }
-      }
-    }
+    zero_blind_tiles<T>(a, q_tiles, lane, 32);
   } else {
     // ---------------------------------------------------------------- softmax, one thread per query row
     constexpr int kPartKeys = kKeyTile / Shape::kParts;
@@ -1082,22 +771,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         warp_arrive(&bar.both, lane);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
-        if (tid == 0) {
-          if (!bar.few) {
-            const long long g0 = bar.unit0 + (bar.first.left - p.left) - p.pos + kItemUnits;
-            bar.join_c0 = run_of(bar.total, g0, gridDim.x);
-            bar.join_c1 = run_of(bar.total, g0 + p.span.n - 1, gridDim.x);
-          }
-          const unsigned others = bar.join_c1 - bar.join_c0;
-          const unsigned done = atomicInc(&work.count[bar.join_c0], others);
-          __threadfence();
-          bar.join = done == others;
-        }
+        if (tid == 0) finish_piece(work, bar.cut, p);
         warp_arrive(&bar.both, lane);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
         const Piece here = p;
-        if (bar.join) join_pieces<T, kDim, Shape::kRows>(a, work, here, bar.join_c0, bar.join_c1, tid);
+        if (bar.cut.join) join_pieces<T, kDim, Shape::kRows, 8>(a, work, here, bar.cut.c0, bar.cut.c1, tid);
       }
       if (!kPair) {  // O, the maxima and the flags have been read; the next piece's first P waits for the other stream's
         tc_fence_before();

@@ -11,6 +11,7 @@
 
 #include "../../include/domino_draft.h"
 #include "dd_attend.cuh"
+#include "dd_attend_f32.cuh"
 #include "dd_attend_tc.cuh"
 #include "dd_cache_write.cuh"
 #include "dd_common.h"
@@ -117,8 +118,10 @@ Scratch scratch_of(const dd_paged_cache* c) {
   s.count = reinterpret_cast<unsigned*>(p);
   s.pages = p + counters;
   s.partial = reinterpret_cast<float*>(p + counters + lists);
+  const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
   s.bytes = counters + lists;
-  if (c->dtype != DD_F32 && c->head_dim <= 128) s.bytes += attend_work_bytes(c->head_dim <= 64 ? 64 : 128, true);
+  s.bytes += c->dtype != DD_F32 && c->head_dim <= 128 ? attend_work_bytes(kMaxTensorCtas, 256, dim)
+                                                      : attend_work_bytes(kMaxAttendCtas, kF32Rows, dim);
   return s;
 }
 
@@ -272,13 +275,33 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, Att
   p.q_tma = encode_queries(c, args, p.group, (kPair ? 128 : 128 / p.copies) / p.group, &mq);
   const Scratch scratch = scratch_of(c);
   constexpr int kRows = AttendShape<kDim, kPair>::kRows;
-  const int grid = std::min(dev.sms, kMaxAttendCtas);
+  const int grid = std::min(dev.sms, kMaxTensorCtas);
   AttendWork w;
   w.count = scratch.count;
   w.o = scratch.partial;
   w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * kRows * kDim);
   return launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(grid), dim3(kAttThreads), kAttSmem, stream, mk, mv, mq, p, w);
 }
+template <typename T, int kDim>
+int launch_attend_f32(const dd_paged_cache* c, AttendParams p, const DeviceInfo& dev, void* stream) {
+  constexpr int kSmem = F32Shape<kDim>::kSmem;
+  static bool ready[64];
+  if (!ready[c->device]) {
+    DD_TRY(cudaFuncSetAttribute(attend_f32_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    ready[c->device] = true;
+  }
+  p.item_rows = p.tile_rows = kF32Rows;
+  p.min_tiles = 1;
+  // two CTAs fit an SM with heads of up to 64 values
+  const int grid = std::min(dev.sms * (kDim <= 64 ? 2 : 1), kMaxAttendCtas);
+  const Scratch scratch = scratch_of(c);
+  AttendWork w;
+  w.count = scratch.count;
+  w.o = scratch.partial;
+  w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * kF32Rows * kDim);
+  return launch("attend", attend_f32_kernel<T, kDim>, dim3(grid), dim3(kF32Threads), kSmem, stream, p, w);
+}
+
 template <typename T>
 int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, const AttendPlan& plan, const AttendParams& p,
                   const DeviceInfo& dev, void* stream) {
@@ -302,7 +325,7 @@ int check_attend(const dd_paged_cache* c, const dd_cache_attend_args* a) {
     return global_fail(DD_EINVAL, "cache attend: a window needs causal attention, sinks need a window");
   if ((long long)a->tokens * (a->heads / c->kv_heads) > (1ll << 29) || (long long)a->heads * c->head_dim > 0x7fffffffll)
     return global_fail(DD_EINVAL, "cache attend: chunk too large");
-  // the kernel counts key tiles of one row and head, and of one SM's share, in 32 bits
+  // the kernels count key tiles of one row and head, and of one SM's share, in 32 bits
   const double tiles = ((double)c->row_pages * c->page_size / 128 + 2) * c->kv_heads;
   const double entries = (double)c->batch * ((double)a->tokens * (a->heads / c->kv_heads) / 128 + 1);
   if (tiles > 1e9 || entries > 1e9 || tiles * entries > 1e11) return global_fail(DD_EINVAL, "cache attend: chunk too large");
@@ -470,13 +493,12 @@ int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void
     if (c->dtype == DD_FP16) return launch_attend<__half>(c, a, plan, p, dev, stream);
     return launch_attend<__nv_bfloat16>(c, a, plan, p, dev, stream);
   }
-  const long long units = (long long)c->batch * a->tokens * a->heads;
-  const long long blocks = (units + kSimpleWarps - 1) / kSimpleWarps;
-  if (blocks > 0x7fffffffll) return global_fail(DD_EINVAL, "dd_cache_attend: chunk too large");
-  const dim3 grid((unsigned)blocks), block(32 * kSimpleWarps);
-  if (c->dtype == DD_F32) return launch("attend", attend_simple_kernel<float>, grid, block, 0, stream, p);
-  if (c->dtype == DD_FP16) return launch("attend", attend_simple_kernel<__half>, grid, block, 0, stream, p);
-  return launch("attend", attend_simple_kernel<__nv_bfloat16>, grid, block, 0, stream, p);
+  if (c->dtype == DD_F32)
+    return c->head_dim <= 64    ? launch_attend_f32<float, 64>(c, p, dev, stream)
+           : c->head_dim <= 128 ? launch_attend_f32<float, 128>(c, p, dev, stream)
+                                : launch_attend_f32<float, 256>(c, p, dev, stream);
+  if (c->dtype == DD_FP16) return launch_attend_f32<__half, 256>(c, p, dev, stream);
+  return launch_attend_f32<__nv_bfloat16, 256>(c, p, dev, stream);
 }
 
 }  // extern "C"
