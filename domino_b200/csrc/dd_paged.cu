@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstdio>
 #include <mutex>
 #include <type_traits>
@@ -169,8 +170,8 @@ int page_call(const dd_paged_cache* c, const void* arg, const char* what, const 
 template <typename T, int kGroup, bool kVec>
 int launch_write(const WriteParams& p, int batch, int tokens_per_cta, bool interleaved, void* stream) {
   const int half = p.rotary / 2;
-  const int pairs = interleaved ? 2 : half % 8 == 0 ? 0 : 1;
-  size_t smem = sizeof(float) * 2 * tokens_per_cta * half;
+  const int pairs = interleaved ? 2 : half % 4 == 0 ? 0 : 1;
+  size_t smem = sizeof(float) * 2 * tokens_per_cta * ((half + 3) / 4 * 4);
   if (pairs == 1) smem += sizeof(float) * (kWriteThreads / kGroup) * p.dim;
   const dim3 grid(ceil_div(p.tokens, tokens_per_cta), batch);
   auto kernel = pairs == 0   ? cache_write_kernel<T, kGroup, 0, kVec>
@@ -419,6 +420,8 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
       p.stride[i][k] = st[i][k];
       vec = vec && st[i][k] % per16 == 0;
     }
+    if (std::llabs(st[i][1]) > 0x7fffffffll || std::llabs(st[i][2]) > 0x7fffffffll)
+      return global_fail(DD_EINVAL, "dd_cache_write: token and head strides must stay below 2^31 elements");
   }
   const void* norm[2] = {a->q_norm, a->k_norm};
   for (int i = 0; i < 2; ++i) {
@@ -442,10 +445,11 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
   p.rotary = a->rotary;
   p.pages = c->pages;
   p.page_size = c->page_size;
+  while (1 << p.page_shift < c->page_size) ++p.page_shift;
   p.row_pages = c->row_pages;
   // One token a CTA until that fills the GPU several times over; then four, so
   // that all threads have an angle to compute.
-  const int per_cta = (long long)c->batch * a->tokens > 16ll * dev.sms ? 4 : 1;
+  const int per_cta = (long long)c->batch * a->tokens > 16ll * dev.sms ? kWriteTokens : 1;
   const bool il = a->interleaved != 0;
   if (c->dtype == DD_F32) return launch_write<float>(p, c->batch, per_cta, il, vec, stream);
   if (c->dtype == DD_FP16) return launch_write<__half>(p, c->batch, per_cta, il, vec, stream);
