@@ -82,14 +82,15 @@ class DDPagedCache(ctypes.Structure):
 
 class DDCacheWriteArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")]
-                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(f"{n}_stride{i}", ctypes.c_int64) for n in ("q", "k", "v") for i in range(3)]  # int64_t x[3] each
                 + [(n, ctypes.c_void_p) for n in ("start", "lens", "q_norm", "k_norm", "inv_freq")]
                 + [("eps", ctypes.c_float), ("factor", ctypes.c_float)]
                 + [(n, ctypes.c_int32) for n in ("layer", "tokens", "heads", "rotary", "interleaved")])
 
 
 class DDCacheAttendArgs(ctypes.Structure):
-    _fields_ = ([("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 3)]
+    _fields_ = ([("q", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(f"q_stride{i}", ctypes.c_int64) for i in range(3)]
                 + [(n, ctypes.c_void_p) for n in ("start", "lens")] + [("scale", ctypes.c_float)]
                 + [(n, ctypes.c_int32) for n in ("layer", "tokens", "heads", "causal", "window", "sinks")])
 

@@ -447,9 +447,10 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
   p.page_size = c->page_size;
   while (1 << p.page_shift < c->page_size) ++p.page_shift;
   p.row_pages = c->row_pages;
-  // One token a CTA until that fills the GPU several times over; then four, so
-  // that all threads have an angle to compute.
-  const int per_cta = (long long)c->batch * a->tokens > 16ll * dev.sms ? kWriteTokens : 1;
+  // One token a CTA while all of them are resident at once (four an SM); beyond
+  // that four tokens, whose rounds overlap (2331 tokens x 36 heads: 24 us with
+  // one, see dd_cache_write.cuh for large calls).
+  const int per_cta = (long long)c->batch * a->tokens > 4ll * dev.sms ? kWriteTokens : 1;
   const bool il = a->interleaved != 0;
   if (c->dtype == DD_F32) return launch_write<float>(p, c->batch, per_cta, il, vec, stream);
   if (c->dtype == DD_FP16) return launch_write<__half>(p, c->batch, per_cta, il, vec, stream);

@@ -29,6 +29,10 @@ __all__ = ["PagedKVCache", "Rope"]
 _DTYPES = {torch.bfloat16: _lib.DD_BF16, torch.float16: _lib.DD_FP16, torch.float32: _lib.DD_F32}
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class Rope:
     """Rotary positions of one kind of head.
 
@@ -160,7 +164,8 @@ class PagedKVCache:
 
     # ---------------------------------------------------------------- checks
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        """The current stream of the cache's device (the object that torch.cuda.current_stream makes costs 2 us)."""
+        return _raw_stream(self.device.index)
 
     def _check(self, rc: int, what: str) -> None:
         if rc < 0:
@@ -168,11 +173,11 @@ class PagedKVCache:
 
     def _rows(self, t: torch.Tensor, name: str) -> int:
         """An int64 [batch] tensor of the cache's device."""
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.long or t.dim() != 1 or t.shape[0] != self.batch:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.long or t.shape != self.length.shape:
             raise ValueError(f"{name} must be an int64 tensor [{self.batch}]")
         if t.device != self.device:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
-        if t.stride(0) != 1 and self.batch > 1:
+        if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         return t.data_ptr()
 
@@ -202,7 +207,6 @@ class PagedKVCache:
         return layer
 
     # ---------------------------------------------------------------- operators
-    @torch.no_grad()
     def write(self, layer: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rope: Optional[Rope],
               start: torch.Tensor, lens: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
               k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Optional[torch.Tensor]:
@@ -214,39 +218,37 @@ class PagedKVCache:
         ``k_norm`` [head_dim] where given, then turned by ``rope`` (None: not turned); the arithmetic is fp32 (angles
         fp64) with one rounding.  Rows of the result behind ``lens[b]`` are zero.  ``length`` does not change.
         """
-        a = _lib.DDCacheWriteArgs()
-        a.layer = self._layer(layer)
         k = self._heads(k, "k", None, self.kv_heads)
         tokens = k.shape[1]
         v = self._heads(v, "v", tokens, self.kv_heads)
+        a = _lib.DDCacheWriteArgs(layer=self._layer(layer), tokens=tokens, eps=eps)
         out = None
-        a.tokens, a.heads, a.q, a.q_out = tokens, 0, None, None
         if q is not None:
             q = self._heads(q, "q", tokens, None)
-            out = torch.empty(self.batch, tokens, q.shape[2], self.head_dim, dtype=self.dtype, device=self.device)
+            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
             a.heads, a.q, a.q_out = q.shape[2], q.data_ptr(), out.data_ptr()
-            a.q_stride[:] = q.stride()[:3]
+            a.q_stride0, a.q_stride1, a.q_stride2, _ = q.stride()
         a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.k_stride[:] = k.stride()[:3]
-        a.v_stride[:] = v.stride()[:3]
+        a.k_stride0, a.k_stride1, a.k_stride2, _ = k.stride()
+        a.v_stride0, a.v_stride1, a.v_stride2, _ = v.stride()
         a.start = self._rows(start, "start")
-        a.lens = None if lens is None else self._rows(lens, "lens")
-        q_norm, k_norm = self._norm(q_norm, "q_norm"), self._norm(k_norm, "k_norm")
-        a.q_norm = None if q_norm is None else q_norm.data_ptr()
-        a.k_norm = None if k_norm is None else k_norm.data_ptr()
-        a.eps = eps
-        if rope is None:
-            a.rotary, a.inv_freq, a.factor, a.interleaved = 0, None, 1.0, 0
-        else:
+        if lens is not None:
+            a.lens = self._rows(lens, "lens")
+        if q_norm is not None:
+            q_norm = self._norm(q_norm, "q_norm")
+            a.q_norm = q_norm.data_ptr()
+        if k_norm is not None:
+            k_norm = self._norm(k_norm, "k_norm")
+            a.k_norm = k_norm.data_ptr()
+        if rope is not None:
             if rope.head_dim != self.head_dim or rope.inv_freq.device != self.device:
                 raise ValueError(f"rope is for heads of {rope.head_dim} on {rope.inv_freq.device}, the cache has "
                                  f"{self.head_dim} on {self.device}")
             a.rotary, a.inv_freq, a.factor = rope.rotary_dim, rope.inv_freq.data_ptr(), rope.factor
-            a.interleaved = int(rope.interleaved)
+            a.interleaved = rope.interleaved
         self._check(self._lib.dd_cache_write(self._cp, ctypes.byref(a), self._stream()), "dd_cache_write")
         return out
 
-    @torch.no_grad()
     def attend(self, layer: int, q: torch.Tensor, start: torch.Tensor, lens: Optional[torch.Tensor] = None,
                causal: bool = True, window: int = 0, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
         """Attention of a chunk of new tokens over one layer of the cache -> [batch, tokens, heads, head_dim].
@@ -257,22 +259,20 @@ class PagedKVCache:
         ``p - j < window`` or ``j < sinks``.  ``scale`` defaults to ``head_dim ** -0.5``.  A query that sees no key
         gives zeros, as do the rows behind ``lens[b]``; what a query does not see has no effect on it.
         """
-        a = _lib.DDCacheAttendArgs()
-        a.layer = self._layer(layer)
         q = self._heads(q, "q", None, None)
-        tokens, heads = q.shape[1], q.shape[2]
+        _, tokens, heads, _ = q.shape
         if heads % self.kv_heads:
             raise ValueError(f"{heads} query heads for {self.kv_heads} key heads")
         if window < 0 or sinks < 0 or (sinks and not window) or (window and not causal):
             raise ValueError("a window needs causal attention, sinks need a window")
-        a.start = self._rows(start, "start")
-        a.lens = None if lens is None else self._rows(lens, "lens")
-        a.tokens, a.heads, a.causal, a.window, a.sinks = tokens, heads, int(bool(causal)), window, sinks
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
-        a.q = q.data_ptr()
-        a.q_stride[:] = q.stride()[:3]
-        out = torch.empty(self.batch, tokens, heads, self.head_dim, dtype=self.dtype, device=self.device)
-        a.out = out.data_ptr()
+        out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
+        a = _lib.DDCacheAttendArgs(layer=self._layer(layer), tokens=tokens, heads=heads, causal=bool(causal),
+                                   window=window, sinks=sinks, q=q.data_ptr(), out=out.data_ptr(),
+                                   start=self._rows(start, "start"),
+                                   scale=self.head_dim ** -0.5 if scale is None else scale)
+        a.q_stride0, a.q_stride1, a.q_stride2, _ = q.stride()
+        if lens is not None:
+            a.lens = self._rows(lens, "lens")
         self._check(self._lib.dd_cache_attend(self._cp, ctypes.byref(a), self._stream()), "dd_cache_attend")
         return out
 
