@@ -279,13 +279,13 @@ __device__ __forceinline__ void finish_piece(const AttendWork& work, CutShared& 
 }
 
 // The pieces of one item, in slot 1 of CTA c0 and slot 0 of those behind it, by
-// kWarps warps.  A warp takes four rows at a time: the lanes read the pieces'
-// (m, l) side by side, then the rows are added up piece by piece with sixteen
+// kWarps warps.  A warp takes two rows at a time: the lanes read the pieces'
+// (m, l) side by side, then the rows are added up piece by piece with eight
 // loads in flight (the reads come from L2 and one SM does them all).
 template <typename T, int kDim, int kRows, int kWarps>
 __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork& work, const Piece& p, int c0, int c1,
                                          int tid) {
-  constexpr int kVec = kDim / 32, kBatch = kDim > 128 ? 2 : 4;  // values per lane, rows at a time
+  constexpr int kVec = kDim / 32, kBatch = kDim > 128 ? 1 : 2;  // values per lane, rows at a time
   const int lane = tid & 31, r0 = p.qt * a.item_rows, last = min(a.item_rows, a.tokens * a.group - r0);
   for (int row0 = tid >> 5; row0 < last; row0 += kWarps * kBatch) {
     float o[kBatch][kVec] = {}, m[kBatch], l[kBatch];
@@ -319,24 +319,33 @@ __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork
 #pragma unroll
         for (int v = 0; v < kVec; ++v) o[i][v] *= keep;
       }
-#pragma unroll 4
-      for (int k = 0; k < pieces; ++k) {
-        const float* part = work.o + (2 * (size_t)(c + k) + (c + k == c0)) * kRows * kDim + lane * kVec;
+      // four pieces at a time; what is behind the last one is that one again, with weight zero
+      for (int k = 0; k < pieces; k += 4) {
+        alignas(16) float x[4][kBatch][kVec];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int row = min(row0 + kWarps * i, last - 1);
-          const float wk = __shfl_sync(0xffffffffu, w[i], k);
-          alignas(16) float x[kVec];
-          if constexpr (kVec == 2) {
-            *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(part + row * kDim));
-          } else {
+        for (int u = 0; u < 4; ++u) {
+          const int piece = c + min(k + u, pieces - 1);
+          const float* part = work.o + (2 * (size_t)piece + (piece == c0)) * kRows * kDim + lane * kVec;
 #pragma unroll
-            for (int v = 0; v < kVec; v += 4)
-              *reinterpret_cast<float4*>(x + v) = __ldcg(reinterpret_cast<const float4*>(part + row * kDim + v));
+          for (int i = 0; i < kBatch; ++i) {
+            const float* from = part + min(row0 + kWarps * i, last - 1) * kDim;
+            if constexpr (kVec == 2) {
+              *reinterpret_cast<float2*>(x[u][i]) = __ldcg(reinterpret_cast<const float2*>(from));
+            } else {
+#pragma unroll
+              for (int v = 0; v < kVec; v += 4)
+                *reinterpret_cast<float4*>(x[u][i] + v) = __ldcg(reinterpret_cast<const float4*>(from + v));
+            }
           }
-#pragma unroll
-          for (int v = 0; v < kVec; ++v) o[i][v] += x[v] * wk;
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const float wk = __shfl_sync(0xffffffffu, w[i], (k + u) & 31);
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) o[i][v] += x[u][i][v] * (k + u < pieces ? wk : 0.0f);
+          }
       }
     }
 #pragma unroll
