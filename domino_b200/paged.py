@@ -16,6 +16,7 @@ make streams wait for one another.  The reference keeps one contiguous cache per
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
 from typing import Optional
@@ -24,7 +25,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["PagedKVCache", "Rope"]
+__all__ = ["PagedKVCache", "Rope", "rope_frequencies"]
 
 _DTYPES = {torch.bfloat16: _lib.DD_BF16, torch.float16: _lib.DD_FP16, torch.float32: _lib.DD_F32}
 
@@ -67,7 +68,7 @@ class Rope:
         self.head_dim, self.rotary_dim, self.interleaved = int(head_dim), int(rotary_dim), bool(interleaved)
         scale = 1.0
         if inv_freq is None:
-            inv_freq, scale = _frequencies(theta, rotary_dim, scaling)
+            inv_freq, scale = rope_frequencies(theta, rotary_dim, scaling)
         self.factor = float(scale if factor is None else factor)
         self.inv_freq = inv_freq.detach().to(device=device, dtype=torch.float32).contiguous()
 
@@ -77,7 +78,7 @@ class Rope:
         return Rope(self.head_dim, interleaved=self.interleaved, inv_freq=self.inv_freq, factor=self.factor, device=device)
 
 
-def _frequencies(theta: float, dim: int, scaling: Optional[dict]):
+def rope_frequencies(theta: float, dim: int, scaling: Optional[dict]):
     """(inv_freq fp32 [dim / 2], factor) of the default frequencies, scaled for long contexts."""
     inv = 1.0 / (theta ** (torch.arange(0, dim, 2, dtype=torch.int64).float() / max(dim, 1)))
     kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
@@ -161,6 +162,17 @@ class PagedKVCache:
         c = self._c
         c.data, c.table, c.length, c.refs = (x.data_ptr() for x in (self.data, self.table, self.length, self.refs))
         c.scratch, c.status, c.device = self._scratch.data_ptr(), self._status.data_ptr(), device.index
+
+    def first_rows(self, n: int) -> "PagedKVCache":
+        """The first ``n`` rows as a cache of their own, with the same pages and state: for a call on them alone."""
+        if not 1 <= n <= self.batch:
+            raise ValueError(f"{n} rows of {self.batch}")
+        part = copy.copy(self)
+        part.batch, part.table, part.length = n, self.table[:n], self.length[:n]
+        part._c = _lib.DDPagedCache.from_buffer_copy(self._c)
+        part._c.batch = n
+        part._cp = ctypes.byref(part._c)
+        return part
 
     # ---------------------------------------------------------------- checks
     def _stream(self) -> int:

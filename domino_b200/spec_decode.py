@@ -60,11 +60,20 @@ def _events(on_gpu: bool = True):
     return torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
 
 
+def common_prefix(prompts: Sequence[torch.Tensor]) -> int:
+    """Tokens that all prompts begin with, leaving each at least one of its own."""
+    n = min(int(p.numel()) for p in prompts) - 1
+    for p in prompts[1:]:
+        differ = (p[:n].cpu() != prompts[0][:n].cpu()).nonzero()
+        n = int(differ[0, 0]) if differ.numel() else n
+    return n
+
+
 @torch.inference_mode()
 def spec_generate(draft: DFlashBackbone, target: TargetLM, runner, prompts: Sequence[torch.Tensor],
                   max_new_tokens: int = 2048, block_size: Optional[int] = None,
                   stop_token_ids: Optional[Sequence[int]] = None, time_blocks: bool = False,
-                  use_graphs: Optional[bool] = None) -> SpecResult:
+                  use_graphs: Optional[bool] = None, page_size: int = 0, share_prefix: bool = False) -> SpecResult:
     """Greedy speculative decoding of ``len(prompts)`` requests at once.
 
     ``runner`` is a ``DraftCorrectionGraphRunner`` built for this drafter and
@@ -79,6 +88,12 @@ def spec_generate(draft: DFlashBackbone, target: TargetLM, runner, prompts: Sequ
     and the verify half of the steady-state block are each captured once in a
     CUDA graph and replayed; the host reads one flag per block to stop.  With
     ``time_blocks`` both halves are timed with CUDA events around the replays.
+
+    ``page_size`` (16, 32, 64 or 128; 0: the padded ragged caches) keeps both
+    models' keys and values in paged caches, whose writes and attention run in
+    the library's kernels; pages behind the accepted tokens go back after every
+    block.  ``share_prefix`` (paged only) prefills the tokens that all prompts
+    begin with once and lets the rows share their pages.
     """
     cfg = draft.cfg
     dev = target.lm_head.weight.device
@@ -101,14 +116,25 @@ def spec_generate(draft: DFlashBackbone, target: TargetLM, runner, prompts: Sequ
         ids[b, : p.numel()] = p.to(dev)
         out[b, : p.numel()] = p.to(dev)
     rows = torch.arange(B, device=dev)
-    tcache = target.new_cache(B, cap)
-    dcache = draft.new_cache(B, cap)
+    if share_prefix and not page_size:
+        raise ValueError("share_prefix needs a paged cache (page_size)")
+    tcache = target.new_cache(B, cap, page_size) if page_size else target.new_cache(B, cap)
+    dcache = draft.new_cache(B, cap, page_size) if page_size else draft.new_cache(B, cap)
     layers = cfg.target_layer_ids
     max_blocks = int(max_new_tokens) + 2
 
     # prefill (dflash.py:362-383)
     valid = torch.arange(pmax, device=dev)[None] < plen[:, None]
-    logits, ctx0 = target(ids, tcache, valid, feature_layers=layers, logits_at=plen - 1)
+    common = common_prefix(prompts) if share_prefix else 0
+    if common:
+        _, shared = target(ids[:1, :common], tcache.first_rows(1), valid[:1, :common], feature_layers=layers,
+                           logits_at=torch.zeros(1, dtype=torch.long, device=dev))
+        tcache.fork(torch.zeros(B, dtype=torch.long, device=dev))
+        logits, rest = target(ids[:, common:], tcache, valid[:, common:], feature_layers=layers,
+                              logits_at=plen - 1 - common)
+        ctx0 = torch.cat([shared.expand(B, -1, -1), rest], dim=1)
+    else:
+        logits, ctx0 = target(ids, tcache, valid, feature_layers=layers, logits_at=plen - 1)
     out[rows, plen] = torch.argmax(logits, dim=-1)
 
     # block state, updated in place
@@ -149,7 +175,10 @@ def spec_generate(draft: DFlashBackbone, target: TargetLM, runner, prompts: Sequ
         write = live[:, None] & (j <= acc[:, None] + 1)
         out.scatter_(1, cols, torch.where(write, vals, out.gather(1, cols)))
         start.add_(n_acc)
-        tcache.length.copy_(start)
+        if page_size:
+            tcache.crop(start)
+        else:
+            tcache.length.copy_(start)
         ctx.copy_(feats)
         ctx_valid.copy_(j[:, : k_draft + 1] < n_acc[:, None])
         acc_log.index_copy_(0, blk, n_acc[None])

@@ -19,7 +19,10 @@ Numerics follow ``transformers`` 5.x Qwen3 (RMSNorm in fp32, rotary tables in
 fp32, eager attention with an fp32 softmax and a min-float mask), so that
 with the same weights the logits agree with the reference's to rounding.
 This is host-side glue (PyTorch ops); the draft step itself runs in
-libdomino_draft.so.
+libdomino_draft.so.  With a paged cache (``new_cache(..., page_size=)``) the
+query / key norms, the rotary positions, the cache writes and the attention
+run in its kernels too (``domino_b200.paged``), in fp32 with one rounding
+where the ops above round each step.
 """
 from __future__ import annotations
 
@@ -29,6 +32,8 @@ from typing import List, Optional, Sequence
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .paged import PagedKVCache, Rope, rope_frequencies
 
 
 @dataclass
@@ -52,14 +57,33 @@ class StackConfig:
     gru_hidden_dim: int = 0
     pure_draft_prefix_len: int = 0
     shift_label: bool = False  # draft all block_size positions instead of block_size - 1 (dflash.py:347-349)
+    # long contexts: scaled rotary frequencies (paged.Rope), and causal layers that see the last `sliding_window`
+    # positions and the first `sink_tokens` only (all layers, or those set in `window_layers`)
+    rope_scaling: Optional[dict] = None
+    sliding_window: int = 0
+    sink_tokens: int = 0
+    window_layers: Optional[List[bool]] = None
+
+    def window(self, layer: int) -> int:
+        """Sliding window of a layer's causal attention, 0 for none."""
+        return self.sliding_window if self.window_layers is None or self.window_layers[layer] else 0
 
     @classmethod
-    def from_hf(cls, cfg) -> "StackConfig":
+    def from_hf(cls, cfg, long_context: bool = False) -> "StackConfig":
+        """``long_context`` also takes over the config's rotary scaling and sliding-window layers (left out otherwise)."""
         rope = getattr(cfg, "rope_parameters", None) or {}
         theta = rope.get("rope_theta", getattr(cfg, "rope_theta", 1e6))
         head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         out = cls(cfg.vocab_size, cfg.hidden_size, cfg.intermediate_size, cfg.num_hidden_layers,
                   cfg.num_attention_heads, cfg.num_key_value_heads, head_dim, cfg.rms_norm_eps, float(theta))
+        if long_context:
+            if rope.get("rope_type", "default") != "default":
+                out.rope_scaling = {k: v for k, v in rope.items() if k != "rope_theta"}
+                out.rope_scaling.setdefault("original_max_position_embeddings", cfg.max_position_embeddings)
+            kinds = getattr(cfg, "layer_types", None) or []
+            if getattr(cfg, "sliding_window", None) and "sliding_attention" in kinds:
+                out.sliding_window = int(cfg.sliding_window)
+                out.window_layers = [k == "sliding_attention" for k in kinds]
         dc = getattr(cfg, "dflash_config", None)
         if dc:
             out.block_size = int(getattr(cfg, "block_size", 16))
@@ -103,14 +127,36 @@ def rope_tables(cfg: StackConfig, positions: torch.Tensor, dtype):
     The inverse frequencies are computed on the host, as ``transformers`` does,
     and moved to the device once."""
     d = cfg.head_dim
-    key = (d, cfg.rope_theta, positions.device)
-    inv = _INV_FREQ.get(key)
+    key = (d, cfg.rope_theta, repr(cfg.rope_scaling), positions.device)
+    inv, factor = _INV_FREQ.get(key, (None, 1.0))
     if inv is None:
-        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, d, 2, dtype=torch.int64).float() / d))
-        inv = _INV_FREQ.setdefault(key, inv.to(positions.device))
+        inv, factor = rope_frequencies(cfg.rope_theta, d, cfg.rope_scaling)
+        inv, factor = _INV_FREQ.setdefault(key, (inv.to(positions.device), factor))
     freqs = positions.float()[..., None] * inv[None, None, :]
     emb = torch.cat([freqs, freqs], dim=-1)
-    return emb.cos().to(dtype), emb.sin().to(dtype)
+    cos, sin = emb.cos(), emb.sin()
+    if factor != 1.0:
+        cos, sin = cos * factor, sin * factor
+    return cos.to(dtype), sin.to(dtype)
+
+
+_ROPES: dict = {}
+
+
+def cache_rope(cfg: StackConfig, device) -> Rope:
+    """The same rotary positions for ``PagedKVCache.write``, made once per device."""
+    key = (cfg.head_dim, cfg.rope_theta, repr(cfg.rope_scaling), device)
+    rope = _ROPES.get(key)
+    if rope is None:
+        rope = _ROPES.setdefault(key, Rope(cfg.head_dim, cfg.rope_theta, scaling=cfg.rope_scaling, device=device))
+    return rope
+
+
+def paged_cache(cfg: StackConfig, batch: int, capacity: int, page_size: int, dtype, device) -> PagedKVCache:
+    """A paged cache with pages for ``capacity`` tokens of every row, for the layers of ``cfg``."""
+    row_pages = -(-capacity // page_size)
+    return PagedKVCache(cfg.num_hidden_layers, batch, cfg.num_key_value_heads, batch * row_pages, cfg.head_dim, dtype,
+                        device, page_size=page_size, row_pages=row_pages)
 
 
 def apply_rope(x, cos, sin):
@@ -169,6 +215,10 @@ class Attention(nn.Module):
         self.q_norm = RMSNorm(d, cfg.rms_norm_eps)
         self.k_norm = RMSNorm(d, cfg.rms_norm_eps)
 
+    def split(self, x, proj):
+        """Projected heads as they come, [B, T, heads, D]."""
+        return proj(x).view(x.shape[0], x.shape[1], -1, self.cfg.head_dim)
+
     def heads(self, x, proj, norm):
         B, T, _ = x.shape
         y = proj(x).view(B, T, -1, self.cfg.head_dim)
@@ -212,8 +262,11 @@ class TargetLM(nn.Module):
         self.model = _Model(cfg)
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
 
-    def new_cache(self, batch: int, capacity: int) -> RaggedKVCache:
+    def new_cache(self, batch: int, capacity: int, page_size: int = 0):
+        """A ragged cache, or with ``page_size`` a ``PagedKVCache`` (on the GPU: its attention runs in the kernels)."""
         p = self.lm_head.weight
+        if page_size:
+            return paged_cache(self.cfg, batch, capacity, page_size, p.dtype, p.device)
         return RaggedKVCache(self.cfg.num_hidden_layers, batch, self.cfg.num_key_value_heads, capacity,
                              self.cfg.head_dim, p.dtype, p.device)
 
@@ -231,24 +284,40 @@ class TargetLM(nn.Module):
         cfg = self.cfg
         B, T = ids.shape
         start = cache.length.clone()
-        pos = start[:, None] + torch.arange(T, device=ids.device)[None]
-        slots = pos.clamp(max=cache.capacity - 1)
-        L = cache.capacity  # keys past a row's length are masked
-        key_pos = torch.arange(L, device=ids.device)
-        allowed = key_pos[None, None, :] <= pos[:, :, None]
-        allowed = allowed | ~valid[:, :, None]  # padded queries attend to everything (ignored)
+        n_new = valid.sum(1)
         x = self.model.embed_tokens(ids)
-        cos, sin = rope_tables(cfg, pos, x.dtype)
-        groups = cfg.num_attention_heads // cfg.num_key_value_heads
+        paged = isinstance(cache, PagedKVCache)
+        if paged:
+            rope = cache_rope(cfg, x.device)
+            cache.reserve(start + n_new)
+        else:
+            pos = start[:, None] + torch.arange(T, device=ids.device)[None]
+            slots = pos.clamp(max=cache.capacity - 1)
+            L = cache.capacity  # keys past a row's length are masked
+            key_pos = torch.arange(L, device=ids.device)
+            causal = key_pos[None, None, :] <= pos[:, :, None]
+            allowed = causal | ~valid[:, :, None]  # padded queries attend to everything (ignored)
+            if cfg.sliding_window:
+                near = (key_pos[None, None, :] > pos[:, :, None] - cfg.sliding_window) | (key_pos < cfg.sink_tokens)
+                allowed_near = (causal & near) | ~valid[:, :, None]
+            cos, sin = rope_tables(cfg, pos, x.dtype)
+            groups = cfg.num_attention_heads // cfg.num_key_value_heads
         feats = {}
         for li, layer in enumerate(self.model.layers):
             a = layer.self_attn
             hn = layer.input_layernorm(x)
-            q = apply_rope(a.heads(hn, a.q_proj, a.q_norm), cos, sin)
-            k = apply_rope(a.heads(hn, a.k_proj, a.k_norm), cos, sin)
-            v = a.heads(hn, a.v_proj, None)
-            cache.write(li, k, v, slots, valid)
-            o = _attend(q, cache.k[li][:, :, :L], cache.v[li][:, :, :L], allowed, groups, a.cfg.head_dim ** -0.5)
+            if paged:
+                q = cache.write(li, a.split(hn, a.q_proj), a.split(hn, a.k_proj), a.split(hn, a.v_proj), rope, start,
+                                n_new, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps)
+                w = cfg.window(li)
+                o = cache.attend(li, q, start, n_new, window=w, sinks=cfg.sink_tokens if w else 0).view(B, T, -1)
+            else:
+                q = apply_rope(a.heads(hn, a.q_proj, a.q_norm), cos, sin)
+                k = apply_rope(a.heads(hn, a.k_proj, a.k_norm), cos, sin)
+                v = a.heads(hn, a.v_proj, None)
+                cache.write(li, k, v, slots, valid)
+                o = _attend(q, cache.k[li][:, :, :L], cache.v[li][:, :, :L], allowed_near if cfg.window(li) else allowed,
+                            groups, a.cfg.head_dim ** -0.5)
             x = x + a.o_proj(o)
             x = x + layer.mlp(layer.post_attention_layernorm(x))
             if li in feature_layers and li != cfg.num_hidden_layers - 1:
@@ -257,7 +326,7 @@ class TargetLM(nn.Module):
         for li in feature_layers:
             if li == cfg.num_hidden_layers - 1:
                 feats[li] = x
-        cache.length.copy_(start + valid.sum(1))
+        cache.length.copy_(start + n_new)
         if logits_at is not None:
             x = x[torch.arange(B, device=ids.device), logits_at]
         logits = self.lm_head(x)
@@ -283,8 +352,11 @@ class DFlashBackbone(nn.Module):
         self.embed_proj = nn.Sequential(nn.Linear(H + cfg.gru_hidden_dim, cfg.emb_dim, bias=False), nn.SiLU(),
                                         nn.Linear(cfg.emb_dim, cfg.vocab_size, bias=False))
 
-    def new_cache(self, batch: int, capacity: int) -> RaggedKVCache:
+    def new_cache(self, batch: int, capacity: int, page_size: int = 0):
+        """A ragged cache, or with ``page_size`` a ``PagedKVCache`` (on the GPU: its attention runs in the kernels)."""
         p = self.fc.weight
+        if page_size:
+            return paged_cache(self.cfg, batch, capacity, page_size, p.dtype, p.device)
         return RaggedKVCache(self.cfg.num_hidden_layers, batch, self.cfg.num_key_value_heads, capacity,
                              self.cfg.head_dim, p.dtype, p.device)
 
@@ -306,10 +378,25 @@ class DFlashBackbone(nn.Module):
         dev = noise.device
         start = cache.length.clone()
         n_ctx = ctx_valid.sum(1)
-        ctx_pos = start[:, None] + torch.arange(C, device=dev)[None]
-        blk_pos = (start + n_ctx)[:, None] + torch.arange(T, device=dev)[None]
         ctx_h = self.hidden_norm(self.fc(ctx_features))
         x = noise
+        if isinstance(cache, PagedKVCache):
+            rope = cache_rope(cfg, x.device)
+            blk_start = start + n_ctx
+            cache.reserve(blk_start + T)
+            for li, layer in enumerate(self.layers):
+                a = layer.self_attn
+                hn = layer.input_layernorm(x)
+                cache.write(li, None, a.split(ctx_h, a.k_proj), a.split(ctx_h, a.v_proj), rope, start, n_ctx, None,
+                            a.k_norm.weight, a.k_norm.eps)
+                q = cache.write(li, a.split(hn, a.q_proj), a.split(hn, a.k_proj), a.split(hn, a.v_proj), rope, blk_start,
+                                None, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps)
+                x = x + a.o_proj(cache.attend(li, q, blk_start, causal=False).view(B, T, -1))
+                x = x + layer.mlp(layer.post_attention_layernorm(x))
+            cache.length.copy_(blk_start)
+            return self.norm(x)
+        ctx_pos = start[:, None] + torch.arange(C, device=dev)[None]
+        blk_pos = (start + n_ctx)[:, None] + torch.arange(T, device=dev)[None]
         cos_c, sin_c = rope_tables(cfg, ctx_pos, x.dtype)
         cos_b, sin_b = rope_tables(cfg, blk_pos, x.dtype)
         L = cache.capacity  # keys past a row's context + block are masked

@@ -125,3 +125,53 @@ def test_rope_frequencies_match_transformers(scaling):
         inv, factor = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu")
     assert torch.allclose(r.inv_freq.double(), inv.double(), rtol=8 * 2.0 ** -24, atol=0)
     assert abs(r.factor - factor) < 1e-6
+
+
+def _tiny(**kw):
+    from transformers import Qwen3Config
+    return Qwen3Config(vocab_size=97, hidden_size=32, intermediate_size=48, num_hidden_layers=3, num_attention_heads=4,
+                       num_key_value_heads=2, head_dim=16, max_position_embeddings=64, **kw)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(rope_parameters={"rope_theta": 1e4, "rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 16}),
+    dict(rope_parameters={"rope_theta": 1e4, "rope_type": "linear", "factor": 2.0}),
+    dict(use_sliding_window=True, sliding_window=5, max_window_layers=0),
+    dict(use_sliding_window=True, sliding_window=7, layer_types=["full_attention", "sliding_attention", "full_attention"])])
+def test_long_context_config_matches_transformers(kw):
+    """TargetLM with a config's scaled frequencies or sliding-window layers against transformers' Qwen3 (fp32 both: a
+    few operations of 2^-24 on values of order one)."""
+    from transformers import Qwen3ForCausalLM
+
+    from domino_b200.stack import StackConfig, TargetLM
+
+    torch.manual_seed(0)
+    cfg = _tiny(**kw)
+    cfg._attn_implementation = "eager"
+    hf = Qwen3ForCausalLM(cfg).eval()
+    c = StackConfig.from_hf(cfg, long_context=True)
+    assert (c.rope_scaling is not None) == ("rope_parameters" in kw) and (c.sliding_window > 0) == ("sliding_window" in kw)
+    plain = StackConfig.from_hf(cfg)
+    assert plain.rope_scaling is None and plain.sliding_window == 0
+    t = TargetLM(c).eval()
+    t.load_state_dict(hf.state_dict())
+    ids = torch.randint(0, 97, (1, 40))
+    with torch.no_grad():
+        ref = hf(ids).logits
+    cache = t.new_cache(1, 64)
+    got = torch.cat([t(part, cache, torch.ones_like(part, dtype=torch.bool))[0] for part in ids.split([25, 1, 14], dim=1)], 1)
+    assert torch.allclose(got, ref, atol=1e-5, rtol=1e-5)
+
+
+def test_paged_caches_need_a_gpu_and_a_page_size():
+    from domino_b200.spec_decode import common_prefix
+    from domino_b200.stack import StackConfig, TargetLM
+
+    t = TargetLM(StackConfig.from_hf(_tiny()))
+    with pytest.raises(RuntimeError):
+        t.new_cache(1, 64, page_size=16)
+    p = torch.arange(10)
+    assert common_prefix([p, p]) == 9
+    assert common_prefix([p]) == 9
+    assert common_prefix([p, torch.tensor([0, 1, 2, 9, 9])]) == 3
+    assert common_prefix([p, torch.tensor([1])]) == 0
