@@ -80,6 +80,8 @@ def parse_args():
     ap.add_argument("--prompt-len", type=int, default=512)
     ap.add_argument("--new-tokens", type=int, default=2048)
     ap.add_argument("--draft-layers", type=int, default=5)
+    ap.add_argument("--page-size", type=int, default=0,
+                    help="--spec-loop: paged caches with pages of this many tokens (0: the padded ragged caches)")
     ap.add_argument("--requests", type=int, default=2, help="--spec-loop: requests per GPU")
     return ap.parse_args()
 
@@ -797,14 +799,14 @@ def run_spec_loop(args):
     runner = DraftCorrectionGraphRunner(draft, target, B, S, H, G, V, P + 1, device, use_graph=False)
     g = torch.Generator().manual_seed(args.seed + 100 + rank)
     prompts = [torch.randint(0, V - 1, (args.prompt_len,), generator=g) for _ in range(B)]
-    spec_generate(draft, target, runner, prompts, 64)  # warm-up
+    spec_generate(draft, target, runner, prompts, 64, page_size=args.page_size)  # warm-up
     torch.cuda.synchronize()
     if world > 1:
         dist.barrier()
     clocks = ClockSampler(local)
     if rank == 0:
         clocks.start()
-    res = spec_generate(draft, target, runner, prompts, args.new_tokens, time_blocks=True)
+    res = spec_generate(draft, target, runner, prompts, args.new_tokens, time_blocks=True, page_size=args.page_size)
     clk = clocks.stop() if rank == 0 else None
     status = runner.status()
     drafted = res.blocks * B * S

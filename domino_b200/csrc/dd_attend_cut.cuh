@@ -22,7 +22,7 @@ constexpr int kKeyTile = 128;
 
 struct AttendWork {
   unsigned* count;  // [kMaxAttendCtas], zero between calls: finished pieces of the item that starts in a CTA and leaves it
-  float* o;         // [grid][2][rows][dim_pad]: the piece that comes from the CTA before, and the one that goes on in the next
+  float* o;         // [grid][2][rows][dim_pad]: a piece from the CTA before, and one that goes on in the next
   float2* ml;       // [grid][2][rows]
 };
 constexpr int kMaxAttendCtas = 320;

@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
         float* part = work.o + (slot * kF32Rows + row) * kDim;
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
-          *reinterpret_cast<float4*>(part + 4 * tx + 64 * c) = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
+          *reinterpret_cast<float4*>(part + 4 * tx + 64 * c) =
+              make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
         if (tx == 0) work.ml[slot * kF32Rows + row] = make_float2(m[i], l[i]);
       } else {
         const int t = r / group, g = r - t * group;

@@ -285,8 +285,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA issuer
     // The whole warp walks the schedule and one elected lane issues: descriptors
-    // then stay in uniform registers (issued from inside a lane's own branch,
-    // each MMA cost about 100 cycles and the issue bound the kernel).
+    // then stay in uniform registers (issued from inside a lane's own branch, the
+    // 16 MMAs of a tile took 1500 cycles, of which the tensor cores need 1024;
+    // like this 1130).
     constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr int kPartKeys = kKeyTile / Shape::kParts;
     constexpr uint32_t idesc_s = idesc_f16(kPartKeys, fmt), idesc_o = idesc_f16(kDim, fmt) | kIdescBMnMajor;
@@ -410,8 +411,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
           for (int i = 0; i < Shape::kTiles * copies; ++i)
 #pragma unroll
             for (int hf = 0; hf < Shape::kHalves; ++hf)
-              tma_load_4d(sm_q + (kPair ? i * Shape::kTileBytes : i * copy_rows * 128) + hf * 128 * 128, &map_q, &bar.q_full,
-                          hf * 64, p.h * group, r0 / group + (kPair ? i * box : 0), p.b);
+              tma_load_4d(sm_q + (kPair ? i * Shape::kTileBytes : i * copy_rows * 128) + hf * 128 * 128, &map_q,
+                          &bar.q_full, hf * 64, p.h * group, r0 / group + (kPair ? i * box : 0), p.b);
         }
         __syncwarp();
         continue;
@@ -424,7 +425,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         for (; row < rows; row += kRowStep) {
           const T* src = q + t * a.q_stride[1] + g * a.q_stride[2];
           for (int to = row; to < 128; to += live_rows) {
-            unsigned char* dst = sm_q + tile * Shape::kTileBytes + (ch / 8) * 128 * 128 + to * 128 + ((ch % 8) ^ (to % 8)) * 16;
+            unsigned char* dst =
+                sm_q + tile * Shape::kTileBytes + (ch / 8) * 128 * 128 + to * 128 + ((ch % 8) ^ (to % 8)) * 16;
             if (vec) {
               cp_async16(dst, in ? src : a.q, in ? 16 : 0);
             } else {
@@ -493,130 +495,130 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         if (i + kStep < n) page = group_page(a, p.b, p.span.tile(p.i0 + i + kStep), lane);
 #pragma unroll 1
         for (int part = 0; part < Shape::kParts; ++part, ++n_part) {
-        const int key0 = tile * kKeyTile, part0 = key0 + part * kPartKeys, part1 = part0 + kPartKeys;
-        const bool whole = missing == 0 && part1 <= all_hi && (part0 >= all_lo || part1 <= a.sinks);
-        ok = mbar_wait_bounded(&bar.s_full[s][part], n_s & 1, abort);
-        if (!ok) break;
-        if (part + 1 == Shape::kParts) ++n_s;
-        tc_fence_after();
-        const int chunk_a = kPair ? part * (kPartKeys / 32) : chunk0, chunk_b = kPair ? chunk_a + kPartKeys / 32 : chunk1;
-        if (warp_live) {
-          // bit k: the row sees key 32 c + k of the tile
-          auto see = [&](int c) {
-            const int k0 = key0 + 32 * c;
-            const uint32_t gap = (missing >> (2 * c) & 1) * 0xffffu | (missing >> (2 * c + 1) & 1) * 0xffff0000u;
-            return low_bits(hi - k0) & (~low_bits(lo - k0) | low_bits(a.sinks - k0)) & ~gap;
-          };
-          // kCols x 32 scores in registers at a time; where that is not all of
-          // the thread's, they are read again for the exponentials.
-          uint32_t x[32 * kCols];
-          auto fetch = [&](int c) {
-#pragma unroll
-            for (int d = 0; d < kCols; ++d) tmem_ld32(t_s + 32 * (c + d), x + 32 * d);
-            tmem_ld_wait();
-            if (!whole)
-#pragma unroll
-              for (int d = 0; d < kCols; ++d) mask32(x + 32 * d, see(c + d));
-          };
-          float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c = chunk_a; c < chunk_b; c += kCols) {
-            fetch(c);
-#pragma unroll
-            for (int k = 0; k < 32 * kCols; k += 4) {
-              top[0] = max3_nan(top[0], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-              top[1] = max3_nan(top[1], __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
-            }
-          }
-          const float mt = max3_nan(top[0], top[1], top[1]);
-          if (!(mt < INFINITY)) l = __int_as_float(0x7fc00000);  // a NaN or +infinity among the scores: the row is NaN
-          const bool moves = (mt - m) * sl > 8.0f;
-          if (__any_sync(0xffffffffu, moves)) {
-            const float m1 = moves ? mt : m;
-            const float keep = moves ? exp2_approx((m - m1) * sl) : 1.0f;
-            l *= keep;
-            m = m1;
-            if (have_o) {
-              // (the scores of part k come after the products of part k - 2; those of k - 1 may still run)
-              if (Shape::kParts > 1) ok = mbar_wait_bounded(&bar.pv_done[s], (n_part - 1) & 1, abort);
-              if (Shape::kParts > 1) tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < kDim; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(t_o + s * kDim + c, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                tmem_st32(t_o + s * kDim + c, o);
-              }
-            }
-          }
-          have_o = true;
-          const float sub = m == -INFINITY ? 0.0f : m * sl;
-          uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
-          const uint64_t sl2 = pack_f32x2(sl, sl), sub2 = pack_f32x2(-sub, -sub);
-#pragma unroll 1
-          for (int c = chunk_a; c < chunk_b; c += kCols) {
-            if (chunk_b - chunk_a > kCols) fetch(c);
-#pragma unroll
-            for (int d = 0; d < kCols; ++d) {
-              uint32_t w[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const uint64_t e = fma_f32x2(pack_f32x2(__uint_as_float(x[32 * d + 2 * k]), __uint_as_float(x[32 * d + 2 * k + 1])),
-                                             sl2, sub2);
-                float e0, e1;
-                unpack_f32x2(e, e0, e1);
-                const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
-                sum[k & 3] = add_f32x2(sum[k & 3], pack_f32x2(p0, p1));
-                w[k] = pack2<T>(p0, p1);
-              }
-              // over scores that have been read, a part's weights within its own columns
-              tmem_st16(t_s + (kPair ? part * kPartKeys + 16 * (c + d - chunk_a) : 16 * (c + d)), w);
-            }
-          }
-          float sum0, sum1;
-          unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), sum0, sum1);
-          l += sum0 + sum1;
-          if (!kPair && copies > 1) {  // the other copies' keys
-            const uint32_t zero[16] = {};
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c)
-              if (c < chunk0 || c >= chunk1) tmem_st16(t_s + 16 * c, zero);
-          }
-          tmem_st_wait();
-        }
-        if (!whole) {
-          const int c = (base + load_index_v<kPair>(i, n)) % (2 * Shape::kStages);
-          const int st = c % Shape::kStages;
-          ok = mbar_wait_bounded(&bar.full[st], c / Shape::kStages, abort);
+          const int key0 = tile * kKeyTile, part0 = key0 + part * kPartKeys, part1 = part0 + kPartKeys;
+          const bool whole = missing == 0 && part1 <= all_hi && (part0 >= all_lo || part1 <= a.sinks);
+          ok = mbar_wait_bounded(&bar.s_full[s][part], n_s & 1, abort);
           if (!ok) break;
-          // keys that no row of the item sees become zero; those that only some see are searched.
-          // Eight lanes a 128-byte row, four rows a step.
-          unsigned char* v = sm_ring + st * Shape::kTileBytes + (lane % 8) * 16;
-          bool odd = false, wrote = false;
-#pragma unroll 1
-          for (int k = part * kPartKeys + (warp & 3) * (kPartKeys / 4) + lane / 8, k1 = k + kPartKeys / 4; k < k1; k += 4) {
-            const int j = key0 + k;
-            const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (k / 16) & 1);
-            const bool search = seen && (j >= all_hi || (j < all_lo && j >= a.sinks));
+          if (part + 1 == Shape::kParts) ++n_s;
+          tc_fence_after();
+          const int chunk_a = kPair ? part * (kPartKeys / 32) : chunk0, chunk_b = kPair ? chunk_a + kPartKeys / 32 : chunk1;
+          if (warp_live) {
+            // bit k: the row sees key 32 c + k of the tile
+            auto see = [&](int c) {
+              const int k0 = key0 + 32 * c;
+              const uint32_t gap = (missing >> (2 * c) & 1) * 0xffffu | (missing >> (2 * c + 1) & 1) * 0xffff0000u;
+              return low_bits(hi - k0) & (~low_bits(lo - k0) | low_bits(a.sinks - k0)) & ~gap;
+            };
+            // kCols x 32 scores in registers at a time; where that is not all of
+            // the thread's, they are read again for the exponentials.
+            uint32_t x[32 * kCols];
+            auto fetch = [&](int c) {
 #pragma unroll
-            for (int hf = 0; hf < Shape::kHalves; ++hf) {
-              uint4* at = reinterpret_cast<uint4*>(v + hf * 128 * 128 + k * 128);
-              if (!seen) {
-                *at = make_uint4(0, 0, 0, 0);
-                wrote = true;
-              } else if (search) {
-                const uint4 w = *at;
-                odd = odd || non_finite2<T>(w.x) || non_finite2<T>(w.y) || non_finite2<T>(w.z) || non_finite2<T>(w.w);
+              for (int d = 0; d < kCols; ++d) tmem_ld32(t_s + 32 * (c + d), x + 32 * d);
+              tmem_ld_wait();
+              if (!whole)
+#pragma unroll
+                for (int d = 0; d < kCols; ++d) mask32(x + 32 * d, see(c + d));
+            };
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = chunk_a; c < chunk_b; c += kCols) {
+              fetch(c);
+#pragma unroll
+              for (int k = 0; k < 32 * kCols; k += 4) {
+                top[0] = max3_nan(top[0], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                top[1] = max3_nan(top[1], __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
               }
             }
+            const float mt = max3_nan(top[0], top[1], top[1]);
+            if (!(mt < INFINITY)) l = __int_as_float(0x7fc00000);  // a NaN or +infinity among the scores: the row is NaN
+            const bool moves = (mt - m) * sl > 8.0f;
+            if (__any_sync(0xffffffffu, moves)) {
+              const float m1 = moves ? mt : m;
+              const float keep = moves ? exp2_approx((m - m1) * sl) : 1.0f;
+              l *= keep;
+              m = m1;
+              if (have_o) {
+                // (the scores of part k come after the products of part k - 2; those of k - 1 may still run)
+                if (Shape::kParts > 1) ok = mbar_wait_bounded(&bar.pv_done[s], (n_part - 1) & 1, abort);
+                if (Shape::kParts > 1) tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < kDim; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld32(t_o + s * kDim + c, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                  tmem_st32(t_o + s * kDim + c, o);
+                }
+              }
+            }
+            have_o = true;
+            const float sub = m == -INFINITY ? 0.0f : m * sl;
+            uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
+            const uint64_t sl2 = pack_f32x2(sl, sl), sub2 = pack_f32x2(-sub, -sub);
+#pragma unroll 1
+            for (int c = chunk_a; c < chunk_b; c += kCols) {
+              if (chunk_b - chunk_a > kCols) fetch(c);
+#pragma unroll
+              for (int d = 0; d < kCols; ++d) {
+                uint32_t w[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const float x0 = __uint_as_float(x[32 * d + 2 * k]), x1 = __uint_as_float(x[32 * d + 2 * k + 1]);
+                  const uint64_t e = fma_f32x2(pack_f32x2(x0, x1), sl2, sub2);
+                  float e0, e1;
+                  unpack_f32x2(e, e0, e1);
+                  const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
+                  sum[k & 3] = add_f32x2(sum[k & 3], pack_f32x2(p0, p1));
+                  w[k] = pack2<T>(p0, p1);
+                }
+                // over scores that have been read, a part's weights within its own columns
+                tmem_st16(t_s + (kPair ? part * kPartKeys + 16 * (c + d - chunk_a) : 16 * (c + d)), w);
+              }
+            }
+            float sum0, sum1;
+            unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), sum0, sum1);
+            l += sum0 + sum1;
+            if (!kPair && copies > 1) {  // the other copies' keys
+              const uint32_t zero[16] = {};
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c)
+                if (c < chunk0 || c >= chunk1) tmem_st16(t_s + 16 * c, zero);
+            }
+            tmem_st_wait();
           }
-          if (wrote) fence_proxy_async_shared();
-          if (odd) bar.redo[s] = n_pieces;
-        }
-        tc_fence_before();
-        warp_arrive(&bar.p_full[s][part], lane);
+          if (!whole) {
+            const int c = (base + load_index_v<kPair>(i, n)) % (2 * Shape::kStages);
+            const int st = c % Shape::kStages;
+            ok = mbar_wait_bounded(&bar.full[st], c / Shape::kStages, abort);
+            if (!ok) break;
+            // keys that no row of the item sees become zero; those that only some see are searched.
+            // Eight lanes a 128-byte row, four rows a step.
+            unsigned char* v = sm_ring + st * Shape::kTileBytes + (lane % 8) * 16;
+            bool odd = false, wrote = false;
+#pragma unroll 1
+            for (int k = part * kPartKeys + (warp & 3) * (kPartKeys / 4) + lane / 8, k1 = k + kPartKeys / 4; k < k1; k += 4) {
+              const int j = key0 + k;
+              const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (k / 16) & 1);
+              const bool search = seen && (j >= all_hi || (j < all_lo && j >= a.sinks));
+#pragma unroll
+              for (int hf = 0; hf < Shape::kHalves; ++hf) {
+                uint4* at = reinterpret_cast<uint4*>(v + hf * 128 * 128 + k * 128);
+                if (!seen) {
+                  *at = make_uint4(0, 0, 0, 0);
+                  wrote = true;
+                } else if (search) {
+                  const uint4 w = *at;
+                  odd = odd || non_finite2<T>(w.x) || non_finite2<T>(w.y) || non_finite2<T>(w.z) || non_finite2<T>(w.w);
+                }
+              }
+            }
+            if (wrote) fence_proxy_async_shared();
+            if (odd) bar.redo[s] = n_pieces;
+          }
+          tc_fence_before();
+          warp_arrive(&bar.p_full[s][part], lane);
         }
       }
       if (!ok) break;
@@ -755,8 +757,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               *reinterpret_cast<float4*>(part + (size_t)k * kDim + col) = o;
             } else if (col < a.dim) {
               const float norm = bar.row_norm[k];
-              *reinterpret_cast<uint2*>(out_row(k) + col) =
-                  norm == 0.0f ? make_uint2(0, 0) : make_uint2(pack2<T>(o.x * norm, o.y * norm), pack2<T>(o.z * norm, o.w * norm));
+              const uint2 w = make_uint2(pack2<T>(o.x * norm, o.y * norm), pack2<T>(o.z * norm, o.w * norm));
+              *reinterpret_cast<uint2*>(out_row(k) + col) = norm == 0.0f ? make_uint2(0, 0) : w;
             }
           }
           // the other buffer next: the wait in between keeps the two apart
