@@ -178,9 +178,64 @@ __device__ __forceinline__ void block_scan2(CutScan& sh, long long& before, long
 template <int kThreads>
 __device__ __forceinline__ void cut_work(const AttendParams& a, CutShared& sh, CutScan& scan, int q_tiles, int tid) {
   const int warp = tid >> 5, lane = tid & 31;
-  const int entries = a.batch * q_tiles, per = (entries + kThreads - 1) / kThreads;
-  const int e0 = tid * per, e1 = min(entries, e0 + per), grid = gridDim.x;
+  const int entries = a.batch * q_tiles, per = (entries + kThreads - 1) / kThreads, grid = gridDim.x;
   Piece mine;
+  if (entries <= 32) {
+    // One warp, a lane per entry (the general way below costs a small call 3000
+    // cycles, this one 1500, most of it the lengths' way from memory).
+    if (warp > 0) return;
+    mine.e = lane;
+    int n = 0;
+    if (lane < entries) {
+      piece_enter(a, mine, q_tiles, a.item_rows);
+      n = mine.span.n;
+    }
+    const int items = __popc(__ballot_sync(0xffffffffu, n > 0));
+    const int tiles = __reduce_add_sync(0xffffffffu, n);
+    const bool few = (long long)items * a.kv_heads * 4 <= grid;
+    // units, or CTAs, for one key head of the entry
+    const int own = few ? item_ctas(a, n, (long long)tiles * a.kv_heads, grid - items * a.kv_heads) : n ? n + kItemUnits : 0;
+    int inc = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    const long long before = (long long)(inc - own) * a.kv_heads;
+    const long long total = (long long)__shfl_sync(0xffffffffu, inc, 31) * a.kv_heads;
+    const long long u0 = few ? blockIdx.x : run_start(total, blockIdx.x, grid);
+    const long long u1 = few ? u0 + 1 : run_start(total, blockIdx.x + 1, grid);
+    const bool found = u0 < u1 && u0 >= before && u0 < before + (long long)own * a.kv_heads;
+    if (lane == 0) {
+      sh.few = few;
+      sh.total = total;
+      sh.unit0 = u0;
+      sh.first.left = 0;
+    }
+    __syncwarp();
+    if (found) {
+      const int rem = (int)(u0 - before);
+      mine.h = rem / own;
+      const int part = rem - mine.h * own;
+      if (few) {
+        mine.i0 = (int)((long long)n * part / own);
+        mine.i1 = (int)((long long)n * (part + 1) / own);
+        mine.pos = 0;
+        mine.left = 1;  // one piece only
+        sh.c0 = blockIdx.x - part;
+        sh.c1 = sh.c0 + own - 1;
+      } else {
+        mine.pos = part;
+        mine.left = (int)(u1 - u0);
+        mine.i0 = max(mine.pos - kItemUnits, 0);
+        mine.i1 = min(n, mine.pos + mine.left - kItemUnits);
+        if (mine.i1 <= mine.i0) mine.left = 0;
+      }
+      sh.first = mine;
+    }
+    return;
+  }
+  const int e0 = tid * per, e1 = min(entries, e0 + per);
   // sums over the block: tiles and items of one key head
   long long tiles = 0;
   int items = 0;
@@ -194,7 +249,7 @@ __device__ __forceinline__ void cut_work(const AttendParams& a, CutShared& sh, C
   block_scan2<kThreads>(scan, before, total, tiles, items, warp, lane);
   before *= a.kv_heads;
   total *= a.kv_heads;
-  const bool few = (long long)items * a.kv_heads * 4 <= grid;
+  const bool few = (long long)items * a.kv_heads * 4 <= grid;  // (with many entries behind the end of their chunks)
   int c0 = 0, c1 = 0;
   bool found = false;
   if (!few) {

@@ -633,6 +633,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         const int t = r / group, g = r - t * group;
         return static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * group + g) * a.dim;
       };
+      T* const out0 = out_row(kPair ? r : row / 4);  // (the divisions run while the last products do)
       bool again;
       float f0 = 1.0f, f1 = 0.0f;  // weights of the streams' sums (kPair: only its own)
       if (m != -INFINITY) m *= sl;
@@ -688,7 +689,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       } else if (kPair) {
         if (split && in_tile < a.tile_rows) part_ml[slot_row] = make_float2(m, l);
         const float norm = split ? 1.0f : inv;
-        T* out = out_row(r);
 #pragma unroll 1
         for (int c = 0; c < kDim; c += 32) {
           uint32_t x[32];
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; k += 8)
               if (c + k < a.dim)
-                *reinterpret_cast<uint4*>(out + c + k) =
+                *reinterpret_cast<uint4*>(out0 + c + k) =
                     make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),
                                pack2<T>(o[k + 6], o[k + 7]));
           }
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             } else if (col < a.dim) {
               const float norm = bar.row_norm[k];
               const uint2 w = make_uint2(pack2<T>(o.x * norm, o.y * norm), pack2<T>(o.z * norm, o.w * norm));
-              *reinterpret_cast<uint2*>(out_row(k) + col) = norm == 0.0f ? make_uint2(0, 0) : w;
+              *reinterpret_cast<uint2*>((k == row / 4 ? out0 : out_row(k)) + col) = norm == 0.0f ? make_uint2(0, 0) : w;
             }
           }
           // the other buffer next: the wait in between keeps the two apart
