@@ -69,7 +69,10 @@ struct Piece {
   int pos, left;            // unit of the item where the run enters it; units of the run from there on
   TileSpan span;
 };
-constexpr int kItemUnits = 3;
+// (Start and end cost about as much as seven tiles: with 3 / 5 / 7 / 10 the calls
+// of 64 rows x 1 token took 210 / 198 / 198 / 199 us, of 32 rows x 16 tokens 265
+// / 262 / 254 / 253 us; with none, short rows' CTAs ran twice as long as others.)
+constexpr int kItemUnits = 7;
 __device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
   p.b = p.e / q_tiles;
   p.qt = p.e - p.b * q_tiles;
