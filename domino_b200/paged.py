@@ -12,7 +12,8 @@ behind ``dd_pages_*`` and ``dd_cache_*`` of include/domino_draft.h:
 
 Everything runs on the current stream of the cache's device without host synchronisation and can be captured in a CUDA
 graph (lengths, positions and tables are read on the device).  Calls on one cache must be ordered: use one stream, or
-make streams wait for one another.  The reference keeps one contiguous cache per sequence (code/dflash.py:359-360, 488).
+make streams wait for one another.  There is no backward pass.  The reference keeps one contiguous cache per sequence
+(code/dflash.py:359-360, 488).
 """
 from __future__ import annotations
 
@@ -279,7 +280,7 @@ class PagedKVCache:
             raise ValueError("a window needs causal attention, sinks need a window")
         out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
         a = _lib.DDCacheAttendArgs(layer=self._layer(layer), tokens=tokens, heads=heads, causal=bool(causal),
-                                   window=window, sinks=sinks, q=q.data_ptr(), out=out.data_ptr(),
+                                   window=min(window, 1 << 30), sinks=min(sinks, 1 << 30), q=q.data_ptr(), out=out.data_ptr(),
                                    start=self._rows(start, "start"),
                                    scale=self.head_dim ** -0.5 if scale is None else scale)
         a.q_stride0, a.q_stride1, a.q_stride2, _ = q.stride()

@@ -501,3 +501,132 @@ def test_captured_calls_replay_on_new_lengths():
         assert torch.equal(captured, eager), i
         assert torch.equal(caches[0].table, caches[1].table) and torch.equal(caches[0].length, caches[1].length)
     assert caches[0].status() == 0 and caches[1].status() == 0
+
+
+@pytest.mark.parametrize("case", [
+    (200, 1, 64, 32, 2, [70, 5], [2, 1]),                # more query heads per key head than a tile has rows
+    (256, 2, 128, 16, 1, [300], [1]),
+    (6, 2, 72, 128, 20, [250, 0], [20, 20]),             # pages of a whole key tile; 72 and 104 values
+    (22, 2, 104, 128, 40, [129], [40]),
+])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attend_odd_head_layouts(case, dtype):
+    heads, kv, dim, page, T, past, lens = case
+    total = [p + n for p, n in zip(past, lens)]
+    c, g = make(len(past), kv, dim, dtype, page, total, seed=heads)
+    keys, values = fill(c, total, g)
+    q = torch.randn(len(past), T, heads, dim, generator=g).to(dtype).cuda()
+    start, n = torch.tensor(past, device="cuda"), torch.tensor(lens, device="cuda")
+    for causal in (True, False):
+        check_attend(c, c.attend(0, q, start, n, causal=causal), q, keys, values, past, lens, causal)
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,tokens,alive", [(450, 1, 450), (450, 2, 5), (40, 1, 2), (40, 70, 3), (33, 1, 33)])
+def test_attend_many_rows_some_empty(batch, tokens, alive, dtype):
+    """Batches of more rows than a warp or a block has lanes, with rows that have no tokens this time."""
+    g = torch.Generator().manual_seed(batch + tokens)
+    past = [int(x) for x in torch.randint(0, 300, (batch,), generator=g)]
+    lens = [0] * batch
+    for i, b in enumerate(torch.randperm(batch, generator=g)[:alive].tolist()):
+        lens[b] = 1 + i % tokens
+    total = [p + n for p, n in zip(past, lens)]
+    c, g = make(batch, 1, 64, dtype, 32, total, seed=batch)
+    keys, values = fill(c, total, g)
+    q = torch.randn(batch, tokens, 4, 64, generator=g).to(dtype).cuda()
+    out = c.attend(0, q, torch.tensor(past, device="cuda"), torch.tensor(lens, device="cuda"))
+    check_attend(c, out, q, keys, values, past, lens)
+    again = c.attend(0, q, torch.tensor(past, device="cuda"), torch.tensor(lens, device="cuda"))
+    assert torch.equal(out, again)  # the joins add in the order of the CTAs, whoever finishes last
+
+
+def test_rows_that_see_nothing():
+    """Positions before the row's first key, and chunks behind the table's end, give zeros or what the table holds."""
+    c, g = make(3, 1, 64, torch.bfloat16, 16, [40, 40, 40], seed=3)
+    keys, values = fill(c, [40, 40, 40], g)
+    q = torch.randn(3, 4, 2, 64, generator=g).to(torch.bfloat16).cuda()
+    start = torch.tensor([-10, -2, 2 ** 40], device="cuda")
+    out = c.attend(0, q, start)
+    assert (out[0] == 0).all()                       # no key at all
+    assert (out[1, :2] == 0).all() and (out[1, 2:] != 0).any()
+    see = torch.arange(c.capacity) < 40              # the table's last page is missing
+    k = torch.cat([keys[2], torch.zeros(1, c.capacity - 40, 64, dtype=torch.bfloat16)], 1)
+    v = torch.cat([values[2], torch.zeros(1, c.capacity - 40, 64, dtype=torch.bfloat16)], 1)
+    held = (c.table[2].cpu() >= 0).repeat_interleave(16)
+    c.data[0, :, :, :, 8:][:, c.table[2, 2].item()] = 0  # entries 40 .. 47 of row 2's last page
+    out = c.attend(0, q, start)
+    ref = R.attend(q.cpu()[2:], [k], [v], [held], [c.capacity - 4], [4], False, 0, 0, 0.125)
+    assert see.any() and (out[2].double().cpu() - ref[0]).abs().max() <= 2.0 ** -7 * v.abs().max()
+
+
+def test_pool_past_32_bit_offsets():
+    """Pages behind 2^31 elements of one plane, written, attended, copied on write and moved."""
+    from domino_b200 import PagedKVCache, Rope
+
+    pages, page, kv, D = 40000, 64, 8, 128           # 2.6e9 elements a plane
+    c = PagedKVCache(1, 2, kv, pages, D, torch.bfloat16, "cuda", page_size=page, row_pages=4)
+    c.refs.fill_(1)
+    c.refs[-6:] = 0                                  # only the last pages are free
+    g = torch.Generator().manual_seed(0)
+    rope = Rope(D, device="cuda")
+    q, k, v = (torch.randn(2, 100, h, D, generator=g).to(torch.bfloat16).cuda() for h in (8, kv, kv))
+    start = torch.zeros(2, dtype=torch.long, device="cuda")
+    n = torch.tensor([100, 0], device="cuda")
+    c.reserve(start + n)
+    assert c.table[0, :2].tolist() == [pages - 6, pages - 5]
+    qr = c.write(0, q, k, v, rope, start, n)
+    small = PagedKVCache(1, 2, kv, 4, D, torch.bfloat16, "cuda", page_size=page, row_pages=4)
+    small.reserve(start + n)
+    assert torch.equal(small.write(0, q, k, v, rope, start, n), qr)
+    out = c.attend(0, qr, start, n)
+    assert torch.equal(out, small.attend(0, qr, start, n))
+    for x in (c, small):
+        x.length.copy_(n)
+        x.fork(torch.zeros(2, dtype=torch.long, device="cuda"))
+        x.reserve(x.length + 20)                     # row 1 gets a copy of the shared last page
+    assert torch.equal(c.attend(0, qr[:, :1], c.length - 1), small.attend(0, qr[:, :1], small.length - 1))
+    assert c.table[1, 1] != c.table[0, 1]
+    c.refs[: pages - 6] = 0
+    before = c.attend(0, qr[:, :1], c.length - 1)
+    c.compact()
+    assert int(c.table.max()) < 5 and torch.equal(c.attend(0, qr[:, :1], c.length - 1), before)
+    assert c.status() == 0
+
+
+def test_calls_on_another_stream():
+    from domino_b200 import PagedKVCache, Rope
+
+    g = torch.Generator().manual_seed(1)
+    rope = Rope(64, device="cuda")
+    q, k, v = (torch.randn(2, 30, h, 64, generator=g).to(torch.float16).cuda() for h in (4, 2, 2))
+    start = torch.zeros(2, dtype=torch.long, device="cuda")
+    results = []
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        c = PagedKVCache(1, 2, 2, 8, 64, torch.float16, "cuda", page_size=16, row_pages=4)
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            c.reserve(start + 30)
+            out = c.attend(0, c.write(0, q, k, v, rope, start), start)
+            c.length.add_(30)
+            c.crop(start + 17)
+        torch.cuda.current_stream().wait_stream(stream)
+        torch.cuda.synchronize()
+        results.append((out, c.table.clone(), c.length.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_first_rows_share_the_pool():
+    from domino_b200 import PagedKVCache
+
+    c = PagedKVCache(1, 3, 1, 8, 8, torch.float32, "cuda", page_size=16, row_pages=2)
+    one = c.first_rows(1)
+    one.reserve(torch.tensor([20], device="cuda"))
+    one.length.fill_(20)
+    assert c.table.tolist() == [[0, 1], [-1, -1], [-1, -1]] and c.length.tolist() == [20, 0, 0]
+    c.fork(torch.zeros(3, dtype=torch.long, device="cuda"))
+    assert c.refs.tolist()[:2] == [3, 3]
+    one.reserve(torch.tensor([25], device="cuda"))   # the shared second page is replaced for this row alone
+    assert c.table.tolist() == [[0, 2], [0, 1], [0, 1]] and c.refs.tolist()[:3] == [3, 2, 1]
+    with pytest.raises(ValueError):
+        c.first_rows(4)
