@@ -2,13 +2,13 @@
 // products must not be rounded to 11 or 8 bits, and 16-bit heads of more than
 // 128 values.
 //
-// One CTA of 256 threads holds 64 query rows (token t, head g of the group) and
+// One CTA of 256 threads holds 16 kR query rows (token t, head g of the group) and
 // walks the keys in tiles of kKeys, double-buffered by asynchronous copies.
-// Thread (ty, tx) of 16 x 16 computes rows 4 ty .. 4 ty + 3: scores of keys tx,
-// tx + 16, .. (a 4 x kKeys / 16 register tile, both operands read 16 bytes at a
+// Thread (ty, tx) of 16 x 16 computes rows kR ty ..: scores of keys tx, tx + 16,
+// .. (a kR x kKeys / 16 register tile, both operands read 16 bytes at a
 // time along the head dimension), the running maximum and sum (shuffles among
 // the 16 threads of a row), the weights through shared memory, which only the
-// row's own half-warp reads, and 4 x kDim / 16 sums of weighted values.
+// row's own half-warp reads, and kR x kDim / 16 sums of weighted values.
 // Bound by the FMA units when a tile has many rows, by latency when calls are
 // small.  The cut and the join are those of dd_attend_cut.cuh.
 //
@@ -20,27 +20,31 @@
 namespace dd {
 
 constexpr int kF32Threads = 256;
-constexpr int kF32Rows = 64;
+constexpr int kF32Rows = 64;  // at most
 
-template <int kDim>
+// kR rows a thread, 16 kR rows a tile: one for a token or two (more would only
+// be empty), four where calls are large, two where that leaves SMs without work.
+template <int kDim, int kR>
 struct F32Shape {
+  static constexpr int kRows = 16 * kR;
   static constexpr int kKeys = kDim > 128 ? 32 : 64;
   static constexpr int kRow = kDim + 4;  // floats of a padded row: 16-byte reads of consecutive rows fall in different banks
   static constexpr int kWeightRow = kKeys + 4;
-  static constexpr int kSmem = 4 * (kF32Rows * kRow + 4 * kKeys * kRow + kF32Rows * kWeightRow);
+  static constexpr int kSmem = 4 * (kRows * kRow + 4 * kKeys * kRow + kRows * kWeightRow);
 };
 
-template <typename T, int kDim>
+template <typename T, int kDim, int kR>
 __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_constant__ AttendParams a,
                                                                  const __grid_constant__ AttendWork work) {
-  using Shape = F32Shape<kDim>;
+  using Shape = F32Shape<kDim, kR>;
+  constexpr int kRows = Shape::kRows;
   constexpr int kKeys = Shape::kKeys, kRow = Shape::kRow, kCols = kDim / 64, kScores = kKeys / 16;
   extern __shared__ __align__(16) float sm_f32[];
   __shared__ CutShared cut;
   __shared__ CutScan scan;
   __shared__ int key_seen[2][kKeys];  // whether any row of the item sees the key
   float* sm_q = sm_f32;
-  float* sm_k = sm_q + kF32Rows * kRow;   // two buffers
+  float* sm_k = sm_q + kRows * kRow;   // two buffers
   float* sm_v = sm_k + 2 * kKeys * kRow;  // two buffers
   float* sm_w = sm_v + 2 * kKeys * kRow;
   const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
@@ -51,16 +55,23 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
   Piece p = cut.first;
   bool more = p.left > 0;
   const int chunks = a.dim / 4;  // 16-byte chunks of an fp32 row
-  // (columns behind the head's end stay zero)
-  for (int i = tid; i < (kF32Rows + 4 * kKeys) * kRow; i += kF32Threads) sm_f32[i] = 0.0f;
-  __syncthreads();
+  // (columns behind the head's end and rows behind the last hold anything: they
+  // only reach sums that are not stored)
+  const bool vec = std::is_same<T, float>::value && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 &&
+                   a.q_stride[0] % 4 == 0 && a.q_stride[1] % 4 == 0 && a.q_stride[2] % 4 == 0;
 
   for (; more; more = piece_next(a, p, q_tiles, a.item_rows)) {
     const int r0 = p.qt * a.item_rows, rows = min(p.span.rows - r0, a.item_rows);
     const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + (long long)p.h * group * a.q_stride[2];
-    for (int i = tid; i < rows * a.dim; i += kF32Threads) {
-      const int row = i / a.dim, d = i - row * a.dim, t = (r0 + row) / group, g = r0 + row - t * group;
-      sm_q[row * kRow + d] = io<T>::to_f(q[t * a.q_stride[1] + g * a.q_stride[2] + d]);
+    for (int i = tid; i < rows * chunks; i += kF32Threads) {
+      const int row = i / chunks, d = (i - row * chunks) * 4, t = (r0 + row) / group, g = r0 + row - t * group;
+      const T* src = q + t * a.q_stride[1] + g * a.q_stride[2] + d;
+      float4 x;
+      if (vec)
+        x = *reinterpret_cast<const float4*>(src);
+      else
+        x = make_float4(io<T>::to_f(src[0]), io<T>::to_f(src[1]), io<T>::to_f(src[2]), io<T>::to_f(src[3]));
+      *reinterpret_cast<float4*>(sm_q + row * kRow + d) = x;
     }
     constexpr int kSub = kKeyTile / kKeys;
     const int steps = (p.i1 - p.i0) * kSub;
@@ -95,11 +106,11 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       cp_async_commit();
     };
     // the thread's rows: what they see
-    int hi[4], lo[4];
-    float m[4], l[4], o[4][4 * kCols];
+    int hi[kR], lo[kR];
+    float m[kR], l[kR], o[kR][4 * kCols];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * ty + i;
+    for (int i = 0; i < kR; ++i) {
+      const int row = kR * ty + i;
       hi[i] = lo[i] = 0;
       if (row < rows) {
         const int pos = p.span.start + (r0 + row) / group;
@@ -123,16 +134,16 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       const int key0 = p.span.tile(p.i0 + step / kSub) * kKeyTile + step % kSub * kKeys, buf = step & 1;
       const float* ks = sm_k + buf * kKeys * kRow;
       const float* vs = sm_v + buf * kKeys * kRow;
-      float s[4][kScores] = {};
+      float s[kR][kScores] = {};
 #pragma unroll 2
       for (int d = 0; d < a.dim; d += 4) {
-        float4 x[4], y[kScores];
+        float4 x[kR], y[kScores];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(sm_q + (4 * ty + i) * kRow + d);
+        for (int i = 0; i < kR; ++i) x[i] = *reinterpret_cast<const float4*>(sm_q + (kR * ty + i) * kRow + d);
 #pragma unroll
         for (int j = 0; j < kScores; ++j) y[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kRow + d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kR; ++i)
 #pragma unroll
           for (int j = 0; j < kScores; ++j) {
             s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
@@ -143,7 +154,7 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       }
       bool whole = true;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kR; ++i) {
         float top = -INFINITY;
         bool see[kScores];
 #pragma unroll
@@ -164,7 +175,7 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
         for (int j = 0; j < kScores; ++j) {
           const float w = see[j] ? exp2f(s[i][j] - sub) : -0.0f;
           sum += w;
-          sm_w[(4 * ty + i) * Shape::kWeightRow + tx + 16 * j] = w;
+          sm_w[(kR * ty + i) * Shape::kWeightRow + tx + 16 * j] = w;
         }
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -177,9 +188,9 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       auto weigh = [&](auto masked) {
 #pragma unroll 2
         for (int k = 0; k < kKeys; k += 4) {
-          float4 w4[4];
+          float4 w4[kR];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w4[i] = *reinterpret_cast<const float4*>(sm_w + (4 * ty + i) * Shape::kWeightRow + k);
+          for (int i = 0; i < kR; ++i) w4[i] = *reinterpret_cast<const float4*>(sm_w + (kR * ty + i) * Shape::kWeightRow + k);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             float v[4 * kCols];
@@ -187,7 +198,7 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
             for (int c = 0; c < kCols; ++c)
               *reinterpret_cast<float4*>(v + 4 * c) = *reinterpret_cast<const float4*>(vs + (k + u) * kRow + 4 * tx + 64 * c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kR; ++i) {
               const float w = u == 0 ? w4[i].x : u == 1 ? w4[i].y : u == 2 ? w4[i].z : w4[i].w;
 #pragma unroll
               for (int c = 0; c < 4 * kCols; ++c) {
@@ -210,17 +221,17 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
     const bool split = p.i0 > 0 || p.i1 < p.span.n;
     const size_t slot = 2 * (size_t)blockIdx.x + (p.i0 == 0 ? 1 : 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * ty + i, r = r0 + row;
+    for (int i = 0; i < kR; ++i) {
+      const int row = kR * ty + i, r = r0 + row;
       if (row >= a.item_rows || r >= a.tokens * group) continue;
       const float inv = l[i] == 0.0f || row >= rows ? 0.0f : 1.0f / l[i];
       if (split) {
-        float* part = work.o + (slot * kF32Rows + row) * kDim;
+        float* part = work.o + (slot * kRows + row) * kDim;
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
           *reinterpret_cast<float4*>(part + 4 * tx + 64 * c) =
               make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
-        if (tx == 0) work.ml[slot * kF32Rows + row] = make_float2(m[i], l[i]);
+        if (tx == 0) work.ml[slot * kRows + row] = make_float2(m[i], l[i]);
       } else {
         const int t = r / group, g = r - t * group;
         T* out = static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * group + g) * a.dim;
@@ -238,7 +249,7 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       __syncthreads();
       if (tid == 0) finish_piece(work, cut, p);
       __syncthreads();
-      if (cut.join) join_pieces<T, kDim, kF32Rows, kF32Threads / 32>(a, work, p, cut.c0, cut.c1, tid);
+      if (cut.join) join_pieces<T, kDim, kRows, kF32Threads / 32>(a, work, p, cut.c0, cut.c1, tid);
     }
   }
   zero_blind_tiles<T>(a, q_tiles, tid, kF32Threads);

@@ -283,15 +283,15 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, Att
   w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * kRows * kDim);
   return launch("attend", attend_tc_kernel<T, kDim, kPair>, dim3(grid), dim3(kAttThreads), kAttSmem, stream, mk, mv, mq, p, w);
 }
-template <typename T, int kDim>
+template <typename T, int kDim, int kR>
 int launch_attend_f32(const dd_paged_cache* c, AttendParams p, const DeviceInfo& dev, void* stream) {
-  constexpr int kSmem = F32Shape<kDim>::kSmem;
+  using Shape = F32Shape<kDim, kR>;
   static bool ready[64];
   if (!ready[c->device]) {
-    DD_TRY(cudaFuncSetAttribute(attend_f32_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    DD_TRY(cudaFuncSetAttribute(attend_f32_kernel<T, kDim, kR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem));
     ready[c->device] = true;
   }
-  p.item_rows = p.tile_rows = kF32Rows;
+  p.item_rows = p.tile_rows = Shape::kRows;
   p.min_tiles = 1;
   // two CTAs fit an SM with heads of up to 64 values
   const int grid = std::min(dev.sms * (kDim <= 64 ? 2 : 1), kMaxAttendCtas);
@@ -299,8 +299,17 @@ int launch_attend_f32(const dd_paged_cache* c, AttendParams p, const DeviceInfo&
   AttendWork w;
   w.count = scratch.count;
   w.o = scratch.partial;
-  w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * kF32Rows * kDim);
-  return launch("attend", attend_f32_kernel<T, kDim>, dim3(grid), dim3(kF32Threads), kSmem, stream, p, w);
+  w.ml = reinterpret_cast<float2*>(w.o + (size_t)grid * 2 * Shape::kRows * kDim);
+  return launch("attend", attend_f32_kernel<T, kDim, kR>, dim3(grid), dim3(kF32Threads), Shape::kSmem, stream, p, w);
+}
+// Rows of a tile: with 64 a call of 3 x 16 tokens over 300-1500 keys (12 items of
+// 64 rows) took 29 us, of which a tile's products alone are 9 us on one SM.
+template <typename T, int kDim>
+int launch_attend_f32(const dd_paged_cache* c, const AttendParams& p, const DeviceInfo& dev, void* stream) {
+  const long long rows = (long long)p.tokens * p.group, items = (rows + 63) / 64 * p.batch * p.kv_heads;
+  if (rows <= 16) return launch_attend_f32<T, kDim, 1>(c, p, dev, stream);
+  if (items < dev.sms) return launch_attend_f32<T, kDim, 2>(c, p, dev, stream);
+  return launch_attend_f32<T, kDim, 4>(c, p, dev, stream);
 }
 
 template <typename T>
