@@ -336,15 +336,22 @@ __device__ __forceinline__ void finish_piece(const AttendWork& work, CutShared& 
   sh.join = done == others;
 }
 
-// The pieces of one item, in slot 1 of CTA c0 and slot 0 of those behind it, by
-// kWarps warps.  A warp takes two rows at a time: the lanes read the pieces'
-// (m, l) side by side, then the rows are added up piece by piece with eight
-// loads in flight (the reads come from L2 and one SM does them all).
-template <typename T, int kDim, int kRows, int kWarps>
-__device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork& work, const Piece& p, int c0, int c1,
-                                         int tid) {
-  constexpr int kVec = kDim / 32, kBatch = kDim > 128 ? 1 : 2;  // values per lane, rows at a time
-  const int lane = tid & 31, r0 = p.qt * a.item_rows, last = min(a.item_rows, a.tokens * a.group - r0);
+// A split item whose last piece this CTA brought.
+struct JoinItem {
+  int b, qt, h, rows;  // rows: of the batch row (tokens x group)
+  int c0, c1;
+};
+
+// Its pieces, in slot 1 of CTA c0 and slot 0 of those behind it, by kWarps warps.
+// A warp takes kBatch rows at a time: the lanes read the pieces' (m, l) side by
+// side, then the rows are added up, kUnroll pieces at once.  All that counts here
+// is how many loads are in flight: each comes from L2 and takes about 1000 cycles,
+// and one SM does them all (with 8 loads a thread, 64 rows of 7 pieces took
+// 17 000 cycles of a 45 000-cycle call).
+template <typename T, int kDim, int kRows, int kWarps, int kBatch, int kUnroll>
+__device__ __forceinline__ void join_pieces(const AttendParams& a, const AttendWork& work, const JoinItem& j, int tid) {
+  constexpr int kVec = kDim / 32;  // values per lane
+  const int lane = tid & 31, r0 = j.qt * a.item_rows, last = min(a.item_rows, a.tokens * a.group - r0);
   for (int row0 = tid >> 5; row0 < last; row0 += kWarps * kBatch) {
     float o[kBatch][kVec] = {}, m[kBatch], l[kBatch];
 #pragma unroll
@@ -352,14 +359,15 @@ __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork
       m[i] = -INFINITY;
       l[i] = 0.0f;
     }
-    for (int c = c0; c <= c1; c += 32) {
-      const int mine = c + lane, pieces = min(32, c1 - c + 1);
+    for (int c = j.c0; c <= j.c1; c += 32) {
+      const int mine = c + lane, pieces = min(32, j.c1 - c + 1);
       float2 ml[kBatch];
       float w[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int row = min(row0 + kWarps * i, last - 1);
-        ml[i] = mine <= c1 ? __ldcg(&work.ml[(2 * (size_t)mine + (mine == c0)) * kRows + row]) : make_float2(-INFINITY, 0.0f);
+        ml[i] = mine <= j.c1 ? __ldcg(&work.ml[(2 * (size_t)mine + (mine == j.c0)) * kRows + row])
+                             : make_float2(-INFINITY, 0.0f);
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -377,13 +385,14 @@ __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork
 #pragma unroll
         for (int v = 0; v < kVec; ++v) o[i][v] *= keep;
       }
-      // four pieces at a time; what is behind the last one is that one again, with weight zero
-      for (int k = 0; k < pieces; k += 4) {
-        alignas(16) float x[4][kBatch][kVec];
+      // what is behind the last piece is that one again, with weight zero
+#pragma unroll 1
+      for (int k = 0; k < pieces; k += kUnroll) {
+        alignas(16) float x[kUnroll][kBatch][kVec];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kUnroll; ++u) {
           const int piece = c + min(k + u, pieces - 1);
-          const float* part = work.o + (2 * (size_t)piece + (piece == c0)) * kRows * kDim + lane * kVec;
+          const float* part = work.o + (2 * (size_t)piece + (piece == j.c0)) * kRows * kDim + lane * kVec;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const float* from = part + min(row0 + kWarps * i, last - 1) * kDim;
@@ -397,7 +406,7 @@ __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork
           }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const float wk = __shfl_sync(0xffffffffu, w[i], (k + u) & 31);
@@ -411,10 +420,10 @@ __device__ __noinline__ void join_pieces(const AttendParams& a, const AttendWork
       const int row = row0 + kWarps * i, r = r0 + row, t = r / a.group, g = r - t * a.group;
       if (row >= last || lane * kVec >= a.dim) continue;
       const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-      const bool live = r < p.span.rows;  // the pieces of rows behind the chunk's end hold anything
+      const bool live = r < j.rows;  // the pieces of rows behind the chunk's end hold anything
 #pragma unroll
       for (int v = 0; v < kVec; ++v) o[i][v] = live ? o[i][v] * inv : 0.0f;
-      T* out = static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * a.group + g) * a.dim + lane * kVec;
+      T* out = static_cast<T*>(a.out) + (((long long)j.b * a.tokens + t) * a.heads + j.h * a.group + g) * a.dim + lane * kVec;
 #pragma unroll
       for (int v = 0; v < kVec; v += 2) store2(out + v, o[i][v], o[i][v + 1]);
     }

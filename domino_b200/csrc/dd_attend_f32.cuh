@@ -249,7 +249,9 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       __syncthreads();
       if (tid == 0) finish_piece(work, cut, p);
       __syncthreads();
-      if (cut.join) join_pieces<T, kDim, kRows, kF32Threads / 32>(a, work, p, cut.c0, cut.c1, tid);
+      if (cut.join)
+        join_pieces<T, kDim, kRows, kF32Threads / 32, (kDim > 128 ? 2 : 4), 3>(
+            a, work, JoinItem{p.b, p.qt, p.h, p.span.rows, cut.c0, cut.c1}, tid);
     }
   }
   zero_blind_tiles<T>(a, q_tiles, tid, kF32Threads);

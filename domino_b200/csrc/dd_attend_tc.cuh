@@ -179,6 +179,8 @@ struct AttendShared {
   uint32_t tmem_base;
   int abort_flag;
   CutShared cut;
+  int n_joins;
+  JoinItem joins[2];    // a run's first and last item
   unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
   float row_norm[128];
   union {
@@ -213,6 +215,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 
   if (tid == 0) {
     bar.abort_flag = 0;
+    bar.n_joins = 0;
     bar.redo[0] = bar.redo[1] = 0;
     for (int i = 0; i < Shape::kStages; ++i) {
       mbar_init(&bar.full[i], 1);
@@ -768,17 +771,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         if (!ok) break;
       }
       if (split) {
-        // the piece is in the workspace; whoever brings the last one adds them up
+        // the piece is in the workspace; whoever brings the item's last adds them up, when its own run is done
         __threadfence();
         warp_arrive(&bar.both, lane);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
-        if (tid == 0) finish_piece(work, bar.cut, p);
-        warp_arrive(&bar.both, lane);
-        ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
-        if (!ok) break;
-        const Piece here = p;
-        if (bar.cut.join) join_pieces<T, kDim, Shape::kRows, 8>(a, work, here, bar.cut.c0, bar.cut.c1, tid);
+        if (tid == 0) {
+          finish_piece(work, bar.cut, p);
+          if (bar.cut.join) bar.joins[bar.n_joins++] = JoinItem{p.b, p.qt, p.h, p.span.rows, bar.cut.c0, bar.cut.c1};
+        }
       }
       if (!kPair) {  // O, the maxima and the flags have been read; the next piece's first P waits for the other stream's
         tc_fence_before();
@@ -796,6 +797,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     tmem_dealloc(tmem, 512);
   }
   if (tid == 0 && bar.abort_flag) atomicOr(a.status, DD_STATUS_TIMEOUT);
+  for (int i = 0; i < bar.n_joins; ++i)
+    join_pieces<T, kDim, Shape::kRows, kAttThreads / 32, 6, 3>(a, work, bar.joins[i], tid);
 }
 
 }  // namespace dd
