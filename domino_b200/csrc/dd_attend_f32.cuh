@@ -78,20 +78,30 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
     // tile `step`'s keys and values into buffer step & 1; what no row sees becomes zero
     auto load = [&](int step) {
       const int key0 = p.span.tile(p.i0 + step / kSub) * kKeyTile + step % kSub * kKeys, buf = step & 1;
-      for (int i = tid; i < kKeys * chunks; i += kF32Threads) {
-        const int k = i / chunks, c = i - k * chunks, j = key0 + k;
-        int page = -1;
-        if (j < p.span.hi && (j >= p.span.lo || j < a.sinks)) {
-          page = a.table[(long long)p.b * a.row_pages + (j >> a.page_shift)];
-          if (page >= a.pages) page = -1;
-        }
-        if (c == 0) key_seen[buf][k] = page >= 0;
-        const long long at = (((long long)page * a.kv_heads + p.h) * a.page_size + (j & (a.page_size - 1))) * a.dim + c * 4;
+      // a thread keeps one 16-byte chunk of the rows; all its table entries are read before the first copy
+      constexpr int kChunks = kDim / 4, kStep = kF32Threads / kChunks, kLoads = kKeys / kStep;
+      const int c = tid % kChunks, k0 = tid / kChunks;
+      int page[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int j = key0 + k0 + i * kStep;
+        page[i] = -1;
+        if (j < p.span.hi && (j >= p.span.lo || j < a.sinks))
+          page[i] = a.table[(long long)p.b * a.row_pages + (j >> a.page_shift)];
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int k = k0 + i * kStep, j = key0 + k;
+        const bool have = page[i] >= 0 && page[i] < a.pages;
+        if (c == 0) key_seen[buf][k] = have;
+        if (c >= chunks) continue;
+        const long long at =
+            (((long long)page[i] * a.kv_heads + p.h) * a.page_size + (j & (a.page_size - 1))) * a.dim + c * 4;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           float* dst = (kv ? sm_v : sm_k) + (buf * kKeys + k) * kRow + c * 4;
           const T* src = static_cast<const T*>(a.pool[kv]) + at;
-          if (page < 0) {
+          if (!have) {
             *reinterpret_cast<float4*>(dst) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           } else if constexpr (std::is_same<T, float>::value) {
             cp_async16(dst, src, 16);
@@ -123,6 +133,7 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       for (int c = 0; c < 4 * kCols; ++c) o[i][c] = 0.0f;
     }
     const float sl = a.scale * 1.4426950408889634f;
+    const bool busy = kR * (tid / 32 * 2) < rows;  // a warp without rows leaves shared memory to the others
     load(0);
     for (int step = 0; step < steps; ++step) {
       if (step + 1 < steps) load(step + 1);
@@ -134,87 +145,89 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
       const int key0 = p.span.tile(p.i0 + step / kSub) * kKeyTile + step % kSub * kKeys, buf = step & 1;
       const float* ks = sm_k + buf * kKeys * kRow;
       const float* vs = sm_v + buf * kKeys * kRow;
-      float s[kR][kScores] = {};
+      if (busy) {
+        float s[kR][kScores] = {};
 #pragma unroll 2
-      for (int d = 0; d < a.dim; d += 4) {
-        float4 x[kR], y[kScores];
+        for (int d = 0; d < a.dim; d += 4) {
+          float4 x[kR], y[kScores];
 #pragma unroll
-        for (int i = 0; i < kR; ++i) x[i] = *reinterpret_cast<const float4*>(sm_q + (kR * ty + i) * kRow + d);
+          for (int i = 0; i < kR; ++i) x[i] = *reinterpret_cast<const float4*>(sm_q + (kR * ty + i) * kRow + d);
 #pragma unroll
-        for (int j = 0; j < kScores; ++j) y[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kRow + d);
+          for (int j = 0; j < kScores; ++j) y[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kRow + d);
 #pragma unroll
-        for (int i = 0; i < kR; ++i)
+          for (int i = 0; i < kR; ++i)
+#pragma unroll
+            for (int j = 0; j < kScores; ++j) {
+              s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
+              s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
+              s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
+              s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+            }
+        }
+        bool whole = true;
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+          float top = -INFINITY;
+          bool see[kScores];
 #pragma unroll
           for (int j = 0; j < kScores; ++j) {
-            s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-            s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-            s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-            s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+            const int key = key0 + tx + 16 * j;
+            see[j] = key < hi[i] && (key >= lo[i] || key < a.sinks) && key_seen[buf][tx + 16 * j];
+            whole = whole && see[j];
+            s[i][j] = see[j] ? s[i][j] * sl : -INFINITY;
+            top = max3_nan(top, s[i][j], s[i][j]);
           }
-      }
-      bool whole = true;
 #pragma unroll
-      for (int i = 0; i < kR; ++i) {
-        float top = -INFINITY;
-        bool see[kScores];
+          for (int d = 8; d > 0; d >>= 1) top = max3_nan(top, __shfl_xor_sync(0xffffffffu, top, d), top);
+          if (!(top < INFINITY)) l[i] = __int_as_float(0x7fc00000);  // a NaN or +infinity among the scores: the row is NaN
+          const float m1 = fmaxf(m[i], top), sub = m1 == -INFINITY ? 0.0f : m1, keep = exp2f(m[i] - sub);
+          m[i] = m1;
+          float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kScores; ++j) {
-          const int key = key0 + tx + 16 * j;
-          see[j] = key < hi[i] && (key >= lo[i] || key < a.sinks) && key_seen[buf][tx + 16 * j];
-          whole = whole && see[j];
-          s[i][j] = see[j] ? s[i][j] * sl : -INFINITY;
-          top = max3_nan(top, s[i][j], s[i][j]);
+          for (int j = 0; j < kScores; ++j) {
+            const float w = see[j] ? exp2f(s[i][j] - sub) : -0.0f;
+            sum += w;
+            sm_w[(kR * ty + i) * Shape::kWeightRow + tx + 16 * j] = w;
+          }
+#pragma unroll
+          for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          l[i] = l[i] * keep + sum;
+#pragma unroll
+          for (int c = 0; c < 4 * kCols; ++c) o[i][c] *= keep;
         }
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) top = max3_nan(top, __shfl_xor_sync(0xffffffffu, top, d), top);
-        if (!(top < INFINITY)) l[i] = __int_as_float(0x7fc00000);  // a NaN or +infinity among the scores: the row is NaN
-        const float m1 = fmaxf(m[i], top), sub = m1 == -INFINITY ? 0.0f : m1, keep = exp2f(m[i] - sub);
-        m[i] = m1;
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kScores; ++j) {
-          const float w = see[j] ? exp2f(s[i][j] - sub) : -0.0f;
-          sum += w;
-          sm_w[(kR * ty + i) * Shape::kWeightRow + tx + 16 * j] = w;
-        }
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        l[i] = l[i] * keep + sum;
-#pragma unroll
-        for (int c = 0; c < 4 * kCols; ++c) o[i][c] *= keep;
-      }
-      __syncwarp();
-      whole = __all_sync(0xffffffffu, whole);
-      auto weigh = [&](auto masked) {
+        __syncwarp();
+        whole = __all_sync(0xffffffffu, whole);
+        auto weigh = [&](auto masked) {
 #pragma unroll 2
-        for (int k = 0; k < kKeys; k += 4) {
-          float4 w4[kR];
+          for (int k = 0; k < kKeys; k += 4) {
+            float4 w4[kR];
 #pragma unroll
-          for (int i = 0; i < kR; ++i) w4[i] = *reinterpret_cast<const float4*>(sm_w + (kR * ty + i) * Shape::kWeightRow + k);
+            for (int i = 0; i < kR; ++i) w4[i] = *reinterpret_cast<const float4*>(sm_w + (kR * ty + i) * Shape::kWeightRow + k);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            float v[4 * kCols];
+            for (int u = 0; u < 4; ++u) {
+              float v[4 * kCols];
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
-              *reinterpret_cast<float4*>(v + 4 * c) = *reinterpret_cast<const float4*>(vs + (k + u) * kRow + 4 * tx + 64 * c);
+              for (int c = 0; c < kCols; ++c)
+                *reinterpret_cast<float4*>(v + 4 * c) = *reinterpret_cast<const float4*>(vs + (k + u) * kRow + 4 * tx + 64 * c);
 #pragma unroll
-            for (int i = 0; i < kR; ++i) {
-              const float w = u == 0 ? w4[i].x : u == 1 ? w4[i].y : u == 2 ? w4[i].z : w4[i].w;
+              for (int i = 0; i < kR; ++i) {
+                const float w = u == 0 ? w4[i].x : u == 1 ? w4[i].y : u == 2 ? w4[i].z : w4[i].w;
 #pragma unroll
-              for (int c = 0; c < 4 * kCols; ++c) {
-                if constexpr (decltype(masked)::value)
-                  o[i][c] = __float_as_int(w) < 0 ? o[i][c] : fmaf(w, v[c], o[i][c]);
-                else
-                  o[i][c] = fmaf(w, v[c], o[i][c]);
+                for (int c = 0; c < 4 * kCols; ++c) {
+                  if constexpr (decltype(masked)::value)
+                    o[i][c] = __float_as_int(w) < 0 ? o[i][c] : fmaf(w, v[c], o[i][c]);
+                  else
+                    o[i][c] = fmaf(w, v[c], o[i][c]);
+                }
               }
             }
           }
-        }
-      };
-      if (whole)
-        weigh(std::false_type());
-      else
-        weigh(std::true_type());
+        };
+        if (whole)
+          weigh(std::false_type());
+        else
+          weigh(std::true_type());
+      }
       __syncthreads();  // the buffer is loaded again in the next step
     }
     // the piece's result
