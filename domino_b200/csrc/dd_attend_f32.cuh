@@ -202,13 +202,15 @@ __global__ void __launch_bounds__(kF32Threads) attend_f32_kernel(const __grid_co
           for (int k = 0; k < kKeys; k += 4) {
             float4 w4[kR];
 #pragma unroll
-            for (int i = 0; i < kR; ++i) w4[i] = *reinterpret_cast<const float4*>(sm_w + (kR * ty + i) * Shape::kWeightRow + k);
+            for (int i = 0; i < kR; ++i)
+              w4[i] = *reinterpret_cast<const float4*>(sm_w + (kR * ty + i) * Shape::kWeightRow + k);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               float v[4 * kCols];
 #pragma unroll
               for (int c = 0; c < kCols; ++c)
-                *reinterpret_cast<float4*>(v + 4 * c) = *reinterpret_cast<const float4*>(vs + (k + u) * kRow + 4 * tx + 64 * c);
+                *reinterpret_cast<float4*>(v + 4 * c) =
+                    *reinterpret_cast<const float4*>(vs + (k + u) * kRow + 4 * tx + 64 * c);
 #pragma unroll
               for (int i = 0; i < kR; ++i) {
                 const float w = u == 0 ? w4[i].x : u == 1 ? w4[i].y : u == 2 ? w4[i].z : w4[i].w;

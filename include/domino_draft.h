@@ -292,6 +292,7 @@ int dd_set_trace(dd_handle* h, const dd_trace* t);
  * taken lowest number first, so equal calls give equal tables.
  *   data    [layers, 2 (keys, values), pages, kv_heads, page_size, head_dim]
  *   scratch dd_cache_scratch bytes, 16-byte aligned, zero before the first call
+ *           (and again after DD_STATUS_TIMEOUT)
  *   status  one word of DD_STATUS_* bits, set by the kernels, never cleared
  * Calls on one cache must be ordered (one stream, or events between streams).
  * Nothing here synchronises or allocates; everything can be captured. */
