@@ -630,3 +630,27 @@ def test_first_rows_share_the_pool():
     assert c.table.tolist() == [[0, 2], [0, 1], [0, 1]] and c.refs.tolist()[:3] == [3, 2, 1]
     with pytest.raises(ValueError):
         c.first_rows(4)
+
+
+@pytest.mark.parametrize("tokens,dim,past", [(3, 128, 40), (3, 64, 2000), (16, 128, 1500), (30, 128, 900), (90, 128, 60),
+                                             (90, 64, 3000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_non_finite_value_in_every_kind_of_tile(tokens, dim, past, dtype):
+    """A NaN value of the chunk's middle token, in calls with copies of the rows, one tile, pairs of tiles, whole items and
+    items split over CTAs: the tokens before it are untouched, the others have the NaN in its place alone."""
+    c, g = make(1, 2, dim, dtype, 32, [past + tokens], seed=tokens)
+    keys, values = fill(c, [past + tokens], g)
+    q = torch.randn(1, tokens, 8, dim, generator=g).to(dtype).cuda()
+    start = torch.tensor([past], device="cuda")
+    clean = c.attend(0, q, start)
+    check_attend(c, clean, q, keys, values, [past], [tokens])
+    j = past + tokens // 2
+    c.data[0, 1, int(c.table[0, j // 32]), 1, j % 32, 7] = float("nan")  # key head 1: query heads 4 .. 7
+    out = c.attend(0, q, start)
+    assert torch.equal(out[:, :, :4], clean[:, :, :4])
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[:, tokens // 2:, 4:, 7] = True
+    assert bool(torch.isnan(out[bad]).all()) and bool(torch.isfinite(out[~bad]).all())
+    tol = (2 * torch.finfo(dtype).eps / 2 + 2.0 ** -13) * 2 * values[0].abs().max().item()
+    assert (out[~bad].float() - clean[~bad].float()).abs().max() <= tol
+    assert c.status() == 0
