@@ -1,0 +1,78 @@
+"""Edges of the paged key / value cache's operators: what a row's company in the batch may change, numbers at the ends of
+their formats, infinities and NaN in every place, long pieces, shared pages in odd places, tables of 2^31 entries."""
+import math
+
+import pytest
+import torch
+
+from tests import paged_reference as R
+from tests.test_gpu_paged import DTYPES, check_attend, fill, make
+
+pytestmark = pytest.mark.gpu
+LN2 = 0.6931471824645996  # in fp32; times log2(e) in fp32 this is exactly 1, so scores are powers of two
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _require_gpu():
+    if not torch.cuda.is_available() or torch.cuda.get_device_capability(0)[0] != 10:
+        pytest.fail("GPU tests need an sm_100 device")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 16, 40])
+def test_scores_of_2_to_the_29(tokens, dtype):
+    """Scores near the end of what 16-bit queries and keys give, where fp32 counts in steps of 32: the best key is further
+    from the next than those steps, so it takes everything."""
+    past, dim, heads = 300, 128, 4
+    c, g = make(1, 1, dim, dtype, 32, [past + tokens], seed=11)
+    keys, values = fill(c, [past + tokens], g)
+    keys = (torch.rand(past + tokens, dim, generator=g) * 4096 - 2048).to(dtype)
+    pos = torch.arange(past + tokens)
+    c.data[0, 0][c.table.cpu()[0].long()[pos // 32].cuda(), 0, (pos % 32).cuda()] = keys.cuda()
+    q = (torch.rand(1, tokens, heads, dim, generator=g) * 4096 - 2048).to(dtype)
+    s = torch.einsum("thd,jd->thj", q[0].double(), keys.double()) * 8
+    s = s.masked_fill(pos[None, None] > past + torch.arange(tokens)[:, None, None], -math.inf)
+    top = s.topk(2, dim=-1)
+    out = c.attend(0, q.cuda(), torch.tensor([past], device="cuda"), scale=8.0)[0].cpu()
+    # a product's 128 terms of up to 2^25 are summed with steps of at most 2^9 each (2^32 in fp32, cut off): 2^16 in all
+    clear = top.values[..., 0] - top.values[..., 1] > 2.0 ** 17
+    assert clear.double().mean() > 0.9
+    assert torch.equal(out[clear], values[0][0][top.indices[..., 0]][clear])
+    assert c.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 7, 16, 32, 40])
+def test_a_row_alone_and_in_a_batch(tokens, dtype):
+    """The weights' rounding to 16 bits does not depend on where the batch cuts a row's keys.
+
+    Scores are multiples of 2^-6 (in powers of two), so they are exact whatever maximum is taken off, and values are +-1:
+    weights of [2^-3, 1] in 8 or 11 bits add up exactly in fp32 (1024 of them: at most 10 + 3 + 11 bits).  What the cut
+    may change is the fp32 order of the 1024 weights' sum, at most 1024 * 2^-24 = 2^-14 of it: a result moves by one step
+    of its type at most, and only where it lies that near to the middle between two: 2^-14 / 2^-8 of the results in bf16,
+    2^-14 / 2^-11 in fp16, twice that for the two sides."""
+    keys_n, heads, dim, rows = 1024, 4, 64, 45
+    c, g = make(1, 1, dim, dtype, 64, [keys_n], seed=tokens, extra=0)
+    sign = lambda *s: (torch.randint(0, 2, s, generator=g) * 2 - 1).to(dtype)  # noqa: E731
+    table = c.table.cpu()[0].long()
+    c.data[0, 0, table[:16].cuda(), 0] = sign(keys_n, dim).view(16, 64, dim).cuda()
+    c.data[0, 1, table[:16].cuda(), 0] = sign(keys_n, dim).view(16, 64, dim).cuda()
+    q = 3 * sign(1, tokens, heads, dim).cuda()
+    start = torch.tensor([keys_n - tokens], device="cuda")
+    alone = c.attend(0, q, start, scale=LN2 / 64)
+
+    from domino_b200 import PagedKVCache
+
+    many = PagedKVCache(1, rows, 1, c.pages, dim, dtype, "cuda", page_size=64, row_pages=c.row_pages)
+    many.data.copy_(c.data)
+    many.table.copy_(c.table.expand(rows, -1))
+    past = torch.randint(0, keys_n - tokens, (rows,), generator=g)  # the others are shorter, by every length
+    past[::5] = keys_n - tokens
+    out = many.attend(0, q.expand(rows, -1, -1, -1).contiguous(), past.cuda(), scale=LN2 / 64)
+    eps = torch.finfo(dtype).eps / 2
+    a, b = alone.double(), out[::5].double()
+    step = 2 * eps * torch.maximum(a.abs(), b.abs())
+    assert ((a - b).abs() <= 1.01 * step + 2.0 ** -24).all()
+    share = (a != b).double().mean().item()
+    assert share <= 2 * 2.0 ** -14 / eps, share
+    assert many.status() == 0
