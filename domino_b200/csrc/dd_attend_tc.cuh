@@ -557,9 +557,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               }
             }
             have_o = true;
-            const float sub = m == -INFINITY ? 0.0f : m * sl;
+            const float sub = m == -INFINITY ? 0.0f : __fmul_rn(m, sl);
             uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
-            const uint64_t sl2 = pack_f32x2(sl, sl), sub2 = pack_f32x2(-sub, -sub);
+            const uint64_t sub2 = pack_f32x2(-sub, -sub);
 #pragma unroll 1
             for (int c = chunk_a; c < chunk_b; c += kCols) {
               if (chunk_b - chunk_a > kCols) fetch(c);
@@ -569,7 +569,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                   const float x0 = __uint_as_float(x[32 * d + 2 * k]), x1 = __uint_as_float(x[32 * d + 2 * k + 1]);
-                  const uint64_t e = fma_f32x2(pack_f32x2(x0, x1), sl2, sub2);
+                  // scaled and rounded before m is taken off, as m was, so that no score comes out above its maximum
+                  // (a product and a sum in one step put scores of 2^29 up to 2^5 beside it: infinite weights in fp16)
+                  const uint64_t e = add_f32x2(pack_f32x2(__fmul_rn(x0, sl), __fmul_rn(x1, sl)), sub2);
                   float e0, e1;
                   unpack_f32x2(e, e0, e1);
                   const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
