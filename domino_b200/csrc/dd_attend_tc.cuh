@@ -24,11 +24,14 @@
 // result is the same every time.  Lengths are read on the device, so the cut
 // needs no host synchronisation.
 //
-// The running maximum moves only when a row's scores pass it by more than 8
+// The running maximum m moves only when a row's scores pass it by more than 8
 // (as powers of two): P then stays below 2^8 and the rescaling of O, a round
 // trip through TMEM, is rare.  m, l, S and O are fp32; P is rounded to the
 // cache's type, the one rounding besides the result's (its error is that of
-// one rounding of each weight).
+// one rounding of each weight).  m is a whole number, the maximum rounded up:
+// pieces, streams and copies of a row that took different maxima differ by
+// exact powers of two, so that rounding is the same wherever a row's keys are
+// cut, and what else shares the batch changes a result by fp32 sums alone.
 //
 // A masked key has weight 0, and 0 times a NaN is NaN in a matrix product.
 // So the values of keys that no row of the item sees are set to zero in
@@ -482,7 +485,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       const int p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * a.item_rows) - 1) / group;
       const int all_hi = a.causal ? min(p.span.hi, p_min + 1) : p.span.hi;
       const int all_lo = a.window > 0 ? max(p_max - a.window + 1, 0) : 0;
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, m_limit = -INFINITY, l = 0.0f;  // m_limit: the score, unscaled, beyond which m moves
       bool have_o = false;
       constexpr int kStep = kPair ? 1 : 2;
       int page = (kPair ? 0 : s) < n ? group_page(a, p.b, p.span.tile(p.i0 + (kPair ? 0 : s)), lane) : 0;
@@ -535,10 +538,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             }
             const float mt = max3_nan(top[0], top[1], top[1]);
             if (!(mt < INFINITY)) l = __int_as_float(0x7fc00000);  // a NaN or +infinity among the scores: the row is NaN
-            const bool moves = (mt - m) * sl > 8.0f;
+            const bool moves = mt > m_limit;
             if (__any_sync(0xffffffffu, moves)) {
-              const float m1 = moves ? mt : m;
-              const float keep = moves ? exp2_approx((m - m1) * sl) : 1.0f;
+              const float mt2 = __fmul_rn(mt, sl), m1 = moves ? ceilf(mt2) : m;
+              const float keep = moves ? exp2_approx(m - m1) : 1.0f;
+              // (past 2^20 fp32's steps are not small beside 8: every larger score moves m)
+              if (moves) m_limit = fabsf(mt2) < 1048576.0f ? mt + 8.0f / sl : mt;
               l *= keep;
               m = m1;
               if (have_o) {
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               }
             }
             have_o = true;
-            const float sub = m == -INFINITY ? 0.0f : __fmul_rn(m, sl);
+            const float sub = m == -INFINITY ? 0.0f : m;
             uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
             const uint64_t sub2 = pack_f32x2(-sub, -sub);
 #pragma unroll 1
@@ -569,7 +574,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                   const float x0 = __uint_as_float(x[32 * d + 2 * k]), x1 = __uint_as_float(x[32 * d + 2 * k + 1]);
-                  // scaled and rounded before m is taken off, as m was, so that no score comes out above its maximum
+                  // scaled and rounded before m is taken off, as in m, so that no score comes out above its maximum
                   // (a product and a sum in one step put scores of 2^29 up to 2^5 beside it: infinite weights in fp16)
                   const uint64_t e = add_f32x2(pack_f32x2(__fmul_rn(x0, sl), __fmul_rn(x1, sl)), sub2);
                   float e0, e1;
@@ -641,7 +646,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       T* const out0 = out_row(kPair ? r : row / 4);  // (the divisions run while the last products do)
       bool again;
       float f0 = 1.0f, f1 = 0.0f;  // weights of the streams' sums (kPair: only its own)
-      if (m != -INFINITY) m *= sl;
       if (kPair) {
         ok = mbar_wait_bounded(&bar.o_full[s], n_o[s]++ & 1, abort);
         if (!ok) break;
