@@ -31,21 +31,4 @@ struct AttendParams {
   int causal, window, sinks;
 };
 
-// The keys that a query at position p of a row with `total` keys sees:
-// [0, sinks) and [lo, hi).
-struct Visible {
-  long long lo, hi;
-};
-__device__ __forceinline__ Visible visible(const AttendParams& a, long long p, long long total) {
-  Visible v;
-  v.hi = a.causal ? min(total, p + 1) : total;
-  v.lo = a.window > 0 ? max(p - a.window + 1, 0ll) : 0;
-  return v;
-}
-// Keys of row b: positions below start + lens that its table can hold.
-__device__ __forceinline__ long long row_keys(const AttendParams& a, int b) {
-  const long long n = a.lens ? min(max(a.lens[b], 0ll), (long long)a.tokens) : a.tokens;
-  return min(max(a.start[b] + n, 0ll), (long long)a.row_pages * a.page_size);
-}
-
 }  // namespace dd

@@ -35,9 +35,12 @@
 //
 // A masked key has weight 0, and 0 times a NaN is NaN in a matrix product.
 // So the values of keys that no row of the item sees are set to zero in
-// shared memory (pages behind the end, missing pages, the rest of a page);
-// a tile that only some rows see is searched for infinities and NaN, and an
-// item that holds one is computed again key by key (attend_row_exact).
+// shared memory (pages behind the end, missing pages, the rest of a page).
+// Keys that only some rows see are searched for infinities and NaN, which are
+// set to zero too; where there was one, every row adds those that it sees to
+// its result (add_part_seen).  These keys are at most two for every
+// token of the item (behind its first token, and before its last one's
+// window), so that takes as long for a long row of keys as for a short one.
 #pragma once
 
 #include "dd_attend_cut.cuh"
@@ -124,43 +127,60 @@ __device__ __forceinline__ bool non_finite2(uint32_t w) {
   return (w & e) == e || (w >> 16 & e) == e;
 }
 
-// One query row over the tiles [i0, i1) of its item, key by key, the values
-// of masked keys untouched: the plain definition, for items with non-finite
-// values.  o gets the unnormalised sum, *m the maximum (log2 units), *l the sum.
-template <typename T, int kDim>
-__device__ __noinline__ void attend_row_exact(const AttendParams& a, const Piece& p, int row, float* o, float* m_out,
-                                              float* l_out) {
-  const int group = a.group, t = row / group, g = row - t * group;
-  const Visible v = visible(a, p.span.start + t, row_keys(a, p.b));
-  const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + t * a.q_stride[1] + (p.h * group + g) * a.q_stride[2];
-  const float sl = a.scale * 1.4426950408889634f;
-  float m = -INFINITY, l = 0.0f;
-  for (int d = 0; d < kDim; ++d) o[d] = 0.0f;
-  for (int i = p.i0; i < p.i1; ++i) {
-    const long long j0 = (long long)p.span.tile(i) * kKeyTile;
-    for (long long j = j0; j < j0 + kKeyTile; ++j) {
-      if (j >= v.hi || (j < v.lo && j >= a.sinks)) continue;
+// The word with its infinities and NaN set to zero.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
+}
+
+// (Out of line: in line it cost the hot loop its registers, and 8192 tokens behind 8192 took 1930 us, so 1746.)
+template <typename T>
+__device__ __noinline__ void clean16(uint4* at) {
+  const uint4 w = *at;
+  *at = make_uint4(finite2<T>(w.x), finite2<T>(w.y), finite2<T>(w.z), finite2<T>(w.w));
+}
+
+// The keys that all rows of a piece's item see are [lo, hi) and, below hi, the sinks.
+struct SeenByAll {
+  int lo, hi;
+};
+__device__ __forceinline__ SeenByAll seen_by_all(const AttendParams& a, const Piece& p) {
+  const int first = p.span.start + p.qt * a.item_rows / a.group;
+  const int last = p.span.start + (min(p.span.rows, (p.qt + 1) * a.item_rows) - 1) / a.group;
+  return {a.window > 0 ? max(last - a.window + 1, 0) : 0, a.causal ? min(p.span.hi, first + 1) : p.span.hi};
+}
+
+// Infinities and NaN among values [col, end) of the piece's keys that only some
+// rows of its item see: those that `row` sees are added to its result, which
+// stands in `out` (value col at out[0]).
+template <typename T, typename O>
+__device__ __noinline__ void add_part_seen(const AttendParams& a, const Piece& p, int row, int col, int end, O* out) {
+  const SeenByAll all = seen_by_all(a, p);
+  const int pos = p.span.start + row / a.group;
+  const int hi = a.causal ? min(p.span.hi, pos + 1) : p.span.hi, lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+  // the piece's keys from span.lo on
+  const int from = (p.span.first + max(p.i0 - p.span.n_sink, 0)) * kKeyTile;
+  const int to = min((p.span.first + max(p.i1 - p.span.n_sink, 0)) * kKeyTile, hi);
+  auto add = [&](int j0, int j1) {
+    for (int j = max(j0, from); j < min(j1, to); ++j) {
+      if (j < lo && j >= a.sinks) continue;
       const int page = a.table[(long long)p.b * a.row_pages + (j >> a.page_shift)];
       if (page < 0 || page >= a.pages) continue;
-      const long long at = (((long long)page * a.kv_heads + p.h) * a.page_size + (j & (a.page_size - 1))) * a.dim;
-      const T* k = static_cast<const T*>(a.pool[0]) + at;
-      const T* vv = static_cast<const T*>(a.pool[1]) + at;
-      float s = 0.0f;
-      for (int d = 0; d < a.dim; ++d) s += io<T>::to_f(q[d]) * io<T>::to_f(k[d]);
-      s *= sl;
-      if (s > m) {
-        const float keep = exp2f(m - s);
-        l *= keep;
-        for (int d = 0; d < a.dim; ++d) o[d] *= keep;
-        m = s;
+      const T* v = static_cast<const T*>(a.pool[1]) +
+                   (((long long)page * a.kv_heads + p.h) * a.page_size + (j & (a.page_size - 1))) * a.dim;
+      for (int d = col; d < end; d += 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(v + d);
+        if (!non_finite2<T>(w.x) && !non_finite2<T>(w.y)) continue;
+        const T* x = reinterpret_cast<const T*>(&w);
+        for (int i = 0; i < 4; ++i)
+          if (!isfinite(io<T>::to_f(x[i])))
+            out[d - col + i] = io<O>::from_f(io<O>::to_f(out[d - col + i]) + io<T>::to_f(x[i]));
       }
-      const float w = exp2f(s - (m == -INFINITY ? 0.0f : m));
-      l += w;
-      for (int d = 0; d < a.dim; ++d) o[d] += w * io<T>::to_f(vv[d]);
     }
-  }
-  *m_out = m;
-  *l_out = l;
+  };
+  add(max(p.span.lo, a.sinks), min(all.lo, all.hi));
+  add(all.hi, p.span.hi);
 }
 
 template <int kDim, bool kPair>
@@ -184,7 +204,9 @@ struct AttendShared {
   CutShared cut;
   int n_joins;
   JoinItem joins[2];    // a run's first and last item
-  unsigned redo[2];     // the last piece (counted from 1) of each stream whose values need the exact path
+  // the last piece (counted from 1) with an infinity or a NaN in a key that only some rows see: by stream, with kPair
+  // by even and odd pieces
+  unsigned odd[2];
   float row_norm[128];
   union {
     float2 row_ml[2][128];
@@ -219,7 +241,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
   if (tid == 0) {
     bar.abort_flag = 0;
     bar.n_joins = 0;
-    bar.redo[0] = bar.redo[1] = 0;
+    bar.odd[0] = bar.odd[1] = 0;
     for (int i = 0; i < Shape::kStages; ++i) {
       mbar_init(&bar.full[i], 1);
       mbar_init(&bar.empty[i], 1);
@@ -480,11 +502,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         hi = a.causal ? min(p.span.hi, pos + 1) : p.span.hi;
         lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
       }
-      // rows of the item see all keys of [all_lo, all_hi)
-      const int p_min = p.span.start + p.qt * a.item_rows / group;
-      const int p_max = p.span.start + (min(p.span.rows, (p.qt + 1) * a.item_rows) - 1) / group;
-      const int all_hi = a.causal ? min(p.span.hi, p_min + 1) : p.span.hi;
-      const int all_lo = a.window > 0 ? max(p_max - a.window + 1, 0) : 0;
+      const SeenByAll all = seen_by_all(a, p);
       float m = -INFINITY, m_limit = -INFINITY, l = 0.0f;  // m_limit: the score, unscaled, beyond which m moves
       bool have_o = false;
       constexpr int kStep = kPair ? 1 : 2;
@@ -502,7 +520,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
 #pragma unroll 1
         for (int part = 0; part < Shape::kParts; ++part, ++n_part) {
           const int key0 = tile * kKeyTile, part0 = key0 + part * kPartKeys, part1 = part0 + kPartKeys;
-          const bool whole = missing == 0 && part1 <= all_hi && (part0 >= all_lo || part1 <= a.sinks);
+          const bool whole = missing == 0 && part1 <= all.hi && (part0 >= all.lo || part1 <= a.sinks);
           ok = mbar_wait_bounded(&bar.s_full[s][part], n_s & 1, abort);
           if (!ok) break;
           if (part + 1 == Shape::kParts) ++n_s;
@@ -598,12 +616,12 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             }
             tmem_st_wait();
           }
-          if (!whole) {
+          if (!whole && (!kPair || s == 0)) {  // (pairs: the other stream's products of a part come after this one's)
             const int c = (base + load_index_v<kPair>(i, n)) % (2 * Shape::kStages);
             const int st = c % Shape::kStages;
             ok = mbar_wait_bounded(&bar.full[st], c / Shape::kStages, abort);
             if (!ok) break;
-            // keys that no row of the item sees become zero; those that only some see are searched.
+            // keys that no row of the item sees become zero, and infinities and NaN of those that only some see.
             // Eight lanes a 128-byte row, four rows a step.
             unsigned char* v = sm_ring + st * Shape::kTileBytes + (lane % 8) * 16;
             bool odd = false, wrote = false;
@@ -611,7 +629,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             for (int k = part * kPartKeys + (warp & 3) * (kPartKeys / 4) + lane / 8, k1 = k + kPartKeys / 4; k < k1; k += 4) {
               const int j = key0 + k;
               const bool seen = j < p.span.hi && (j >= p.span.lo || j < a.sinks) && !(missing >> (k / 16) & 1);
-              const bool search = seen && (j >= all_hi || (j < all_lo && j >= a.sinks));
+              const bool search = seen && (j >= all.hi || (j < all.lo && j >= a.sinks));
 #pragma unroll
               for (int hf = 0; hf < Shape::kHalves; ++hf) {
                 uint4* at = reinterpret_cast<uint4*>(v + hf * 128 * 128 + k * 128);
@@ -620,12 +638,15 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                   wrote = true;
                 } else if (search) {
                   const uint4 w = *at;
-                  odd = odd || non_finite2<T>(w.x) || non_finite2<T>(w.y) || non_finite2<T>(w.z) || non_finite2<T>(w.w);
+                  if (non_finite2<T>(w.x) || non_finite2<T>(w.y) || non_finite2<T>(w.z) || non_finite2<T>(w.w)) {
+                    clean16<T>(at);
+                    odd = wrote = true;
+                  }
                 }
               }
             }
             if (wrote) fence_proxy_async_shared();
-            if (odd) bar.redo[s] = n_pieces;
+            if (odd) bar.odd[kPair ? n_pieces & 1 : s] = n_pieces;
           }
           tc_fence_before();
           warp_arrive(&bar.p_full[s][part], lane);
@@ -644,18 +665,14 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         return static_cast<T*>(a.out) + (((long long)p.b * a.tokens + t) * a.heads + p.h * group + g) * a.dim;
       };
       T* const out0 = out_row(kPair ? r : row / 4);  // (the divisions run while the last products do)
-      bool again;
+      bool odd;
       float f0 = 1.0f, f1 = 0.0f;  // weights of the streams' sums (kPair: only its own)
       if (kPair) {
         ok = mbar_wait_bounded(&bar.o_full[s], n_o[s]++ & 1, abort);
         if (!ok) break;
-        warp_arrive(&bar.wg[s], lane);
-        ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
-        if (!ok) break;
-        again = bar.redo[s] == n_pieces;  // nobody searches the next piece before all have read this
-        warp_arrive(&bar.wg[s], lane);
-        ok = mbar_wait_bounded(&bar.wg[s], n_wg++ & 1, abort);
-        if (!ok) break;
+        // The last products came after all of stream 0's weights, and so after its searches; it reaches the piece after
+        // the next, and this word again, only behind the other stream's weights of the next.
+        odd = bar.odd[n_pieces & 1] == n_pieces;
       } else {
         bar.row_ml[s][row] = make_float2(m, l);
         ok = mbar_wait_bounded(&bar.o_full[0], n_o[0]++ & 1, abort);
@@ -664,7 +681,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         warp_arrive(&bar.both, lane);
         ok = mbar_wait_bounded(&bar.both, n_both++ & 1, abort);
         if (!ok) break;
-        again = bar.redo[0] == n_pieces || bar.redo[1] == n_pieces;
+        odd = bar.odd[0] == n_pieces || bar.odd[1] == n_pieces;
         const float m0 = bar.row_ml[0][row].x, m1 = bar.row_ml[1][row].x;
         m = -INFINITY;
         for (int c = row % copy_rows; c < 128; c += copy_rows) m = fmaxf(m, fmaxf(bar.row_ml[0][c].x, bar.row_ml[1][c].x));
@@ -680,22 +697,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       }
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      if (again) {
-        if ((kPair || (s == 0 && row < copy_rows)) && in_chunk) {
-          const Piece here = p;
-          float o[kDim], m_x = -INFINITY, l_x = 0.0f;
-          for (int d = 0; d < kDim; ++d) o[d] = 0.0f;
-          if (live) attend_row_exact<T, kDim>(a, here, r, o, &m_x, &l_x);
-          const float inv_x = l_x == 0.0f ? 0.0f : 1.0f / l_x;
-          if (split) {
-            for (int d = 0; d < kDim; ++d) part[(size_t)slot_row * kDim + d] = o[d];
-            part_ml[slot_row] = make_float2(m_x, l_x);
-          } else {
-            T* out = out_row(r);
-            for (int d = 0; d < a.dim; ++d) out[d] = io<T>::from_f(live ? o[d] * inv_x : 0.0f);
-          }
-        }
-      } else if (kPair) {
+      if (kPair) {
         if (split && in_tile < a.tile_rows) part_ml[slot_row] = make_float2(m, l);
         const float norm = split ? 1.0f : inv;
 #pragma unroll 1
@@ -722,6 +724,13 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                     make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),
                                pack2<T>(o[k + 6], o[k + 7]));
           }
+        }
+        if (odd && in_chunk && live) {
+          const Piece here = p;
+          if (split)
+            add_part_seen<T, float>(a, here, r, 0, a.dim, part + (size_t)slot_row * kDim);
+          else
+            add_part_seen<T, T>(a, here, r, 0, a.dim, out_row(r));
         }
       } else {
         // Each stream's warps take half of the columns, 16 at a time: both
@@ -763,11 +772,21 @@ __global__ void __launch_bounds__(kAttThreads, 1)
                 o.w += x.w;
               }
             if (split) {
-              *reinterpret_cast<float4*>(part + (size_t)k * kDim + col) = o;
+              float* to = part + (size_t)k * kDim + col;
+              *reinterpret_cast<float4*>(to) = o;
+              if (odd && k < rows && col < a.dim) {
+                const Piece here = p;
+                add_part_seen<T, float>(a, here, k, col, col + 4, to);
+              }
             } else if (col < a.dim) {
               const float norm = bar.row_norm[k];
               const uint2 w = make_uint2(pack2<T>(o.x * norm, o.y * norm), pack2<T>(o.z * norm, o.w * norm));
-              *reinterpret_cast<uint2*>((k == row / 4 ? out0 : out_row(k)) + col) = norm == 0.0f ? make_uint2(0, 0) : w;
+              T* to = (k == row / 4 ? out0 : out_row(k)) + col;
+              *reinterpret_cast<uint2*>(to) = norm == 0.0f ? make_uint2(0, 0) : w;
+              if (odd && k < rows) {
+                const Piece here = p;
+                add_part_seen<T, T>(a, here, k, col, col + 4, to);
+              }
             }
           }
           // the other buffer next: the wait in between keeps the two apart

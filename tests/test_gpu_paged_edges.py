@@ -76,3 +76,44 @@ def test_a_row_alone_and_in_a_batch(tokens, dtype):
     share = (a != b).double().mean().item()
     assert share <= 2 * 2.0 ** -14 / eps, share
     assert many.status() == 0
+
+
+@pytest.mark.parametrize("tokens,heads,window", [(300, 1, 0), (300, 1, 60000), (16, 4, 0), (33, 3, 50000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_non_finite_values_in_long_pieces(tokens, heads, window, dtype):
+    """A NaN and infinities that only some queries see, at the end of 65 536 keys that one CTA walks: everything else is
+    as without them, no wait gives up, and the next call on the cache is right."""
+    from domino_b200 import PagedKVCache
+
+    past, dim, page, rows = 65536, 64, 128, 148
+    own = -(-tokens // page)
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    c = PagedKVCache(1, rows, 1, past // page + rows * own, dim, dtype, "cuda", page_size=page, row_pages=past // page + own)
+    c.table[:, : past // page] = torch.arange(past // page, dtype=torch.int32, device="cuda")
+    c.table[:, past // page:] = past // page + torch.arange(rows * own, dtype=torch.int32, device="cuda").view(rows, own)
+    c.data.copy_(torch.randn(c.data.shape, generator=g, device="cuda"))
+    q = torch.randn(rows, tokens, heads, dim, generator=g, device="cuda").to(dtype)
+    start = torch.full((rows,), past, device="cuda")
+    clean = c.attend(0, q, start, window=window)
+    assert c.status() == 0 and bool(torch.isfinite(clean).all())
+    t = tokens // 2
+    edge = past - window + 1 + t if window else None  # seen by tokens 0 .. t, left behind by those after them
+    spots = []
+    for b, value in ((0, float("nan")), (3, float("inf")), (rows - 1, float("-inf"))):
+        spots.append((b, t, slice(t, None), value, (0, 1, past // page + b * own + t // page, 0, t % page, 9)))
+    if window:
+        spots.append((None, None, slice(0, t + 1), float("nan"), (0, 1, edge // page, 0, edge % page, 20)))
+    want, kept = clean.clone(), {}
+    for b, _, seen, value, at in spots:
+        kept[at] = c.data[at].clone()
+        c.data[at] = value
+        rows_hit = slice(None) if b is None else slice(b, b + 1)
+        want[rows_hit, seen, :, at[-1]] = value
+    out = c.attend(0, q, start, window=window)
+    assert c.status() == 0
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    for *_, at in spots:
+        c.data[at] = kept[at]
+    again = c.attend(0, q, start, window=window)
+    assert c.status() == 0 and torch.equal(again, clean)
