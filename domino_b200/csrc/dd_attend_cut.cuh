@@ -385,7 +385,7 @@ __device__ __forceinline__ void join_pieces(const AttendParams& a, const AttendW
 #pragma unroll
         for (int v = 0; v < kVec; ++v) o[i][v] *= keep;
       }
-      // what is behind the last piece is that one again, with weight zero
+      // what is behind the last piece is that one again, left out (an infinity in it must not meet a weight of zero)
 #pragma unroll 1
       for (int k = 0; k < pieces; k += kUnroll) {
         alignas(16) float x[kUnroll][kBatch][kVec];
@@ -411,7 +411,7 @@ __device__ __forceinline__ void join_pieces(const AttendParams& a, const AttendW
           for (int i = 0; i < kBatch; ++i) {
             const float wk = __shfl_sync(0xffffffffu, w[i], (k + u) & 31);
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) o[i][v] += x[u][i][v] * (k + u < pieces ? wk : 0.0f);
+            for (int v = 0; v < kVec; ++v) o[i][v] += k + u < pieces ? x[u][i][v] * wk : 0.0f;
           }
       }
     }

@@ -117,3 +117,47 @@ def test_non_finite_values_in_long_pieces(tokens, heads, window, dtype):
         c.data[at] = kept[at]
     again = c.attend(0, q, start, window=window)
     assert c.status() == 0 and torch.equal(again, clean)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("tokens,dim,past", [(1, 128, 40), (1, 64, 3000), (3, 128, 700), (16, 128, 1500), (16, 64, 9000),
+                                             (30, 128, 900), (90, 64, 3000)])
+@pytest.mark.parametrize("dtype", [torch.float32])
+def test_an_infinite_value_that_is_seen(tokens, dim, past, dtype, value):
+    """An infinity or a NaN among the values, old (every query sees it, in a tile that all see) and new (only the queries
+    behind it do): the results that it is part of are that infinity or a NaN, all others are as without it.
+
+    Queries and keys are of order one, so no weight is anywhere near the end of fp32."""
+    c, g = make(1, 2, dim, dtype, 32, [past + tokens], seed=tokens + dim)
+    fill(c, [past + tokens], g)
+    q = torch.randn(1, tokens, 8, dim, generator=g).to(dtype).cuda()
+    start = torch.tensor([past], device="cuda")
+    clean = c.attend(0, q, start)
+    spots = [0, 5, past // 2, past - 1, past + tokens // 2]
+    for j in spots:
+        at = (0, 1, int(c.table[0, j // 32]), 1, j % 32, 7)
+        keep = c.data[at].clone()
+        c.data[at] = value
+        out = c.attend(0, q, start)
+        c.data[at] = keep
+        t0 = max(j - past, 0)
+        want = torch.full_like(out[0, t0:, 4:, 7], value)  # key head 1 serves query heads 4 .. 7
+        assert torch.allclose(out[0, t0:, 4:, 7], want, equal_nan=True), j
+        out[0, t0:, 4:, 7] = clean[0, t0:, 4:, 7]
+        assert torch.equal(out, clean), j
+    # two infinities of one sign, far apart and side by side, then a NaN's worth: one of each sign
+    for signs in ((1, 1), (1, -1)):
+        for j0, j1 in ((0, past // 2), (5, 6), (past // 2, past + tokens // 2)):
+            keep = []
+            for j, s in zip((j0, j1), signs):
+                at = (0, 1, int(c.table[0, j // 32]), 0, j % 32, 3)
+                keep.append((at, c.data[at].clone()))
+                c.data[at] = s * float("inf")
+            out = c.attend(0, q, start)
+            for at, x in keep:
+                c.data[at] = x
+            t0 = max(j1 - past, 0)
+            got = out[0, t0:, :4, 3]
+            assert bool((got == float("inf")).all() if signs[1] > 0 else torch.isnan(got).all()), (signs, j0, j1)
+            assert bool((out[0, :t0, :4, 3] == float("inf")).all()) or t0 == 0
+    assert c.status() == 0
