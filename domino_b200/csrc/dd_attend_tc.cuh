@@ -334,6 +334,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       return st;
     };
     const uint32_t ring0 = smem_u32(sm_ring), q0 = smem_u32(sm_q);
+    const int copies = kPair ? 1 : a.copies;
     // Scores of stream s from a part of the keys in stage st, and which buffers are free once they are done.
     auto qk = [&](int s, int part, int st, bool free_stage, bool free_q) {
       const uint64_t dq = smem_desc_k_sw128(q0 + (kPair ? s * Shape::kTileBytes : 0));
@@ -354,9 +355,20 @@ __global__ void __launch_bounds__(kAttThreads, 1)
       const uint64_t dv = smem_desc_mn_sw128(ring0 + st * Shape::kTileBytes + part * kPartKeys * 128, 128 * 128);
       if (elect_one()) {
 #pragma unroll
-        for (int d = 0; d < kPartKeys / 16; ++d)
-          mma_f16_ts(tmem + 256 + s * kDim, tmem + s * 128 + part * kPartKeys + d * 8, dv + ((d * 2048) >> 4), idesc_o,
-                     accumulate || d > 0);
+        for (int d = 0; d < kPartKeys / 16; ++d) {
+          const uint32_t to = tmem + 256 + s * kDim, from = tmem + s * 128 + part * kPartKeys + d * 8;
+          if (kPair) {
+            mma_f16_ts(to, from, dv + ((d * 2048) >> 4), idesc_o, accumulate || d > 0);
+          } else {
+            // a step of 16 keys is for the copy of the rows that has them: the others' sums stay (a weight of zero
+            // would make an infinite value NaN there)
+            const int copy = (d * copies) >> 3;
+            uint32_t off[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) off[w] = (w * copies) >> 2 == copy ? 0u : ~0u;
+            mma_f16_ts_lanes(to, from, dv + ((d * 2048) >> 4), idesc_o, accumulate || ((d * copies) & 7) != 0, off);
+          }
+        }
         if (Shape::kParts > 1) mma_commit(&bar.pv_done[s]);
         if (free_stage) mma_commit(&bar.empty[st]);
         if (last) mma_commit(&bar.o_full[s]);
@@ -484,8 +496,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     int base = 0;  // loads before this piece, modulo two rounds of the ring
     bool ok = true, pending = false;
     // Few rows: the tile holds `copies` copies of them, and copy c of a row
-    // takes part c of the tile's keys (P is zero elsewhere), so that all four
-    // warps share the exponentials.  The copies are joined like the streams.
+    // takes part c of the tile's keys (the products leave its sums alone
+    // elsewhere), so that all four warps share the exponentials.  The copies
+    // are joined like the streams.
     const int copies = kPair ? 1 : a.copies, copy_rows = 128 / copies;
     const int chunk0 = (row / copy_rows) * (4 / copies), chunk1 = chunk0 + 4 / copies;
     for (; more && ok; more = piece_next(a, p, q_tiles, a.item_rows)) {
@@ -608,12 +621,6 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             float sum0, sum1;
             unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), sum0, sum1);
             l += sum0 + sum1;
-            if (!kPair && copies > 1) {  // the other copies' keys
-              const uint32_t zero[16] = {};
-#pragma unroll 1
-              for (int c = 0; c < 4; ++c)
-                if (c < chunk0 || c >= chunk1) tmem_st16(t_s + 16 * c, zero);
-            }
             tmem_st_wait();
           }
           if (!whole && (!kPair || s == 0)) {  // (pairs: the other stream's products of a part come after this one's)

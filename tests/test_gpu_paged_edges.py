@@ -122,7 +122,7 @@ def test_non_finite_values_in_long_pieces(tokens, heads, window, dtype):
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 @pytest.mark.parametrize("tokens,dim,past", [(1, 128, 40), (1, 64, 3000), (3, 128, 700), (16, 128, 1500), (16, 64, 9000),
                                              (30, 128, 900), (90, 64, 3000)])
-@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_an_infinite_value_that_is_seen(tokens, dim, past, dtype, value):
     """An infinity or a NaN among the values, old (every query sees it, in a tile that all see) and new (only the queries
     behind it do): the results that it is part of are that infinity or a NaN, all others are as without it.
