@@ -26,8 +26,12 @@
 //
 // The running maximum m moves only when a row's scores pass it by more than 8
 // (as powers of two): P then stays below 2^8 and the rescaling of O, a round
-// trip through TMEM, is rare.  m, l, S and O are fp32; P is rounded to the
-// cache's type, the one rounding besides the result's (its error is that of
+// trip through TMEM, is rare.  In fp16, where weights below 2^-14 would lose
+// bits and those below 2^-25 vanish (from O, not from l: a long even tail under
+// one large weight), P and l are 2^7 times as large: P then stays below 2^15.3,
+// and what loses bits is below 2^-21.  (O is fp32 all the same: of products
+// below 2^-25 of it the tensor cores add nothing.)  m, l, S and O are fp32; P is rounded to
+// the cache's type, the one rounding besides the result's (its error is that of
 // one rounding of each weight).  m is a whole number, the maximum rounded up:
 // pieces, streams and copies of a row that took different maxima differ by
 // exact powers of two, so that rounding is the same wherever a row's keys are
@@ -488,6 +492,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
     // ---------------------------------------------------------------- softmax, one thread per query row
     constexpr int kPartKeys = kKeyTile / Shape::kParts;
     constexpr int kCols = kPair ? 2 : 1;  // groups of 32 columns in registers at a time
+    constexpr float kTopExponent = std::is_same<T, __half>::value ? 7.0f : 0.0f;
     const int s = warp >> 2, row = tid & 127;
     const uint32_t lanes = ((warp & 3) * 32u) << 16;
     const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + lanes;
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
               }
             }
             have_o = true;
-            const float sub = m == -INFINITY ? 0.0f : m;
+            const float sub = (m == -INFINITY ? 0.0f : m) - kTopExponent;
             uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
             const uint64_t sub2 = pack_f32x2(-sub, -sub);
 #pragma unroll 1

@@ -161,3 +161,48 @@ def test_an_infinite_value_that_is_seen(tokens, dim, past, dtype, value):
             assert bool((got == float("inf")).all() if signs[1] > 0 else torch.isnan(got).all()), (signs, j0, j1)
             assert bool((out[0, :t0, :4, 3] == float("inf")).all()) or t0 == 0
     assert c.status() == 0
+
+
+def _one_key_above(n, tokens, below, dtype):
+    """148 rows of `tokens` queries over n keys in one piece each: key 0 has score 0 and value -1, the others score -below
+    (in powers of two) and value 1.  Returns the results and what they are in 64 bits."""
+    from domino_b200 import PagedKVCache
+
+    dim, rows = 64, 148
+    c = PagedKVCache(1, rows, 1, n // 128, dim, dtype, "cuda", page_size=128, row_pages=n // 128)
+    c.table.copy_(torch.arange(n // 128, dtype=torch.int32).expand(rows, -1))
+    c.data[0, 0].zero_()
+    c.data[0, 0, :, :, :, 0] = -below
+    c.data[0, 0, 0, 0, 0, 0] = 0.0
+    c.data[0, 1].fill_(1.0)
+    c.data[0, 1, 0, 0, 0] = -1.0
+    q = torch.zeros(rows, tokens, 1, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    out = c.attend(0, q, torch.full((rows,), n - tokens, device="cuda"), scale=LN2)
+    assert c.status() == 0
+    score = torch.tensor(below, dtype=torch.float64).to(dtype).double().item()
+    others = torch.arange(n - tokens, n, dtype=torch.float64) * 2.0 ** -score
+    return out.double().cpu(), ((others - 1) / (others + 1))[None, :, None, None]
+
+
+@pytest.mark.parametrize("tokens,below", [(130, 25.046875), (130, 18.40625), (300, 24.59375), (100, 25.046875)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_key_far_above_very_many(tokens, below, dtype):
+    """A key that takes nearly all the weight and 65535 others `below` powers of two under it: their sum is part of the
+    result as it is part of the row's sum.
+
+    One rounding of every weight and of the result; at most 1024 additions to the row's sum (2^-24 each).  The products'
+    sum lies in (1/2, 1]: taken one product at a time and rounded to nearest in fp32, whose steps there are 2^-24, each of
+    the 65535 moves it by 2^-25 from the exact one at most, 2^-9 in all, and equal products all to the same side (those
+    below 2^-25 leave it where it is)."""
+    out, ref = _one_key_above(65536, tokens, below, dtype)
+    assert (out - ref).abs().max() <= 2 * torch.finfo(dtype).eps / 2 + 1024 * 2.0 ** -24 + 65535 * 2.0 ** -25
+
+
+@pytest.mark.parametrize("tokens", [130, 300, 100])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_below_fp16_normals_under_one_large_one(tokens, dtype):
+    """The same with weights of 3.02 * 2^-25, whole steps of the products' sum but for 0.02 * 2^-25 each (2^-14.6 in all;
+    3.08 and 2^-12.6 in bf16, whose scores are coarser): a weight that fp16 rounds to 2^-23 by itself would be 2^-9 off."""
+    out, ref = _one_key_above(65536, tokens, 23.40625, dtype)
+    assert (out - ref).abs().max() <= 2 * torch.finfo(dtype).eps / 2 + 1024 * 2.0 ** -24 + 2.0 ** -12.6
