@@ -385,13 +385,20 @@ __device__ __forceinline__ void join_pieces(const AttendParams& a, const AttendW
 #pragma unroll
         for (int v = 0; v < kVec; ++v) o[i][v] *= keep;
       }
-      // what is behind the last piece is that one again, left out (an infinity in it must not meet a weight of zero)
+      // (nothing is read behind the last piece: read again and given weight zero, an infinity in it would be NaN)
 #pragma unroll 1
       for (int k = 0; k < pieces; k += kUnroll) {
         alignas(16) float x[kUnroll][kBatch][kVec];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          const int piece = c + min(k + u, pieces - 1);
+          if (k + u >= pieces) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+              for (int v = 0; v < kVec; ++v) x[u][i][v] = 0.0f;
+            continue;
+          }
+          const int piece = c + k + u;
           const float* part = work.o + (2 * (size_t)piece + (piece == j.c0)) * kRows * kDim + lane * kVec;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
@@ -411,7 +418,7 @@ __device__ __forceinline__ void join_pieces(const AttendParams& a, const AttendW
           for (int i = 0; i < kBatch; ++i) {
             const float wk = __shfl_sync(0xffffffffu, w[i], (k + u) & 31);
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) o[i][v] += k + u < pieces ? x[u][i][v] * wk : 0.0f;
+            for (int v = 0; v < kVec; ++v) o[i][v] += x[u][i][v] * wk;
           }
       }
     }
