@@ -153,6 +153,7 @@ class PagedKVCache:
             device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
         self.capacity = self.row_pages * self.page_size
+        self._whole = True  # all rows that hold pages of this pool
         self.data = torch.zeros(self.layers, 2, self.pages, self.kv_heads, self.page_size, self.head_dim, dtype=dtype,
                                 device=device)
         self.table = torch.full((self.batch, self.row_pages), -1, dtype=torch.int32, device=device)
@@ -165,10 +166,14 @@ class PagedKVCache:
         c.scratch, c.status, c.device = self._scratch.data_ptr(), self._status.data_ptr(), device.index
 
     def first_rows(self, n: int) -> "PagedKVCache":
-        """The first ``n`` rows as a cache of their own, with the same pages and state: for a call on them alone."""
+        """The first ``n`` rows as a cache of their own, with the same pages and state: for a call on them alone.
+
+        ``compact`` is not for such a part: it moves pages of all rows, whose tables the part does not know.
+        """
         if not 1 <= n <= self.batch:
             raise ValueError(f"{n} rows of {self.batch}")
         part = copy.copy(self)
+        part._whole = self._whole and n == self.batch
         part.batch, part.table, part.length = n, self.table[:n], self.length[:n]
         part._c = _lib.DDPagedCache.from_buffer_copy(self._c)
         part._c.batch = n
@@ -311,6 +316,8 @@ class PagedKVCache:
 
     def compact(self) -> None:
         """Move the pages in use to the lowest numbers, so that all pages behind them are free."""
+        if not self._whole:
+            raise ValueError(f"compact needs all rows of the cache, this is its first {self.batch}")
         self._check(self._lib.dd_pages_compact(self._cp, self._stream()), "dd_pages_compact")
 
     def status(self) -> int:

@@ -329,7 +329,9 @@ int dd_pages_crop(const dd_paged_cache* c, const int64_t* to, void* stream);
 int dd_pages_fork(const dd_paged_cache* c, const int64_t* src, void* stream);
 
 /* Move the pages in use to the lowest numbers (contents, tables and counts);
- * the pages behind them are all free afterwards. */
+ * the pages behind them are all free afterwards.  `batch` and `table` must be
+ * those of all rows that hold pages: a row that is left out keeps the numbers
+ * of pages that have moved. */
 int dd_pages_compact(const dd_paged_cache* c, void* stream);
 
 /* One layer's new tokens into the cache: token t of row b, t < lens[b], has

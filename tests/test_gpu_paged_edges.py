@@ -206,3 +206,24 @@ def test_weights_below_fp16_normals_under_one_large_one(tokens, dtype):
     3.08 and 2^-12.6 in bf16, whose scores are coarser): a weight that fp16 rounds to 2^-23 by itself would be 2^-9 off."""
     out, ref = _one_key_above(65536, tokens, 23.40625, dtype)
     assert (out - ref).abs().max() <= 2 * torch.finfo(dtype).eps / 2 + 1024 * 2.0 ** -24 + 2.0 ** -12.6
+
+
+def test_compact_is_for_the_whole_table():
+    """A view of the first rows does not know the other rows' tables: it may not move the pool's pages."""
+    from domino_b200 import PagedKVCache
+
+    c = PagedKVCache(1, 3, 1, 12, 8, torch.float32, "cuda", page_size=16, row_pages=2)
+    c.table.copy_(torch.tensor([[9, -1], [3, 11], [7, -1]], dtype=torch.int32))
+    c.refs[torch.tensor([9, 3, 11, 7], device="cuda")] = 1
+    c.length.copy_(torch.tensor([10, 30, 16]))
+    c.data.copy_(torch.arange(12.0).view(1, 1, 12, 1, 1, 1).expand_as(c.data))
+    before = [x.clone() for x in (c.table, c.refs, c.data)]
+    for view in (c.first_rows(1), c.first_rows(2), c.first_rows(2).first_rows(2)):
+        with pytest.raises(ValueError, match="rows"):
+            view.compact()
+    assert all(torch.equal(a, b) for a, b in zip(before, (c.table, c.refs, c.data)))
+    c.first_rows(3).compact()  # all of them
+    assert c.table.tolist() == [[1, -1], [3, 2], [0, -1]]
+    for b, stamps in enumerate(([9], [3, 11], [7])):
+        assert [c.data[0, 0, p, 0, 0, 0].item() for p in c.table[b].tolist() if p >= 0] == stamps
+    assert c.status() == 0
