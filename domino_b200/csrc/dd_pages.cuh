@@ -278,7 +278,8 @@ __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(uint4* data, P
   const int moves = *s.n_moves;
   if (table) {
     const int used = s.n_moves[1];
-    for (int i = blockIdx.x * kCopyThreads + threadIdx.x; i < entries; i += gridDim.x * kCopyThreads) {
+    // (64 bits: `entries` may be as near to 2^31 as one step)
+    for (long long i = blockIdx.x * kCopyThreads + threadIdx.x; i < entries; i += (long long)gridDim.x * kCopyThreads) {
       const int p = table[i];
       if (p >= used && p < pages) table[i] = s.list[p];
     }

@@ -227,3 +227,25 @@ def test_compact_is_for_the_whole_table():
     for b, stamps in enumerate(([9], [3, 11], [7])):
         assert [c.data[0, 0, p, 0, 0, 0].item() for p in c.table[b].tolist() if p >= 0] == stamps
     assert c.status() == 0
+
+
+def test_compact_with_a_table_of_nearly_2_31_entries():
+    """Entry numbers near 2^31 (a table of 8.6 GB, as much again in the scratch): the moved pages are followed in the
+    last row as in the first."""
+    from domino_b200 import PagedKVCache
+
+    batch, row_pages = 1024, (1 << 21) - 1
+    c = PagedKVCache(1, batch, 1, 10, 8, torch.bfloat16, "cuda", page_size=16, row_pages=row_pages)
+    spots = [(0, 0), (0, row_pages - 1), (511, 77), (1023, row_pages - 300000), (1023, row_pages - 1)]
+    for p, (b, i) in zip((9, 4, 7, 8, 2), spots):
+        c.table[b, i] = p
+        c.refs[p] = 1
+    c.data.copy_(torch.arange(10.0).view(1, 1, 10, 1, 1, 1).expand_as(c.data))
+    c.compact()
+    assert c.status() == 0
+    where = [int(c.table[b, i]) for b, i in spots]
+    assert sorted(where) == [0, 1, 2, 3, 4]
+    assert [c.data[0, 1, p, 0, 0, 0].item() for p in where] == [9, 4, 7, 8, 2]
+    assert int((c.table >= 0).sum()) == 5
+    del c
+    torch.cuda.empty_cache()
