@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(kWriteThreads) cache_write_kernel(const __grid
   if (a.x[0]) {
     T* out = static_cast<T*>(a.q_out) + ((long long)b * a.tokens + t0) * a.heads * a.dim;
     const float zero[4] = {};
-    for (int i = live * a.heads * a.dim / 4 + threadIdx.x; i < n_tok * a.heads * a.dim / 4; i += kWriteThreads)
+    const long long token = (long long)a.heads * a.dim / 4;
+    for (long long i = live * token + threadIdx.x; i < n_tok * token; i += kWriteThreads)
       store4(out + 4 * i, zero);
   }
 }

@@ -410,7 +410,8 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
   if (a->rotary < 0 || a->rotary % 2 || a->rotary > c->head_dim)
     return global_fail(DD_EINVAL, "dd_cache_write: rotary %d is not an even number up to head_dim %d", a->rotary, c->head_dim);
   if (a->rotary && !a->inv_freq) return global_fail(DD_EINVAL, "dd_cache_write: rotary needs inv_freq");
-  if ((long long)(a->heads + 2ll * c->kv_heads) * a->tokens > 0x7fffffffll)
+  if ((long long)(a->heads + 2ll * c->kv_heads) * a->tokens > 0x7fffffffll ||
+      (a->q && (long long)a->heads * c->head_dim > 0x7fffffffll))
     return global_fail(DD_EINVAL, "dd_cache_write: chunk too large");
   DeviceScope scope(c->device);
   if (!scope.ok) return global_fail(DD_ECUDA, "dd_cache_write: cannot select device %d", c->device);
