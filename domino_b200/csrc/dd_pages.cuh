@@ -74,17 +74,56 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
   return r;
 }
 
+// For reserve, where pages behind a row's first slot are shared: which of the
+// slots [first, last) of every row need a copy (old_table: 1 or 0), and their
+// number per row on top of `need`.  Of the rows that reach a page the lowest
+// keeps it when nobody else holds it.  Counts and lowest rows stand in src and
+// dst, which the moves have not used yet.
+__device__ __forceinline__ void plan_deep_copies(const int* table, const int* refs, const PageScratch& s, const int* first,
+                                                 const int* last, int* need, int batch, int pages, int row_pages) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int round = 0; round < 3; ++round) {
+    for (int b = warp; b < batch; b += kPlanThreads / 32) {
+      int copies = 0;
+      for (int i = first[b] + lane; i < last[b]; i += 32) {
+        const int p = table[(size_t)b * row_pages + i];
+        const bool shared = p >= 0 && p < pages && refs[p] > 1;
+        if (round == 0 && shared) {
+          s.src[p] = 0;
+          s.dst[p] = batch;
+        }
+        if (round == 1 && shared) {
+          atomicAdd(&s.src[p], 1);
+          atomicMin(&s.dst[p], b);
+        }
+        if (round == 2) {
+          const bool copy = shared && (refs[p] > s.src[p] || s.dst[p] < b);
+          s.old_table[(size_t)b * row_pages + i] = copy;
+          copies += copy;
+        }
+      }
+      copies = __reduce_add_sync(0xffffffffu, copies);
+      if (round == 2 && lane == 0) need[b] += copies;
+    }
+    __syncthreads();
+  }
+}
+
 // reserve: slots ceil'd over [length, upto) of every row, in row order and
-// within a row in position order; request i gets the i-th free page.
+// within a row in position order; request i gets the i-th free page.  A request
+// is a slot without a page or one whose page other rows hold too.  The latter is
+// as a rule a row's first slot (the page that `length` ends in); slots behind it
+// hold shared pages only where a caller has set a length back by itself, and
+// then plan_deep_copies decides for all slots.
 __global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(int* table, const long long* length, int* refs,
                                                                      PageScratch s, unsigned* status,
                                                                      const long long* upto, int batch, int pages,
                                                                      int page_size, int row_pages) {
   __shared__ int first[kMaxCacheBatch], last[kMaxCacheBatch], held[kMaxCacheBatch], need[kMaxCacheBatch];
-  __shared__ int n_moves;
+  __shared__ int n_moves, deep;  // deep: shared pages behind a row's first slot
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait_primary();
-  if (tid == 0) n_moves = 0;
+  if (tid == 0) n_moves = deep = 0;
   // what each row misses
   if (tid < batch) {
     const long long len = max(length[tid], 0ll), cap = (long long)row_pages * page_size;
@@ -105,9 +144,15 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(int* table,
     for (int i = first[b] + lane; i < last[b]; i += 32) {
       const int p = table[(size_t)b * row_pages + i];
       miss += p < 0 || p >= pages;
+      if (i > first[b] && p >= 0 && p < pages && refs[p] > 1) deep = 1;
     }
     miss = __reduce_add_sync(0xffffffffu, miss);
     if (lane == 0) need[b] = miss;
+  }
+  __syncthreads();
+  if (deep) {
+    plan_deep_copies(table, refs, s, first, last, need, batch, pages, row_pages);
+    if (tid < batch) held[tid] = -1;  // (its copies are among them)
   }
   __syncthreads();
   // a held page that others hold too is copied, except by the first row of
@@ -163,16 +208,25 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(int* table,
     for (int i0 = first[b]; i0 < last[b]; i0 += 32) {
       const int i = i0 + lane;
       int* e = &table[(size_t)b * row_pages + i];
-      const bool miss = i < last[b] && (*e < 0 || *e >= pages);
+      const bool copy = deep && i < last[b] && s.old_table[(size_t)b * row_pages + i];
+      const bool miss = i < last[b] && (*e < 0 || *e >= pages || copy);
       const unsigned m = __ballot_sync(0xffffffffu, miss);
       const int r = at + __popc(m & ((1u << lane) - 1));
       if (miss && r < found) {
-        *e = s.list[r];
-        refs[s.list[r]] = 1;
+        const int p = s.list[r];
+        if (copy) {
+          const int move = atomicAdd(&n_moves, 1);
+          s.src[move] = *e;
+          s.dst[move] = p;
+          atomicSub(&refs[*e], 1);
+        }
+        *e = p;
+        refs[p] = 1;
       }
       at += __popc(m);
     }
   }
+  __syncthreads();
   if (tid == 0) *s.n_moves = n_moves;
 }
 

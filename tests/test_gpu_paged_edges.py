@@ -249,3 +249,136 @@ def test_compact_with_a_table_of_nearly_2_31_entries():
     assert int((c.table >= 0).sum()) == 5
     del c
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("back", [0, 5, 16, 40])
+def test_reserve_replaces_every_shared_page_it_reaches(back):
+    """Rows that continue one row and are set back by hand (not by crop): all shared pages that the new positions reach
+    are replaced, and the rows that are not asked for keep what they hold."""
+    from domino_b200 import PagedKVCache
+
+    page, n = 16, 70
+    c = PagedKVCache(2, 4, 1, 40, 8, torch.float32, "cuda", page_size=page, row_pages=8)
+    c.reserve(torch.tensor([n, 0, 0, 0], device="cuda"))
+    k = torch.randn(4, n, 1, 8, device="cuda")
+    start = torch.zeros(4, dtype=torch.long, device="cuda")
+    lens = torch.tensor([n, 0, 0, 0], device="cuda")
+    for layer in range(2):
+        c.write(layer, None, k, k, None, start, lens)
+    c.length.copy_(lens)
+    c.fork(torch.zeros(4, dtype=torch.long, device="cuda"))
+    old = c.table.clone()
+    held = c.data.clone()
+    c.length[:3] = back                       # rows 0 .. 2 go back; row 3 keeps all of it
+    upto = torch.tensor([n, n, back + 20, 0], device="cuda")
+    c.reserve(upto)
+    assert c.status() == 0
+    assert torch.equal(c.table[3], old[3])
+    first, table = back // page, c.table.tolist()
+    for b, up in ((0, n), (1, n), (2, back + 20)):
+        own = table[b][first: -(-up // page)]
+        assert all(c.refs[p] == 1 for p in own) and -1 not in own
+        assert table[b][:first] == old[0, :first].tolist()
+        for i in range(first, -(-up // page)):  # copies of what was there
+            if i < 5:
+                assert torch.equal(c.data[:, :, table[b][i]], held[:, :, int(old[0, i])])
+    assert int(c.refs.sum()) == int((c.table >= 0).sum())
+    new = torch.randn(4, n, 1, 8, device="cuda")
+    m = torch.where(torch.arange(4, device="cuda") < 3, upto - back, 0)
+    st = torch.where(torch.arange(4, device="cuda") < 3, back, 0)
+    c.write(1, None, new, new, None, st, m)
+    assert c.status() == 0
+    for i in range(5):
+        assert torch.equal(c.data[:, :, int(old[3, i])], held[:, :, int(old[3, i])])
+    for b in range(3):
+        pos = torch.arange(back, int(upto[b]))
+        got = c.data[1, 0, c.table[b].cpu().long()[pos // page].cuda(), 0, (pos % page).cuda()]
+        assert torch.equal(got, new[b, : len(pos), 0])
+
+
+def test_reserve_lets_the_first_row_keep_pages_that_only_reaching_rows_hold():
+    """Three rows share five pages, all are set back and all reach them: the first keeps the originals, the others copy;
+    a pool that is too small leaves out the last requests and says so."""
+    from domino_b200 import PagedKVCache, _lib
+
+    for pages, ok in ((15, True), (12, False)):
+        c = PagedKVCache(1, 3, 1, pages, 8, torch.float32, "cuda", page_size=16, row_pages=5)
+        c.reserve(torch.tensor([80, 0, 0], device="cuda"))
+        c.length.copy_(torch.tensor([80, 0, 0]))
+        c.fork(torch.zeros(3, dtype=torch.long, device="cuda"))
+        c.length.zero_()
+        c.reserve(torch.full((3,), 80, device="cuda"))
+        assert c.status() == (0 if ok else _lib.DD_STATUS_NO_PAGE)
+        table = c.table.tolist()
+        assert table[0] == [0, 1, 2, 3, 4] and table[1] == [5, 6, 7, 8, 9]
+        assert table[2] == ([10, 11, 12, 13, 14] if ok else [10, 11, 2, 3, 4])
+        assert c.refs.tolist() == ([1] * 15 if ok else [1, 1, 2, 2, 2] + [1] * 7)
+
+
+class _AllSlots(R.HostPages):
+    """The host model with the sharing rule for every slot that a row reaches."""
+
+    def reserve(self, upto):
+        cap = self.row_pages * self.page
+        reach = [(b, i) for b, u in enumerate(upto) if min(u, cap) > self.length[b]
+                 for i in range(self.length[b] // self.page, math.ceil(min(u, cap) / self.page))]
+        by_page = {}
+        for b, i in reach:
+            by_page.setdefault(self.table[b][i], []).append(b)
+        want = []
+        for b, i in reach:
+            p = self.table[b][i]
+            if p < 0:
+                want.append((b, i, -1))
+            elif self.refs[p] > 1 and (self.refs[p] > len(by_page[p]) or by_page[p][0] < b):
+                want.append((b, i, p))
+        free = self._free()
+        for (b, i, old), new in zip(want, free):
+            if old >= 0:
+                self.refs[old] -= 1
+                self.content[new] = self.content[old]
+            self.table[b][i] = new
+            self.refs[new] = 1
+        return len(want) <= len(free) and all(u <= cap for u in upto)
+
+
+@pytest.mark.parametrize("seed,batch,pages,page,row_pages", [(0, 4, 60, 16, 6), (1, 33, 400, 32, 9), (3, 7, 30, 64, 8),
+                                                             (4, 300, 3000, 16, 40)])
+def test_random_sequences_with_lengths_set_back_by_hand(seed, batch, pages, page, row_pages):
+    """Random reserve / advance / fork / crop / lengths set back: tables, counts and contents as the host model's."""
+    import random
+
+    from domino_b200 import PagedKVCache, _lib
+    from tests.test_gpu_paged import _same, _stamp
+
+    rng = random.Random(seed)
+    c = PagedKVCache(2, batch, 2, pages, 8, torch.float32, "cuda", page_size=page, row_pages=row_pages)
+    h = _AllSlots(batch, pages, page, row_pages)
+    c.data.copy_(torch.arange(-pages, 0).view(1, 1, pages, 1, 1, 1).expand_as(c.data))
+    for step in range(40):
+        op = rng.choice(["grow", "grow", "back", "fork", "crop"])
+        if op == "grow":
+            upto = [max(0, n + rng.choice([0, 1, page, 3 * page + 1, -5])) for n in h.length]
+            c.reserve(torch.tensor(upto, device="cuda"))
+            ok = h.reserve(upto)
+            assert c.status() == (0 if ok else _lib.DD_STATUS_NO_PAGE)
+            _same(c, h, step)
+            for b in range(batch):
+                n = h.length[b]
+                while n < upto[b] and n < row_pages * page and h.table[b][n // page] >= 0 and h.refs[h.table[b][n // page]] == 1:
+                    n += 1
+                h.length[b] = n
+            c.length.copy_(torch.tensor(h.length))
+            _stamp(c, h, range(min(batch, 40)))
+        elif op == "back":
+            h.length = [rng.choice([n, n, n // 2, max(0, n - page)]) for n in h.length]
+            c.length.copy_(torch.tensor(h.length))
+        elif op == "crop":
+            to = [max(-1, n - rng.choice([0, 0, 1, page, -9])) for n in h.length]
+            c.crop(torch.tensor(to, device="cuda"))
+            h.crop(to)
+        else:
+            src = [rng.choice([b, b, b, -1, rng.randrange(batch), 0]) for b in range(batch)]
+            c.fork(torch.tensor(src, device="cuda"))
+            h.fork(src)
+        _same(c, h, step)
