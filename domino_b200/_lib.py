@@ -27,6 +27,13 @@ DD_STATUS_NO_ARGMAX = 4
 DD_STATUS_NO_PAGE = 8
 DD_STATUS_BAD_ROW = 16
 DD_STATUS_SHARED_PAGE = 32
+
+
+def status_names(bits: int) -> str:
+    """The names of the DD_STATUS_* bits that are set."""
+    return " | ".join(n for n, v in globals().items() if n.startswith("DD_STATUS_") and bits & v)
+
+
 # dd_set_middle kinds (include/domino_draft.h)
 DD_MIDDLE_SILU, DD_MIDDLE_IDENTITY, DD_MIDDLE_RELU, DD_MIDDLE_GELU = 0, 1, 2, 3
 DD_MIDDLE_GELU_TANH, DD_MIDDLE_TANH, DD_MIDDLE_SIGMOID, DD_MIDDLE_SILU_ROUNDED = 4, 5, 6, 7

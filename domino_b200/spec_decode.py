@@ -27,6 +27,7 @@ from typing import List, Optional, Sequence
 
 import torch
 
+from ._lib import DominoDraftError, status_names
 from .stack import DFlashBackbone, TargetLM
 
 
@@ -93,7 +94,9 @@ def spec_generate(draft: DFlashBackbone, target: TargetLM, runner, prompts: Sequ
     models' keys and values in paged caches, whose writes and attention run in
     the library's kernels; pages behind the accepted tokens go back after every
     block.  ``share_prefix`` (paged only) prefills the tokens that all prompts
-    begin with once and lets the rows share their pages.
+    begin with once and lets the rows share their pages.  A paged cache that
+    could not do a part of its work on the way raises ``DominoDraftError`` at
+    the end, instead of ids that were computed without that part.
     """
     cfg = draft.cfg
     dev = target.lm_head.weight.device
@@ -229,6 +232,10 @@ def spec_generate(draft: DFlashBackbone, target: TargetLM, runner, prompts: Sequ
                 verify_half()
     t1.record()
     t1.synchronize()
+    for name, cache in (("target", tcache), ("drafter", dcache)) if page_size else ():
+        bits = cache.status()
+        if bits:
+            raise DominoDraftError(f"spec_generate: the {name}'s cache reports {status_names(bits)}")
     log = acc_log[:blocks].tolist()
     accs = [[row[b] for row in log if row[b] > 0] for b in range(B)]
     outs, n_out = [], []

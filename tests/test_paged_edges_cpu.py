@@ -1,9 +1,13 @@
-"""Calls of the paged cache that are refused for their size, without a GPU."""
+"""The paged cache without a GPU: calls refused for their size, and what the block loop does with its caches' errors."""
 import ctypes
 
+import numpy as np
 import pytest
+import torch
 
+from tests.fixtures import LOOP_CASES, load_loop
 from tests.test_paged_cpu import full, lib  # noqa: F401 (a fixture)
+from tests.test_spec_loop_cpu import OracleRunner
 
 
 @pytest.mark.parametrize("heads,dim,ok", [(1 << 23, 256, False), (1 << 24, 256, False), ((1 << 28) - 1, 8, True),
@@ -19,3 +23,45 @@ def test_write_refuses_tokens_of_2_31_query_values(lib, heads, dim, ok):  # noqa
     rc = lib.dd_cache_write(ctypes.byref(c), ctypes.byref(a), None)
     assert rc < 0 and (rc == _lib.DD_EINVAL) != ok
     assert (b"chunk too large" in lib.dd_last_error(None)) != ok
+
+
+@pytest.mark.parametrize("bits,who,name", [((8, 0), "target", "DD_STATUS_NO_PAGE"), ((0, 33), "drafter", "DD_STATUS_TIMEOUT"),
+                                           ((0, 33), "drafter", "DD_STATUS_SHARED_PAGE"), ((0, 0), None, None)])
+def test_the_loop_raises_what_its_paged_caches_report(bits, who, name):
+    """Status bits of the caches that the loop makes come out as an error, not as tokens."""
+    from domino_b200 import DominoDraftError
+    from domino_b200.spec_decode import spec_generate
+    from domino_b200.stack import RaggedKVCache
+
+    class Cache(RaggedKVCache):  # the padded cache with a paged one's two calls
+        reads = 0
+
+        def crop(self, length):
+            self.length.copy_(torch.minimum(self.length, length))
+
+        def status(self):
+            self.reads += 1
+            return self.bits
+
+    c = load_loop(LOOP_CASES[0])
+    draft, target = c["draft"], c["target"]
+    made = []
+    for model, b in ((target, bits[0]), (draft, bits[1])):
+        def new_cache(batch, capacity, page_size=0, model=model, b=b):
+            assert page_size == 16
+            cfg = model.cfg
+            cache = Cache(cfg.num_hidden_layers, batch, cfg.num_key_value_heads, capacity, cfg.head_dim,
+                          next(model.parameters()).dtype, "cpu")
+            cache.bits = b
+            made.append(cache)
+            return cache
+
+        model.new_cache = new_cache
+    runner = OracleRunner(draft, target, 1, draft.cfg.pure_draft_prefix_len)
+    go = lambda: spec_generate(draft, target, runner, c["prompts"][:1], c["max_new_tokens"], page_size=16)  # noqa: E731
+    if who:
+        with pytest.raises(DominoDraftError, match=f"{who}.*{name}"):
+            go()
+    else:
+        assert np.array_equal(go().output_ids[0].numpy(), c["outputs"][0])
+        assert [x.reads for x in made] == [1, 1]
