@@ -4,10 +4,10 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
-#include <cstdlib>
 #include <cstdio>
-#include <mutex>
+#include <cstdlib>
 #include <type_traits>
 
 #include "../../include/domino_draft.h"
@@ -48,16 +48,21 @@ struct DeviceScope {
 struct DeviceInfo {
   int sms = 0, major = 0;
 };
-// Properties of a device, read once.
+// Properties of a device, read once and kept in one word: another thread sees both or neither.
+constexpr int kMaxDevices = 64;
 int device_info(int device, DeviceInfo* out) {
-  static DeviceInfo known[64];
-  if (device < 0 || device >= 64) return global_fail(DD_EINVAL, "device %d", device);
-  DeviceInfo d = known[device];
-  if (!d.sms) {
+  static std::atomic<int> known[kMaxDevices];  // SMs, and the major version above them
+  if (device < 0 || device >= kMaxDevices) return global_fail(DD_EINVAL, "device %d", device);
+  DeviceInfo d;
+  int word = known[device].load(std::memory_order_relaxed);
+  if (!word) {
     DD_TRY(cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, device));
     DD_TRY(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
-    known[device] = d;
+    word = d.major << 16 | d.sms;
+    known[device].store(word, std::memory_order_relaxed);
   }
+  d.major = word >> 16;
+  d.sms = word & 0xffff;
   if (d.major != 10) return global_fail(DD_EUNSUPPORTED, "device %d is not sm_100; this library is built for sm_100a", device);
   *out = d;
   return DD_OK;
@@ -266,7 +271,7 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, Att
   int rc = encode_pool(c, args->layer, 0, &mk);
   if (!rc) rc = encode_pool(c, args->layer, 1, &mv);
   if (rc) return rc;
-  static bool ready[64];
+  static std::atomic<bool> ready[kMaxDevices];
   if (!ready[c->device]) {
     DD_TRY(cudaFuncSetAttribute(attend_tc_kernel<T, kDim, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttSmem));
     ready[c->device] = true;
@@ -286,7 +291,7 @@ int launch_attend(const dd_paged_cache* c, const dd_cache_attend_args* args, Att
 template <typename T, int kDim, int kR>
 int launch_attend_f32(const dd_paged_cache* c, AttendParams p, const DeviceInfo& dev, void* stream) {
   using Shape = F32Shape<kDim, kR>;
-  static bool ready[64];
+  static std::atomic<bool> ready[kMaxDevices];
   if (!ready[c->device]) {
     DD_TRY(cudaFuncSetAttribute(attend_f32_kernel<T, kDim, kR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem));
     ready[c->device] = true;

@@ -382,3 +382,52 @@ def test_random_sequences_with_lengths_set_back_by_hand(seed, batch, pages, page
             c.fork(torch.tensor(src, device="cuda"))
             h.fork(src)
         _same(c, h, step)
+
+
+def threads_with_caches_of_their_own():
+    """The first calls of a process come from several threads at once, each on a cache and a stream of its own."""
+    import threading
+
+    from domino_b200 import PagedKVCache, Rope
+
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(2, 20, h, 64, generator=g).to(torch.bfloat16).cuda() for h in (4, 2, 2))
+    start = torch.zeros(2, dtype=torch.long, device="cuda")
+    rope = Rope(64, device="cuda")
+    gate, results, errors = threading.Barrier(8), [None] * 8, []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            c = PagedKVCache(1, 2, 2, 8, 64, torch.bfloat16, "cuda", page_size=16, row_pages=4)
+            torch.cuda.synchronize()
+            gate.wait()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    c.reserve(start + 20)
+                    out = c.attend(0, c.write(0, q, k, v, rope, start), start)
+                    c.crop(start)
+            stream.synchronize()
+            assert c.status() == 0
+            results[i] = out
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert all(torch.equal(results[0], r) for r in results[1:])
+
+
+def test_first_calls_of_several_threads():
+    """In a process of its own, where nothing has been called before."""
+    import subprocess
+    import sys
+
+    code = "from tests.test_gpu_paged_edges import threads_with_caches_of_their_own as go; go()"
+    for _ in range(2):
+        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
