@@ -321,7 +321,8 @@ class PagedKVCache:
         self._check(self._lib.dd_pages_compact(self._cp, self._stream()), "dd_pages_compact")
 
     def status(self) -> int:
-        """Synchronise and return (and clear) the ``DD_STATUS_*`` bits that calls have set."""
+        """Synchronise and return (and clear) the ``DD_STATUS_*`` bits that calls have set, on whatever stream they ran."""
+        torch.cuda.synchronize(self.device)
         s = int(self._status.item())
         self._status.zero_()
         if s & _lib.DD_STATUS_TIMEOUT:  # an attention gave up half-way: its counters start anew

@@ -431,3 +431,19 @@ def test_first_calls_of_several_threads():
     for _ in range(2):
         r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
         assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_status_sees_calls_on_other_streams():
+    """A call that is still waiting on a stream of its own when the status is read from another."""
+    from domino_b200 import PagedKVCache, _lib
+
+    c = PagedKVCache(1, 1, 1, 2, 8, torch.float32, "cuda", page_size=16)
+    x = torch.ones(1, 1, 1, 8, device="cuda")
+    start = torch.zeros(1, dtype=torch.long, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # about 50 ms
+        c.write(0, None, x, x, None, start)  # no page
+    assert c.status() == _lib.DD_STATUS_NO_PAGE
+    assert c.status() == 0
