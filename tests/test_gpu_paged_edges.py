@@ -441,7 +441,8 @@ def test_status_sees_calls_on_other_streams():
     x = torch.ones(1, 1, 1, 8, device="cuda")
     start = torch.zeros(1, dtype=torch.long, device="cuda")
     side = torch.cuda.Stream()
-    torch.cuda.synchronize()
+    c.write(0, None, x, x, None, start)  # (a kernel's first launch may wait for the device)
+    assert c.status() == _lib.DD_STATUS_NO_PAGE
     with torch.cuda.stream(side):
         torch.cuda._sleep(100_000_000)  # about 50 ms
         c.write(0, None, x, x, None, start)  # no page
