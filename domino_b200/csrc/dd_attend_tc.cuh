@@ -36,6 +36,9 @@
 // pieces, streams and copies of a row that took different maxima differ by
 // exact powers of two, so that rounding is the same wherever a row's keys are
 // cut, and what else shares the batch changes a result by fp32 sums alone.
+// (With m the maximum itself, the largest weight was 1 and had no rounding; now
+// it counts in l as it was rounded.  That leaves errors of 1.15 to 1.3 times a
+// result's own rounding where few or many keys matter; without, 1.4 to 1.7.)
 //
 // A masked key has weight 0, and 0 times a NaN is NaN in a matrix product.
 // So the values of keys that no row of the item sees are set to zero in
@@ -521,8 +524,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
       }
       const SeenByAll all = seen_by_all(a, p);
-      float m = -INFINITY, m_limit = -INFINITY, l = 0.0f;  // m_limit: the score, unscaled, beyond which m moves
-      bool have_o = false;
+      float m = -INFINITY, l = 0.0f;
+      bool have_o = false, far = false;  // far: a row of the warp has m of 2^20 or more
       constexpr int kStep = kPair ? 1 : 2;
       int page = (kPair ? 0 : s) < n ? group_page(a, p.b, p.span.tile(p.i0 + (kPair ? 0 : s)), lane) : 0;
       if (!kPair && pending) {  // the last piece's O, maxima and flags have been read by all
@@ -535,7 +538,7 @@ __global__ void __launch_bounds__(kAttThreads, 1)
         // 16-key groups without a page (read one tile ahead)
         const unsigned missing = __ballot_sync(0xffffffffu, lane < 8 && (page < 0 || page >= a.pages));
         if (i + kStep < n) page = group_page(a, p.b, p.span.tile(p.i0 + i + kStep), lane);
-#pragma unroll 1
+#pragma unroll
         for (int part = 0; part < Shape::kParts; ++part, ++n_part) {
           const int key0 = tile * kKeyTile, part0 = key0 + part * kPartKeys, part1 = part0 + kPartKeys;
           const bool whole = missing == 0 && part1 <= all.hi && (part0 >= all.lo || part1 <= a.sinks);
@@ -574,14 +577,14 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             }
             const float mt = max3_nan(top[0], top[1], top[1]);
             if (!(mt < INFINITY)) l = __int_as_float(0x7fc00000);  // a NaN or +infinity among the scores: the row is NaN
-            const bool moves = mt > m_limit;
+            const float mt2 = __fmul_rn(mt, sl);
+            const bool moves = mt2 - m > 8.0f;
             if (__any_sync(0xffffffffu, moves)) {
-              const float mt2 = __fmul_rn(mt, sl), m1 = moves ? ceilf(mt2) : m;
+              const float m1 = moves ? ceilf(mt2) : m;
               const float keep = moves ? exp2_approx(m - m1) : 1.0f;
-              // (past 2^20 fp32's steps are not small beside 8: every larger score moves m)
-              if (moves) m_limit = fabsf(mt2) < 1048576.0f ? mt + 8.0f / sl : mt;
               l *= keep;
               m = m1;
+              far = __any_sync(0xffffffffu, fabsf(m) >= 1048576.0f && m != -INFINITY);
               if (have_o) {
                 // (the scores of part k come after the products of part k - 2; those of k - 1 may still run)
                 if (Shape::kParts > 1) ok = mbar_wait_bounded(&bar.pv_done[s], (n_part - 1) & 1, abort);
@@ -600,19 +603,23 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             have_o = true;
             const float sub = (m == -INFINITY ? 0.0f : m) - kTopExponent;
             uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
-            const uint64_t sub2 = pack_f32x2(-sub, -sub);
+            // With m of 2^20 and more scores are scaled and rounded before m is taken off, as in m, so that none comes out above
+            // its maximum (in one step those of 2^29 came out up to 2^5 beside it: infinite weights in fp16).
+            const float sl1 = far ? 1.0f : sl;
+            const uint64_t sl2 = pack_f32x2(sl1, sl1), sub2 = pack_f32x2(-sub, -sub);
 #pragma unroll 1
             for (int c = chunk_a; c < chunk_b; c += kCols) {
               if (chunk_b - chunk_a > kCols) fetch(c);
+              if (far)
+#pragma unroll
+                for (int k = 0; k < 32 * kCols; ++k) x[k] = __float_as_uint(__fmul_rn(__uint_as_float(x[k]), sl));
 #pragma unroll
               for (int d = 0; d < kCols; ++d) {
                 uint32_t w[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                   const float x0 = __uint_as_float(x[32 * d + 2 * k]), x1 = __uint_as_float(x[32 * d + 2 * k + 1]);
-                  // scaled and rounded before m is taken off, as in m, so that no score comes out above its maximum
-                  // (a product and a sum in one step put scores of 2^29 up to 2^5 beside it: infinite weights in fp16)
-                  const uint64_t e = add_f32x2(pack_f32x2(__fmul_rn(x0, sl), __fmul_rn(x1, sl)), sub2);
+                  const uint64_t e = fma_f32x2(pack_f32x2(x0, x1), sl2, sub2);
                   float e0, e1;
                   unpack_f32x2(e, e0, e1);
                   const float p0 = exp2_approx(e0), p1 = exp2_approx(e1);
@@ -625,7 +632,9 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             }
             float sum0, sum1;
             unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), sum0, sum1);
-            l += sum0 + sum1;
+            // the part's largest weight counts as it was rounded: one that takes everything gives its value as it is
+            const float top_w = exp2_approx(far ? mt2 - sub : fmaf(mt, sl, -sub));
+            l += sum0 + sum1 + (io<T>::to_f(io<T>::from_f(top_w)) - top_w);
             tmem_st_wait();
           }
           if (!whole && (!kPair || s == 0)) {  // (pairs: the other stream's products of a part come after this one's)

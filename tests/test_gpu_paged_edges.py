@@ -448,3 +448,39 @@ def test_status_sees_calls_on_other_streams():
         c.write(0, None, x, x, None, start)  # no page
     assert c.status() == _lib.DD_STATUS_NO_PAGE
     assert c.status() == 0
+
+
+@pytest.mark.parametrize("tokens,heads,dim", [(1, 4, 128), (7, 4, 64), (16, 4, 128), (33, 3, 96), (50, 4, 128), (300, 1, 64)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_query_that_sees_one_key_gives_its_value(tokens, heads, dim, dtype):
+    """Bit for bit: a weight's rounding is part of the row's sum too.  (P v is exact in fp32, 1 / P and the product are
+    within 2^-22 of v, and v is the nearest number of its type; in fp32 itself the weight is 1.)"""
+    past = 200
+    c, g = make(1, 2, dim, dtype, 32, [past + tokens], seed=tokens)
+    keys, values = fill(c, [past + tokens], g)
+    q = torch.randn(1, tokens, 2 * heads, dim, generator=g).to(dtype).cuda()
+    out = c.attend(0, q, torch.tensor([past], device="cuda"), window=1)
+    want = values[0][:, past:].transpose(0, 1).repeat_interleave(heads, dim=1)
+    assert torch.equal(out[0].cpu(), want)
+
+
+@pytest.mark.parametrize("tokens,past", [(16, 0), (16, 130), (1, 90), (64, 0), (200, 0), (64, 500)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_errors_against_a_result_rounded_once(tokens, past, dtype):
+    """The 2-norm of the error in 64 bits against that of rounding the exact result alone.
+
+    A row's weights w_i (sum 1) carry independent roundings d_i, at most half a step u relative and u / sqrt(3) in the mean
+    square, and the largest counts as it was rounded: the result moves by sum w_i d_i v_i less the largest's part along the
+    result itself, at most u / sqrt(3) * sqrt(sum w_i^2) |v| in the mean square, while |o| is sqrt(sum w_i^2) |v| for
+    independent values.  The result's own rounding is u / sqrt(3) to u / (2 sqrt(3)) of |o| between the ends of a binade,
+    about u / sqrt(3) * 0.72 over all of one, and the weights' the same 0.72: together sqrt(2) of the rounding alone."""
+    kv, heads, dim = 2, 8, 64
+    total = [past + tokens] * 6
+    c, g = make(6, kv, dim, dtype, 64, total, seed=past)
+    keys, values = fill(c, total, g)
+    q = 2 * torch.randn(6, tokens, heads, dim, generator=g).to(dtype)
+    out = c.attend(0, q.cuda(), torch.full((6,), past, device="cuda")).double().cpu()
+    ref = R.attend(q, keys, values, [torch.ones(n, dtype=torch.bool) for n in total], [past] * 6, [tokens] * 6, True, 0, 0,
+                   dim ** -0.5)
+    err, own = (out - ref).norm(), (ref.to(dtype).double() - ref).norm()
+    assert err <= 2 ** 0.5 * own, (err / own).item()
