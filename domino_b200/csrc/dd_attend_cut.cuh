@@ -72,6 +72,9 @@ struct Piece {
 // (Start and end cost about as much as seven tiles: with 3 / 5 / 7 / 10 the calls
 // of 64 rows x 1 token took 210 / 198 / 198 / 199 us, of 32 rows x 16 tokens 265
 // / 262 / 254 / 253 us; with none, short rows' CTAs ran twice as long as others.)
+// (Own CTAs up to a quarter of the CTAs: with a half, 5 x 16 tokens over 2560 keys,
+// 40 items, took 26.2 us against 23.8, 8 x 1 token over 8000, 64 items, 67.7 against
+// 52.2; with an eighth, 4 x 16 over 2560, 32 items, 23.6 against 22.7.)
 constexpr int kItemUnits = 7;
 __device__ __forceinline__ void piece_enter(const AttendParams& a, Piece& p, int q_tiles, int tile_rows) {
   p.b = p.e / q_tiles;

@@ -297,6 +297,8 @@ int launch_attend_f32(const dd_paged_cache* c, AttendParams p, const DeviceInfo&
     ready[c->device] = true;
   }
   p.item_rows = p.tile_rows = Shape::kRows;
+  // a tile takes longer here: with at least 1 / 2 / 3 of them a CTA 1 x 1 token over 528 keys takes 10.2 / 18.0 / 24.3
+  // us, 3 x 16 over 1000 22.4 / 23.9 / 39.6 (16 / 4 heads of 64)
   p.min_tiles = 1;
   // two CTAs fit an SM with heads of up to 64 values
   const int grid = std::min(dev.sms * (kDim <= 64 ? 2 : 1), kMaxAttendCtas);
@@ -507,7 +509,16 @@ int dd_cache_attend(const dd_paged_cache* c, const dd_cache_attend_args* a, void
   p.status = c->status;
   const AttendPlan plan = attend_plan(c, a);
   const long long rows = (long long)a->tokens * p.group;
+  // Copies of the rows in a tile, so that all softmax warps have work, up to the
+  // tile's 128 rows (32 / 8 heads of 128, bf16).  4 rows (1 x 1 token over 528 /
+  // 4000 keys): 13.4 / 18.3 us with 4 copies, 13.9 / 18.9 with 2, 15.8 / 20.4
+  // with 1; 16 rows (2 x 4 tokens over 2560): 18.8, 19.5, 20.8; 64 rows (2 x 16
+  // and 8 x 16 tokens over 2560 and 2048): 21.4 and 26.0 us with 2, 22.5 and 28.9 with 1.
   p.copies = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+  // What a CTA more brings a small call against one piece more to join.  With at
+  // least 1 / 2 / 3 / 5 tiles a CTA 1 x 1 token over 528 keys takes 14.1 / 14.6 /
+  // 13.4 / 13.4 us, 2 x 16 tokens over 512 keys 17.2 / 18.1 / 16.4 / 16.5, over
+  // 2560 keys 21.0 / 21.0 / 21.4 / 22.0.
   p.min_tiles = 3;
   if (plan.tensor) {
     if (c->dtype == DD_FP16) return launch_attend<__half>(c, a, plan, p, dev, stream);
