@@ -274,8 +274,9 @@ class PagedKVCache:
         q [batch, tokens, heads, head_dim] (any strides with a contiguous last dimension; ``heads`` a multiple of
         ``kv_heads``).  Query t of row b, t < ``lens[b]``, has position p = ``start[b] + t`` and sees the keys j <
         ``start[b] + lens[b]`` that have a page: with ``causal`` those up to p, and with ``window`` > 0 of these only
-        ``p - j < window`` or ``j < sinks``.  ``scale`` defaults to ``head_dim ** -0.5``.  A query that sees no key
-        gives zeros, as do the rows behind ``lens[b]``; what a query does not see has no effect on it.
+        ``p - j < window`` or ``j < sinks``.  ``scale`` (positive) defaults to ``head_dim ** -0.5``.  A query that sees
+        no key, or none with a score above -infinity, gives zeros, as do the rows behind ``lens[b]``.  What a query does
+        not see has no effect on it; an infinite or NaN value that it sees makes that element infinite or NaN.
         """
         q = self._heads(q, "q", None, None)
         _, tokens, heads, _ = q.shape

@@ -365,12 +365,13 @@ int dd_cache_write(const dd_paged_cache* c, const dd_cache_write_args* a, void* 
  * t < lens[b], has position p = start[b] + t and sees the keys j < start[b] +
  * lens[b] that have a page, with j <= p if `causal`, and with `window` > 0
  * (causal only) p - j < window or j < sinks:
- *   out = sum_j softmax_j(scale q . K[j]) V[j]
+ *   out = sum_j softmax_j(scale q . K[j]) V[j],  scale > 0
  * Query heads h * heads / kv_heads ... share key head h.  A query that sees no
- * key, and every t >= lens[b], gives zeros.  Keys that a query does not see
- * have no effect on it, whatever they hold; an infinite or NaN value that it
- * does see makes that element of its result infinite or NaN.  start[b] outside +-2^30 counts as
- * that bound.  bf16 / fp16 heads of up to 128 values run on the tensor cores. */
+ * key (or none with a score above -infinity), and every t >= lens[b], gives
+ * zeros.  Keys that a query does not see have no effect on it, whatever they
+ * hold; an infinite or NaN value that it does see makes that element of its
+ * result infinite or NaN.  start[b] outside +-2^30 counts as that bound.  bf16 /
+ * fp16 heads of up to 128 values run on the tensor cores. */
 typedef struct dd_cache_attend_args {
   const void* q;
   void* out;                  /* [batch, tokens, heads, head_dim] */

@@ -484,3 +484,23 @@ def test_errors_against_a_result_rounded_once(tokens, past, dtype):
                    dim ** -0.5)
     err, own = (out - ref).norm(), (ref.to(dtype).double() - ref).norm()
     assert err <= 2 ** 0.5 * own, (err / own).item()
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 50])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_of_minus_infinity(tokens, dtype):
+    """Keys whose score is -infinity have no weight beside others, and give zeros where there is no other."""
+    past = 150
+    c, g = make(1, 1, 64, dtype, 16, [past + tokens], seed=3)
+    keys, values = fill(c, [past + tokens], g)
+    q = (1 + torch.rand(1, tokens, 4, 64, generator=g)).to(dtype).cuda()
+    start = torch.tensor([past], device="cuda")
+    pages = c.table[0, : -(-(past + tokens) // 16)].long()
+    keep = c.data[0, 0].clone()
+    c.data[0, 0, :, :, :, 0] = -math.inf
+    assert (c.attend(0, q, start) == 0).all()
+    c.data[0, 0] = keep
+    c.data[0, 0, pages[3], 0, 5, 0] = -math.inf  # position 53 alone
+    seen = torch.ones(past + tokens, dtype=torch.bool)
+    seen[53] = False
+    check_attend(c, c.attend(0, q, start), q, keys, values, [past], [tokens], seen=[seen])
