@@ -26,28 +26,33 @@
 //
 // The running maximum m moves only when a row's scores pass it by more than 8
 // (as powers of two): P then stays below 2^8 and the rescaling of O, a round
-// trip through TMEM, is rare.  In fp16, where weights below 2^-14 would lose
-// bits and those below 2^-25 vanish (from O, not from l: a long even tail under
-// one large weight), P and l are 2^7 times as large: P then stays below 2^15.3,
-// and what loses bits is below 2^-21.  (O is fp32 all the same: of products
-// below 2^-25 of it the tensor cores add nothing.)  m, l, S and O are fp32; P is rounded to
-// the cache's type, the one rounding besides the result's (its error is that of
-// one rounding of each weight).  m is a whole number, the maximum rounded up:
-// pieces, streams and copies of a row that took different maxima differ by
-// exact powers of two, so that rounding is the same wherever a row's keys are
-// cut, and what else shares the batch changes a result by fp32 sums alone.
-// (With m the maximum itself, the largest weight was 1 and had no rounding; now
-// it counts in l as it was rounded.  That leaves errors of 1.15 to 1.3 times a
-// result's own rounding where few or many keys matter; without, 1.4 to 1.7.)
+// trip through TMEM, is rare.  m, l, S and O are fp32; P is rounded to the
+// cache's type, the one rounding besides the result's.
+//
+// In fp16, where weights below 2^-14 would lose bits and those below 2^-25
+// vanish (from O, not from l: a long even tail under one large weight), P and l
+// are 2^7 times as large: P then stays below 2^15.3, and what loses bits is
+// below 2^-21.  (O is fp32 all the same: of products below 2^-25 of it the
+// tensor cores add nothing.)
+//
+// m is a whole number, the maximum rounded up: pieces, streams and copies of a
+// row that took different maxima differ by exact powers of two, so that P's
+// rounding is the same wherever a row's keys are cut.  What else shares the
+// batch changes a row by the order of fp32 sums, and by the few weights that lie
+// on the border between two 16-bit numbers: 0.1-0.2 % of the results of 4096
+// keys in bf16, 0.4-1.5 % in fp16; 42-46 % with the maximum itself as m.  The
+// largest weight, which that made 1, is rounded now; it counts in l as it was
+// rounded.  That leaves errors of 1.15 to 1.3 times a result's own rounding;
+// without, 1.4 to 1.7 times.
 //
 // A masked key has weight 0, and 0 times a NaN is NaN in a matrix product.
 // So the values of keys that no row of the item sees are set to zero in
 // shared memory (pages behind the end, missing pages, the rest of a page).
 // Keys that only some rows see are searched for infinities and NaN, which are
 // set to zero too; where there was one, every row adds those that it sees to
-// its result (add_part_seen).  These keys are at most two for every
-// token of the item (behind its first token, and before its last one's
-// window), so that takes as long for a long row of keys as for a short one.
+// its result (add_part_seen).  These keys are at most two for every token of
+// the item (behind its first token, and before its last one's window), so that
+// takes as long for a long row of keys as for a short one.
 #pragma once
 
 #include "dd_attend_cut.cuh"
@@ -141,7 +146,8 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
   return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
 }
 
-// (Out of line: in line it cost the hot loop its registers, and 8192 tokens behind 8192 took 1930 us, so 1746.)
+// (Out of line: in line it cost the softmax loop its registers, and 8192 tokens
+// behind 8192 took 1930 us against 1746.)
 template <typename T>
 __device__ __noinline__ void clean16(uint4* at) {
   const uint4 w = *at;
@@ -603,8 +609,8 @@ __global__ void __launch_bounds__(kAttThreads, 1)
             have_o = true;
             const float sub = (m == -INFINITY ? 0.0f : m) - kTopExponent;
             uint64_t sum[4] = {0, 0, 0, 0};  // (two fp32 zeros each)
-            // With m of 2^20 and more scores are scaled and rounded before m is taken off, as in m, so that none comes out above
-            // its maximum (in one step those of 2^29 came out up to 2^5 beside it: infinite weights in fp16).
+            // With m of 2^20 and more scores are scaled and rounded before m is taken off, as in m, so that none comes
+            // out above its maximum (in one step those of 2^29 came out up to 2^5 beside it: infinite weights in fp16).
             const float sl1 = far ? 1.0f : sl;
             const uint64_t sl2 = pack_f32x2(sl1, sl1), sub2 = pack_f32x2(-sub, -sub);
 #pragma unroll 1
